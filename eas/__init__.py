@@ -13,7 +13,7 @@ import easy_as_b200 as _pkg
 
 for _name in ("ir", "mk", "meta", "autotune", "analysis", "compiler", "kernel", "tensor", "dlpack", "torch",
               "codegen", "codegen.cuda", "codegen.patterns", "runtime", "runtime.base", "runtime.grid",
-              "runtime.cuda", "runtime.cuda_ext", "shard"):
+              "runtime.cuda", "runtime.cuda_ext", "shard", "ops"):
     try:
         _mod = importlib.import_module(f"easy_as_b200.{_name}")
     except ModuleNotFoundError:

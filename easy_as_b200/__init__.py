@@ -5,11 +5,12 @@ Public API (same names as the reference package ``eas``):
 ``Tensor``, ``tensor``, ``empty``, ``empty_like``, ``from_dlpack``,
 ``to_dlpack``, ``from_torch``, ``to_torch``.  ``import eas`` resolves to this
 package (see the top-level ``eas`` shim), so existing kernels run unchanged.
+``ops`` (dense layers on native kernels) is this package's own.
 """
 
 from __future__ import annotations
 
-from . import mk  # noqa: F401
+from . import mk, ops  # noqa: F401
 from .autotune import Config, autotune
 from .dlpack import from_dlpack, to_dlpack
 from .kernel import Kernel, kernel
@@ -19,5 +20,5 @@ from .torch import from_torch, to_torch
 
 __all__ = [
     "Config", "Kernel", "Tensor", "autotune", "constexpr", "from_dlpack", "empty", "empty_like",
-    "from_torch", "kernel", "mk", "tensor", "to_dlpack", "to_torch",
+    "from_torch", "kernel", "mk", "ops", "tensor", "to_dlpack", "to_torch",
 ]

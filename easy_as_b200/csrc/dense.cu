@@ -1,0 +1,477 @@
+// dense.cu — the dense layers of a model as operators: a linear layer with bias, activation and
+// residual, a gated feed-forward block, and their backward passes (f16 or bf16, f32 sums).
+//
+//   linear            z = x W^T + b;  y = act(z) + r                      x [M,K], W [N,K], y [M,N]
+//   linear_backward   dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = sum_m dz
+//   gated             g = x Wg^T, u = x Wu^T;  h = act(g) u
+//   gated_backward    dg = dh u act'(g), du = dh act(g);  dx = dg Wg + du Wu;  dWg = dg^T x;  dWu = du^T x
+//
+// A backward pass is one pass over dy (act_grad_kernel: dz, and the column sums of db) and the two
+// products.  dz, dg and du are rounded to the operands' type there: they are operands of matrix
+// products, as x and W are, and that rounding is of the size of the one that dy itself had.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "dense_math.cuh"
+#include "eas_internal.h"
+
+namespace {
+
+using namespace dense;
+
+// C[m][n] = sum_t sum_k A_t[m][k] B_t[n][k], element strides for every operand
+struct Product {
+  const uint16_t* a[2];
+  const uint16_t* b[2];
+  int64_t a_m[2], a_k, b_n[2], b_k[2];
+  int M, N, K;
+  int terms;   // 1, or 2: two products summed
+  bool gated;  // one A, two B: the epilogue combines the two products
+  // epilogue
+  const uint16_t* bias;
+  const uint16_t* residual;
+  uint16_t* y;
+  uint16_t* pre;   // z (linear) or g (gated)
+  uint16_t* pre2;  // u (gated)
+  int64_t ldr, ldy, ldp, ldp2;
+  int act;
+  bool bf16;
+};
+
+constexpr int kT = 64, kTK = 16;
+
+// The plain tiled product: 64 x 64 outputs per block of 256 threads, 4 x 4 per thread, f32 FMAs.
+template <bool GATED>
+__global__ void __launch_bounds__(256) product_kernel(const Product p) {
+  __shared__ float sa[kTK][kT + 4];
+  __shared__ float sb[GATED ? 2 : 1][kTK][kT + 4];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int m0 = blockIdx.y * kT, n0 = blockIdx.x * kT;
+  float acc[GATED ? 2 : 1][4][4] = {};
+  const int terms = GATED ? 1 : p.terms;
+  for (int t = 0; t < terms; ++t) {
+    for (int k0 = 0; k0 < p.K; k0 += kTK) {
+      for (int i = threadIdx.x; i < kT * kTK; i += 256) {
+        int r, k;
+        if (p.a_k == 1) { k = i % kTK; r = i / kTK; } else { r = i % kT; k = i / kT; }
+        sa[k][r] = (m0 + r < p.M && k0 + k < p.K) ? to_f32(p.a[t][(m0 + r) * p.a_m[t] + (k0 + k) * p.a_k], p.bf16) : 0.0f;
+        if (p.b_k[0] == 1) { k = i % kTK; r = i / kTK; } else { r = i % kT; k = i / kT; }
+#pragma unroll
+        for (int h = 0; h < (GATED ? 2 : 1); ++h)
+          sb[h][k][r] = (n0 + r < p.N && k0 + k < p.K)
+                            ? to_f32(p.b[GATED ? h : t][(n0 + r) * p.b_n[GATED ? h : t] + (k0 + k) * p.b_k[GATED ? h : t]], p.bf16) : 0.0f;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < kTK; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int h = 0; h < (GATED ? 2 : 1); ++h)
+              acc[h][i][j] = fmaf(sa[k][ty * 4 + i], sb[h][k][tx * 4 + j], acc[h][i][j]);
+      __syncthreads();
+    }
+  }
+  with_act(p.act, [&](auto a) {
+    for (int i = 0; i < 4; ++i)
+      for (int j = 0; j < 4; ++j) {
+        const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
+        if (m >= p.M || n >= p.N) continue;
+        float z = acc[0][i][j];
+        if (!GATED && p.bias) z += to_f32(p.bias[n], p.bf16);
+        if (p.pre) p.pre[m * p.ldp + n] = to_16(z, p.bf16);
+        float v = act<decltype(a)::value>(z);
+        if (GATED) {
+          const float u = acc[GATED ? 1 : 0][i][j];
+          if (p.pre2) p.pre2[m * p.ldp2 + n] = to_16(u, p.bf16);
+          v *= u;
+        } else if (p.residual) {
+          v += to_f32(p.residual[m * p.ldr + n], p.bf16);
+        }
+        p.y[m * p.ldy + n] = to_16(v, p.bf16);
+      }
+  });
+}
+
+int launch_product(const Product& p, cudaStream_t s, const char* who) {
+  const dim3 grid((p.N + kT - 1) / kT, (p.M + kT - 1) / kT);
+  if (p.gated)
+    product_kernel<true><<<grid, 256, 0, s>>>(p);
+  else
+    product_kernel<false><<<grid, 256, 0, s>>>(p);
+  return eas_cuda_check(cudaGetLastError(), who, EAS_ERR_LAUNCH);
+}
+
+// ---------------------------------------------------------------------------
+// the elementwise half of the backward pass
+// ---------------------------------------------------------------------------
+//
+// linear: dz = dy act'(z);  gated: dg = dh u act'(g), du = dh act(g).  One pass, 8 columns (16
+// bytes) per thread; a block covers 256 columns of kRowsPerBlock rows with 8 thread rows.  With
+// db, each thread keeps the f32 sums of its columns, the block adds its 8 thread rows in shared
+// memory and writes one row of partial sums, and colsum_kernel adds those in a fixed order: no
+// atomics, the same bits on every run.
+
+struct ActGrad {
+  const uint16_t* dy;
+  const uint16_t* g;
+  const uint16_t* u;
+  uint16_t* dg;     // dz, or dg; null when dz is dy itself (act none) and only db is wanted
+  uint16_t* du;
+  float* partial;   // [row blocks][N] sums of dz, or null
+  int64_t lddy, ldg, ldu, ldo;
+  int M, N, rows_per_block;
+  int act;
+  bool bf16;
+  bool v_dy, v_g, v_u, v_o;  // 16-byte accesses allowed
+};
+
+__device__ __forceinline__ void load8(const uint16_t* p, int n, bool vec, bool bf16, float (&v)[8]) {
+  if (vec && n >= 8) {
+    const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
+    unpack2(w.x, v[0], v[1], bf16);
+    unpack2(w.y, v[2], v[3], bf16);
+    unpack2(w.z, v[4], v[5], bf16);
+    unpack2(w.w, v[6], v[7], bf16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? to_f32(p[j], bf16) : 0.0f;
+  }
+}
+
+__device__ __forceinline__ void store8(uint16_t* p, int n, bool vec, bool bf16, const float (&v)[8]) {
+  if (vec && n >= 8) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack2(v[0], v[1], bf16), pack2(v[2], v[3], bf16),
+                                              pack2(v[4], v[5], bf16), pack2(v[6], v[7], bf16));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) p[j] = to_16(v[j], bf16);
+  }
+}
+
+template <bool GATED>
+__global__ void __launch_bounds__(256) act_grad_kernel(const ActGrad p) {
+  __shared__ float sums[8][32][9];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int n0 = (blockIdx.x * 32 + tx) * 8;
+  const int cols = p.N - n0;
+  const int64_t r0 = (int64_t)blockIdx.y * p.rows_per_block;
+  const int64_t r1 = min((int64_t)p.M, r0 + p.rows_per_block);
+  float sum[8] = {};
+  if (cols > 0) {
+    with_act(p.act, [&](auto a) {
+      constexpr int ACT = decltype(a)::value;
+      for (int64_t m = r0 + ty; m < r1; m += 8) {
+        float dy[8], g[8], u[8], o[8];
+        load8(p.dy + m * p.lddy + n0, cols, p.v_dy, p.bf16, dy);
+        if (GATED || ACT != kNone) load8(p.g + m * p.ldg + n0, cols, p.v_g, p.bf16, g);
+        if (GATED) {
+          float w[8];
+          load8(p.u + m * p.ldu + n0, cols, p.v_u, p.bf16, u);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float v, d;
+            act_and_slope<ACT>(g[j], v, d);
+            w[j] = dy[j] * u[j] * d;
+            o[j] = dy[j] * v;
+          }
+          store8(p.dg + m * p.ldo + n0, cols, p.v_o, p.bf16, w);
+          store8(p.du + m * p.ldo + n0, cols, p.v_o, p.bf16, o);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float v, d = 1.0f;
+            if (ACT != kNone) act_and_slope<ACT>(g[j], v, d);
+            o[j] = dy[j] * d;
+            sum[j] += o[j];
+          }
+          if (p.dg) store8(p.dg + m * p.ldo + n0, cols, p.v_o, p.bf16, o);
+        }
+      }
+    });
+  }
+  if (GATED || !p.partial) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sums[ty][tx][j] = sum[j];
+  __syncthreads();
+  const int c = threadIdx.x, n = blockIdx.x * 256 + c;  // one column per thread
+  float s = 0;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) s += sums[r][c >> 3][c & 7];
+  if (n < p.N) p.partial[(int64_t)blockIdx.y * p.N + n] = s;
+}
+
+// db[n] = the sum of the row blocks' partial sums, in order
+__global__ void __launch_bounds__(256) colsum_kernel(const float* __restrict__ partial, uint16_t* __restrict__ db,
+                                                     int blocks, int N, bool bf16) {
+  const int n = blockIdx.x * 256 + threadIdx.x;
+  if (n >= N) return;
+  float s = 0;
+  for (int b = 0; b < blocks; ++b) s += partial[(int64_t)b * N + n];
+  db[n] = to_16(s, bf16);
+}
+
+// Rows per block: enough blocks for 8 per SM, at least 8 rows (one per thread row), at most 64 row
+// blocks when sums are wanted (colsum_kernel reads them one after another).
+int rows_per_block(int M, int N) {
+  const int64_t col_blocks = (N + 255) / 256;
+  int64_t want = (8 * 148 + col_blocks - 1) / col_blocks;
+  if (want > 64) want = 64;
+  int64_t rows = ((int64_t)M + want - 1) / want;
+  rows = (rows + 7) / 8 * 8;
+  return (int)(rows < 8 ? 8 : rows);
+}
+
+bool vec_ok(const void* p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld & 7) == 0; }
+
+// Makes `dev` current for the scope of a call.
+struct DeviceScope {
+  int before = -1;
+  int rc = EAS_OK;
+  explicit DeviceScope(int dev) {
+    rc = eas_driver_init();
+    if (rc) return;
+    int cur = -1;
+    rc = eas_cuda_check(cudaGetDevice(&cur), "cudaGetDevice", EAS_ERR_UNAVAILABLE);
+    if (rc || cur == dev) return;
+    rc = eas_cuda_check(cudaSetDevice(dev), "cudaSetDevice", EAS_ERR_VALUE);
+    if (!rc) before = cur;
+  }
+  ~DeviceScope() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
+int check_sizes(const char* who, uint32_t M, uint32_t N, uint32_t K, int dtype, int act) {
+  if (dtype < 0 || dtype >= kTypes) return eas_fail(EAS_ERR_VALUE, "%s: dtype must be 0 (f16) or 1 (bf16)", who);
+  if (act < 0 || act >= kActs) return eas_fail(EAS_ERR_VALUE, "%s: unknown activation %d", who, act);
+  if (M > 0x7fffff00u || N > 0x7fffff00u || K > 0x7fffff00u)
+    return eas_fail(EAS_ERR_VALUE, "%s: a dimension exceeds 2^31 - 256", who);
+  if (N == 0 || K == 0) return eas_fail(EAS_ERR_VALUE, "%s: N and K must be positive", who);
+  return EAS_OK;
+}
+
+int zero_rows(void* p, uint64_t ld, uint32_t rows, uint32_t cols, cudaStream_t s, const char* who) {
+  return eas_cuda_check(cudaMemset2DAsync(p, ld * 2, 0, (size_t)cols * 2, rows, s), who, EAS_ERR_LAUNCH);
+}
+
+uint64_t round256(uint64_t b) { return (b + 255) / 256 * 256; }
+
+const uint16_t* u16(const void* p) { return static_cast<const uint16_t*>(p); }
+uint16_t* u16(void* p) { return static_cast<uint16_t*>(p); }
+
+// Which outputs a backward pass computes, and which operands TMA cannot read in place.
+enum { kDx = 1, kDw = 2, kDb = 4 };
+enum { kXOff = 1, kWOff = 2, kUpOff = 4, kDyOff = 8 };
+
+// Layout of the scratch of a backward pass: dz (or dg, du) in rows padded to 8 elements, then the
+// partial sums of db.
+struct Scratch {
+  uint64_t dz = 0, dz2 = 0, partial = 0, total = 0;
+  uint64_t ld = 0;
+  int rows = 0, blocks = 0;
+  bool need_dz = false;
+};
+
+uint64_t take(Scratch& s, uint64_t bytes) {
+  const uint64_t at = s.total;
+  s.total += round256(bytes);
+  return at;
+}
+
+Scratch backward_scratch(bool gated, uint32_t M, uint32_t N, uint32_t K, int act, int outputs, int off) {
+  Scratch s;
+  s.ld = ((uint64_t)N + 7) / 8 * 8;
+  s.rows = rows_per_block((int)M, (int)N);
+  s.blocks = (int)(((uint64_t)M + s.rows - 1) / s.rows);
+  s.need_dz = gated || act != kNone || ((off & kDyOff) && (outputs & (kDx | kDw)));
+  if (s.need_dz) s.dz = take(s, (uint64_t)M * s.ld * 2);
+  if (gated) s.dz2 = take(s, (uint64_t)M * s.ld * 2);
+  if (outputs & kDb) s.partial = take(s, (uint64_t)s.blocks * N * 4);
+  return s;
+}
+
+Scratch forward_scratch(bool gated, uint32_t M, uint32_t N, uint32_t K, int off) { return Scratch(); }
+
+int check_scratch(const char* who, const Scratch& s, const void* p, uint64_t bytes) {
+  if (s.total && (!p || bytes < s.total || (reinterpret_cast<uintptr_t>(p) & 255)))
+    return eas_fail(EAS_ERR_VALUE, "%s: needs %llu bytes of 256-byte aligned scratch (eas_dense_scratch)", who,
+                    (unsigned long long)s.total);
+  return EAS_OK;
+}
+
+int off_mask(const void* p, uint64_t ld, int bit) { return vec_ok(p, ld) ? 0 : bit; }
+
+// dx = sum_t dz_t W_t and dW_t = dz_t^T x, from dz in memory
+int backward_products(const char* who, int terms, const uint16_t* const (&dz)[2], uint64_t lddz,
+                      const uint16_t* const (&w)[2], const uint64_t (&ldw)[2], const uint16_t* x, uint64_t ldx,
+                      uint16_t* dx, uint64_t lddx, uint16_t* const (&dw)[2], const uint64_t (&lddw)[2], uint32_t M,
+                      uint32_t N, uint32_t K, int dtype, cudaStream_t s) {
+  if (dx) {
+    Product p = {};
+    for (int t = 0; t < 2; ++t) {
+      p.a[t] = dz[t], p.a_m[t] = (int64_t)lddz;
+      p.b[t] = w[t], p.b_n[t] = 1, p.b_k[t] = (int64_t)ldw[t];
+    }
+    p.a_k = 1;
+    p.M = M, p.N = K, p.K = N, p.terms = terms;
+    p.y = dx, p.ldy = lddx, p.bf16 = dtype == kBF16;
+    int rc = launch_product(p, s, who);
+    if (rc) return rc;
+  }
+  for (int t = 0; t < terms; ++t) {
+    if (!dw[t]) continue;
+    Product p = {};
+    p.a[0] = dz[t], p.a_m[0] = 1, p.a_k = (int64_t)lddz;
+    p.b[0] = x, p.b_n[0] = 1, p.b_k[0] = (int64_t)ldx;
+    p.M = N, p.N = K, p.K = M, p.terms = 1;
+    p.y = dw[t], p.ldy = lddw[t], p.bf16 = dtype == kBF16;
+    int rc = launch_product(p, s, who);
+    if (rc) return rc;
+  }
+  return EAS_OK;
+}
+
+}  // namespace
+
+extern "C" int eas_dense_scratch(int op, uint32_t M, uint32_t N, uint32_t K, int act, int outputs, int unaligned,
+                                 uint64_t* bytes) {
+  if (!bytes) return eas_fail(EAS_ERR_VALUE, "eas_dense_scratch: null pointer");
+  if (op < 0 || op > 3) return eas_fail(EAS_ERR_VALUE, "eas_dense_scratch: op must be 0..3");
+  *bytes = 0;
+  int rc = check_sizes("eas_dense_scratch", M, N, K, kF16, act);
+  if (rc || M == 0) return rc;
+  const bool gated = op & 1;
+  *bytes = (op < 2 ? forward_scratch(gated, M, N, K, unaligned)
+                   : backward_scratch(gated, M, N, K, act, outputs, unaligned)).total;
+  return EAS_OK;
+}
+
+extern "C" int eas_linear(int dev, const void* x, const void* w, const void* bias, const void* residual, void* y,
+                          void* pre, uint32_t M, uint32_t N, uint32_t K, uint64_t ldx, uint64_t ldw, uint64_t ldr,
+                          uint64_t ldy, uint64_t ldp, int dtype, int act, void* scratch, uint64_t scratch_bytes,
+                          void* stream) {
+  const char* who = "eas_linear";
+  int rc = check_sizes(who, M, N, K, dtype, act);
+  if (rc || M == 0) return rc;
+  if (!x || !w || !y) return eas_fail(EAS_ERR_VALUE, "%s: null operand", who);
+  const Scratch sc = forward_scratch(false, M, N, K, off_mask(x, ldx, kXOff) | off_mask(w, ldw, kWOff));
+  if ((rc = check_scratch(who, sc, scratch, scratch_bytes))) return rc;
+  DeviceScope scope(dev);
+  if (scope.rc) return scope.rc;
+  Product p = {};
+  p.a[0] = u16(x), p.b[0] = u16(w);
+  p.a_m[0] = (int64_t)ldx, p.a_k = 1, p.b_n[0] = (int64_t)ldw, p.b_k[0] = 1;
+  p.M = M, p.N = N, p.K = K, p.terms = 1;
+  p.bias = u16(bias), p.residual = u16(residual), p.y = u16(y), p.pre = u16(pre);
+  p.ldr = ldr, p.ldy = ldy, p.ldp = ldp;
+  p.act = act, p.bf16 = dtype == kBF16;
+  return launch_product(p, static_cast<cudaStream_t>(stream), who);
+}
+
+extern "C" int eas_gated(int dev, const void* x, const void* w_gate, const void* w_up, void* h, void* gate, void* up,
+                         uint32_t M, uint32_t N, uint32_t K, uint64_t ldx, uint64_t ldwg, uint64_t ldwu, uint64_t ldh,
+                         uint64_t ldg, uint64_t ldu, int dtype, int act, void* scratch, uint64_t scratch_bytes,
+                         void* stream) {
+  const char* who = "eas_gated";
+  int rc = check_sizes(who, M, N, K, dtype, act);
+  if (rc || M == 0) return rc;
+  if (!x || !w_gate || !w_up || !h) return eas_fail(EAS_ERR_VALUE, "%s: null operand", who);
+  const Scratch sc = forward_scratch(true, M, N, K, off_mask(x, ldx, kXOff) | off_mask(w_gate, ldwg, kWOff) |
+                                                        off_mask(w_up, ldwu, kUpOff));
+  if ((rc = check_scratch(who, sc, scratch, scratch_bytes))) return rc;
+  DeviceScope scope(dev);
+  if (scope.rc) return scope.rc;
+  Product p = {};
+  p.a[0] = u16(x), p.b[0] = u16(w_gate), p.b[1] = u16(w_up);
+  p.a_m[0] = (int64_t)ldx, p.a_k = 1, p.b_n[0] = (int64_t)ldwg, p.b_n[1] = (int64_t)ldwu, p.b_k[0] = p.b_k[1] = 1;
+  p.M = M, p.N = N, p.K = K, p.terms = 1, p.gated = true;
+  p.y = u16(h), p.pre = u16(gate), p.pre2 = u16(up);
+  p.ldy = ldh, p.ldp = ldg, p.ldp2 = ldu;
+  p.act = act, p.bf16 = dtype == kBF16;
+  return launch_product(p, static_cast<cudaStream_t>(stream), who);
+}
+
+extern "C" int eas_linear_backward(int dev, const void* dy, const void* pre, const void* x, const void* w, void* dx,
+                                   void* dw, void* db, uint32_t M, uint32_t N, uint32_t K, uint64_t lddy, uint64_t ldp,
+                                   uint64_t ldx, uint64_t ldw, uint64_t lddx, uint64_t lddw, int dtype, int act,
+                                   void* scratch, uint64_t scratch_bytes, void* stream) {
+  const char* who = "eas_linear_backward";
+  int rc = check_sizes(who, M, N, K, dtype, act);
+  if (rc) return rc;
+  if ((M && !dy) || (M && act != kNone && !pre) || (dx && !w) || (M && dw && !x))
+    return eas_fail(EAS_ERR_VALUE, "%s: null operand", who);
+  const int outputs = (dx ? kDx : 0) | (dw ? kDw : 0) | (db ? kDb : 0);
+  if (!outputs) return EAS_OK;
+  const Scratch sc = backward_scratch(false, M, N, K, act, outputs,
+                                      off_mask(x, ldx, kXOff) | off_mask(w, ldw, kWOff) | off_mask(dy, lddy, kDyOff));
+  if (M && (rc = check_scratch(who, sc, scratch, scratch_bytes))) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  DeviceScope scope(dev);
+  if (scope.rc) return scope.rc;
+  if (M == 0) {  // no rows: the sums over them are zero
+    if (dw && (rc = zero_rows(dw, lddw, N, K, s, who))) return rc;
+    if (db && (rc = zero_rows(db, N, 1, N, s, who))) return rc;
+    return EAS_OK;
+  }
+  uint8_t* base = static_cast<uint8_t*>(scratch);
+  uint16_t* dz = sc.need_dz && (outputs & (kDx | kDw)) ? reinterpret_cast<uint16_t*>(base + sc.dz) : nullptr;
+  float* partial = db ? reinterpret_cast<float*>(base + sc.partial) : nullptr;
+  if (dz || db) {
+    ActGrad g = {};
+    g.dy = u16(dy), g.g = u16(pre), g.dg = dz, g.partial = partial;
+    g.lddy = lddy, g.ldg = ldp, g.ldo = sc.ld;
+    g.M = M, g.N = N, g.rows_per_block = sc.rows, g.act = act, g.bf16 = dtype == kBF16;
+    g.v_dy = vec_ok(dy, lddy), g.v_g = pre && vec_ok(pre, ldp), g.v_o = true;
+    act_grad_kernel<false><<<dim3((N + 255) / 256, sc.blocks), 256, 0, s>>>(g);
+    if ((rc = eas_cuda_check(cudaGetLastError(), who, EAS_ERR_LAUNCH))) return rc;
+    if (db) {
+      colsum_kernel<<<(N + 255) / 256, 256, 0, s>>>(partial, u16(db), sc.blocks, N, dtype == kBF16);
+      if ((rc = eas_cuda_check(cudaGetLastError(), who, EAS_ERR_LAUNCH))) return rc;
+    }
+  }
+  return backward_products(who, 1, {dz ? dz : u16(dy), nullptr}, dz ? sc.ld : lddy, {u16(w), nullptr}, {ldw, 0},
+                           u16(x), ldx, u16(dx), lddx, {u16(dw), nullptr}, {lddw, 0}, M, N, K, dtype, s);
+}
+
+extern "C" int eas_gated_backward(int dev, const void* dh, const void* gate, const void* up, const void* x,
+                                  const void* w_gate, const void* w_up, void* dx, void* dw_gate, void* dw_up,
+                                  uint32_t M, uint32_t N, uint32_t K, uint64_t lddh, uint64_t ldg, uint64_t ldu,
+                                  uint64_t ldx, uint64_t ldwg, uint64_t ldwu, uint64_t lddx, uint64_t lddwg,
+                                  uint64_t lddwu, int dtype, int act, void* scratch, uint64_t scratch_bytes,
+                                  void* stream) {
+  const char* who = "eas_gated_backward";
+  int rc = check_sizes(who, M, N, K, dtype, act);
+  if (rc) return rc;
+  if ((M && (!dh || !gate || !up)) || (dx && (!w_gate || !w_up)) || (M && (dw_gate || dw_up) && !x))
+    return eas_fail(EAS_ERR_VALUE, "%s: null operand", who);
+  const int outputs = (dx ? kDx : 0) | (dw_gate || dw_up ? kDw : 0);
+  if (!outputs) return EAS_OK;
+  const Scratch sc = backward_scratch(true, M, N, K, act, outputs,
+                                      off_mask(x, ldx, kXOff) | off_mask(w_gate, ldwg, kWOff) |
+                                          off_mask(w_up, ldwu, kUpOff) | off_mask(dh, lddh, kDyOff));
+  if (M && (rc = check_scratch(who, sc, scratch, scratch_bytes))) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  DeviceScope scope(dev);
+  if (scope.rc) return scope.rc;
+  if (M == 0) {
+    if (dw_gate && (rc = zero_rows(dw_gate, lddwg, N, K, s, who))) return rc;
+    if (dw_up && (rc = zero_rows(dw_up, lddwu, N, K, s, who))) return rc;
+    return EAS_OK;
+  }
+  uint8_t* base = static_cast<uint8_t*>(scratch);
+  uint16_t* dg = reinterpret_cast<uint16_t*>(base + sc.dz);
+  uint16_t* du = reinterpret_cast<uint16_t*>(base + sc.dz2);
+  ActGrad g = {};
+  g.dy = u16(dh), g.g = u16(gate), g.u = u16(up), g.dg = dg, g.du = du;
+  g.lddy = lddh, g.ldg = ldg, g.ldu = ldu, g.ldo = sc.ld;
+  g.M = M, g.N = N, g.rows_per_block = sc.rows, g.act = act, g.bf16 = dtype == kBF16;
+  g.v_dy = vec_ok(dh, lddh), g.v_g = vec_ok(gate, ldg), g.v_u = vec_ok(up, ldu), g.v_o = true;
+  act_grad_kernel<true><<<dim3((N + 255) / 256, sc.blocks), 256, 0, s>>>(g);
+  if ((rc = eas_cuda_check(cudaGetLastError(), who, EAS_ERR_LAUNCH))) return rc;
+  return backward_products(who, 2, {dg, du}, sc.ld, {u16(w_gate), u16(w_up)}, {ldwg, ldwu}, u16(x), ldx, u16(dx),
+                           lddx, {u16(dw_gate), u16(dw_up)}, {lddwg, lddwu}, M, N, K, dtype, s);
+}

@@ -29,7 +29,9 @@ import hashlib
 import math
 import os
 import struct
+import sys
 from collections import deque
+from contextlib import nullcontext
 from pathlib import Path
 from typing import Any, Mapping
 
@@ -41,6 +43,7 @@ from . import cuda_ext
 from .grid import grid_rank, infer_1d_grid, infer_grid, infer_nthreads
 
 ALL_THREADS = 0xFFFFFFFF
+_NO_CONTEXT = nullcontext()
 MAX_GRID_YZ = 65535
 
 
@@ -299,7 +302,7 @@ class CudaRuntime:
         self._available: bool | None = None
         self._reason = ""
         self._pipelines: dict[tuple[str, str, int, int], int] = {}
-        self._pending: deque[tuple[int, int, Any]] = deque()
+        self._pending: deque[tuple[int, int, Any, int]] = deque()
         self._max_in_flight: int | None = None
         self._staging: dict[tuple[int, int], list[DeviceBuffer]] = {}
         self._bounce: dict[int, _Bounce] = {}
@@ -310,7 +313,8 @@ class CudaRuntime:
         self._pending_n = 0
         self._bucket_n = 0
         self._bucket_stream = 0
-        self._event_pool: list[int] = []
+        self._bucket_device = 0
+        self._event_pool: dict[int, list[int]] = {}   # per device: an event records on its own device only
         self.launch_count = 0  # kernels launched through this runtime (generic + native)
         self.native_launches = 0  # of which pattern-lowered native kernels
         self._scratch_bufs: dict[tuple[int, int, str], DeviceBuffer] = {}
@@ -760,13 +764,17 @@ class CudaRuntime:
             self._finish_host_copies(host_copies, device, stream)
             self._unstage(args)
             return
-        # asynchronous launch: keep the arguments alive until a completion event covers it.
-        # One (pooled) event per group of launches; at most EAS_MAX_IN_FLIGHT stay unfinished.
-        if self._bucket_n and stream != self._bucket_stream:
+        self._track((args, runtime_args), stream, device)
+
+    def _track(self, keep: Any, stream: int, device: int) -> None:
+        """Asynchronous launch: keep the arguments alive until a completion event covers it.
+        One (pooled) event per group of launches; at most EAS_MAX_IN_FLIGHT stay unfinished."""
+        if self._bucket_n and (stream != self._bucket_stream or device != self._bucket_device):
             self._close_bucket()
-        self._bucket_keep.append((args, runtime_args))
+        self._bucket_keep.append(keep)
         self._bucket_n += 1
         self._bucket_stream = stream
+        self._bucket_device = device
         limit = self._max_flight()
         if self._bucket_n >= (max(1, limit // 16) if limit else 64):
             self._close_bucket()
@@ -774,6 +782,38 @@ class CudaRuntime:
             if not self._pending:
                 self._close_bucket()
             self._wait_one()
+
+    # -- native operators (easy_as_b200.ops) ---------------------------------------------
+    def check_capture(self, stream: int, sync: bool) -> bool:
+        """Whether ``stream`` is being captured into a CUDA graph; a call that waits cannot be."""
+        if not stream:
+            return False
+        capturing = cuda_ext.ctypes.c_int(0)
+        self.lib().eas_stream_is_capturing(stream, cuda_ext.ctypes.byref(capturing))
+        if capturing.value and sync:
+            raise ValueError("inside CUDA graph capture launch with _sync=False and device buffers only")
+        return bool(capturing.value)
+
+    def finish_native(self, device: int, stream: int, keep: Any, sync: bool, capturing: bool = False) -> None:
+        """After an operator's native launches on ``stream``: wait and read the kernels' status, or
+        keep ``keep`` alive until they are done (a captured launch: the graph's owner does)."""
+        self.launch_count += 1
+        self.native_launches += 1
+        if capturing:
+            return
+        if sync:
+            cuda_ext.check(self.lib().eas_stream_synchronize(stream), "kernel execution")
+            self._check_native_status(device)
+            return
+        self._track(keep, stream, device)
+
+    @staticmethod
+    def on_device(device: int) -> Any:
+        """Context in which ``device`` is current (nothing to do when it is, or without torch)."""
+        t = sys.modules.get("torch")
+        if t is not None and t.cuda.is_initialized() and t.cuda.current_device() != device:
+            return t.cuda.device(device)
+        return _NO_CONTEXT
 
     # -- prepared repeated launches (Kernel.__call__ fast path) ------------------------
     def fast_prepare(self, ck: Any, runtime_args: Mapping[str, Any], opts: Mapping[str, Any],
@@ -916,18 +956,7 @@ class CudaRuntime:
             if sync:
                 cuda_ext.check(lib.eas_stream_synchronize(stream), "kernel execution")
                 return True
-            if self._bucket_n and stream != self._bucket_stream:
-                self._close_bucket()
-            self._bucket_keep.append(args)
-            self._bucket_n += 1
-            self._bucket_stream = stream
-            limit = self._max_flight()
-            if self._bucket_n >= (max(1, limit // 16) if limit else 64):
-                self._close_bucket()
-            while limit and self.in_flight() > limit:
-                if not self._pending:
-                    self._close_bucket()
-                self._wait_one()
+            self._track(args, stream, fl.device)
             return True
         bb = fl.bounce
         if self._bounce.get(fl.device) is not bb:
@@ -950,24 +979,27 @@ class CudaRuntime:
         if not self._bucket_n:
             return
         lib = self.lib()
-        if self._event_pool:
-            ev = self._event_pool.pop()
-        else:
-            e = cuda_ext.ctypes.c_void_p()
-            cuda_ext.check(lib.eas_event_create(cuda_ext.ctypes.byref(e)), "event_create")
-            ev = int(e.value)
-        cuda_ext.check(lib.eas_event_record(ev, self._bucket_stream), "event_record")
-        self._pending.append((ev, self._bucket_n, self._bucket_keep))
+        device = self._bucket_device
+        with self.on_device(device):
+            pool = self._event_pool.get(device)
+            if pool:
+                ev = pool.pop()
+            else:
+                e = cuda_ext.ctypes.c_void_p()
+                cuda_ext.check(lib.eas_event_create(cuda_ext.ctypes.byref(e)), "event_create")
+                ev = int(e.value)
+            cuda_ext.check(lib.eas_event_record(ev, self._bucket_stream), "event_record")
+        self._pending.append((ev, self._bucket_n, self._bucket_keep, device))
         self._pending_n += self._bucket_n
         self._bucket_keep, self._bucket_n = [], 0
 
     def _wait_one(self) -> None:
-        ev, n, _keep = self._pending.popleft()
+        ev, n, _keep, device = self._pending.popleft()
         self._pending_n -= n
         try:
             cuda_ext.check(self.lib().eas_event_synchronize(ev), "kernel execution")
         finally:
-            self._event_pool.append(ev)
+            self._event_pool.setdefault(device, []).append(ev)
 
     def synchronize(self) -> None:
         self._close_bucket()
@@ -981,7 +1013,7 @@ class CudaRuntime:
         """Make ``stream`` wait (device side, no host block) for every launch queued so far."""
         self._close_bucket()
         lib = self.lib()
-        for ev, _n, _keep in self._pending:
+        for ev, _n, _keep, _dev in self._pending:
             cuda_ext.check(lib.eas_stream_wait_event(stream, ev), "stream_wait_event")
 
     def in_flight(self) -> int:

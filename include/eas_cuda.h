@@ -337,6 +337,58 @@ int eas_gemm_f16_noalloc(const void* a, const void* b, float* c, uint32_t M, uin
                          int b_kmajor, uint64_t ldc, uint64_t c_bstride, int block_n, void* stream,
                          int* status_out);
 
+/* ---- dense layers (eas.ops; no counterpart in the reference) ----------- */
+
+/* A linear layer and a gated feed-forward block, forward and backward, on f16
+ * (dtype 0) or bf16 (dtype 1) matrices with f32 sums; every result is rounded
+ * once.  M rows (tokens), K inputs, N outputs (of each projection).
+ *   act: 0 none, 1 relu, 2 gelu (erf), 3 gelu_tanh, 4 silu, 5 sigmoid
+ *   matrices are row-major with unit column stride; ld* are row pitches in
+ *   elements, any alignment
+ *   dev is the device of the operands and of `stream`; it need not be current
+ * M = 0 is a launch of nothing (the gradients of weights and bias, sums over no
+ * rows, are set to zero); N = 0 or K = 0 is EAS_ERR_VALUE.  No output may
+ * overlap an input or another output, except y the residual itself.
+ * Asynchronous on `stream`; status as eas_gemm_f16.
+ * `scratch` is 256-byte aligned device memory of at least the bytes that
+ * eas_dense_scratch returns (NULL when that is 0); it is free again when the
+ * call's work on `stream` is done, and calls that may overlap need one each. */
+
+/* y = act(x W^T + bias) + residual; bias, residual and pre may be NULL.  pre
+ * (if given) receives x W^T + bias, which eas_linear_backward needs. */
+int eas_linear(int dev, const void* x, const void* w, const void* bias, const void* residual, void* y, void* pre,
+               uint32_t M, uint32_t N, uint32_t K, uint64_t ldx, uint64_t ldw, uint64_t ldr, uint64_t ldy,
+               uint64_t ldp, int dtype, int act, void* scratch, uint64_t scratch_bytes, void* stream);
+
+/* h = act(x Wg^T) * (x Wu^T); gate and up (both or neither) receive the two
+ * products, which eas_gated_backward needs. */
+int eas_gated(int dev, const void* x, const void* w_gate, const void* w_up, void* h, void* gate, void* up,
+              uint32_t M, uint32_t N, uint32_t K, uint64_t ldx, uint64_t ldwg, uint64_t ldwu, uint64_t ldh,
+              uint64_t ldg, uint64_t ldu, int dtype, int act, void* scratch, uint64_t scratch_bytes, void* stream);
+
+/* dz = dy act'(pre); dx = dz W, dw = dz^T x, db = the sum of dz's rows (each may
+ * be NULL; the residual's gradient is dy itself).  pre may be NULL for act 0.
+ * dz is rounded to the operands' type; db is summed from the unrounded dz. */
+int eas_linear_backward(int dev, const void* dy, const void* pre, const void* x, const void* w, void* dx, void* dw,
+                        void* db, uint32_t M, uint32_t N, uint32_t K, uint64_t lddy, uint64_t ldp, uint64_t ldx,
+                        uint64_t ldw, uint64_t lddx, uint64_t lddw, int dtype, int act, void* scratch,
+                        uint64_t scratch_bytes, void* stream);
+
+/* dg = dh up act'(gate), du = dh act(gate); dx = dg Wg + du Wu, dw_gate = dg^T x,
+ * dw_up = du^T x (each may be NULL). */
+int eas_gated_backward(int dev, const void* dh, const void* gate, const void* up, const void* x, const void* w_gate,
+                       const void* w_up, void* dx, void* dw_gate, void* dw_up, uint32_t M, uint32_t N, uint32_t K,
+                       uint64_t lddh, uint64_t ldg, uint64_t ldu, uint64_t ldx, uint64_t ldwg, uint64_t ldwu,
+                       uint64_t lddx, uint64_t lddwg, uint64_t lddwu, int dtype, int act, void* scratch,
+                       uint64_t scratch_bytes, void* stream);
+
+/* Scratch bytes of one call.  op: 0 eas_linear, 1 eas_gated, 2
+ * eas_linear_backward, 3 eas_gated_backward.  outputs (2 and 3): 1 dx, 2 a
+ * weight gradient, 4 db, summed.  unaligned: operands whose base or row pitch
+ * is not a multiple of 16 bytes: 1 x, 2 w or w_gate, 4 w_up, 8 dy, summed. */
+int eas_dense_scratch(int op, uint32_t M, uint32_t N, uint32_t K, int act, int outputs, int unaligned,
+                      uint64_t* bytes);
+
 /* ---- host-side fault injection (tests; no device fault is ever made; no
  *      counterpart in the reference) ---------------------------------------- */
 

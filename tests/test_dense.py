@@ -1,0 +1,179 @@
+"""CPU: what eas.ops refuses, and the C entry points' checks of their arguments (no GPU)."""
+
+import ctypes
+
+import numpy as np
+import pytest
+
+import eas
+from easy_as_b200.runtime import cuda_ext
+from easy_as_b200.tensor import Tensor
+
+
+def dev(rows, cols, *, at=0x10000000, device=0, dtype=np.float16):
+    """An eas.Tensor on a device address that nothing reads: every check comes before the launch."""
+    shape = (cols,) if rows is None else (rows, cols)
+    return Tensor._from_cuda_ptr(at, shape, dtype, device, owner=None)
+
+
+_next = [0x20000000]
+
+
+def new(rows, cols, **kw):
+    _next[0] += 1 << 24
+    return dev(rows, cols, at=_next[0], **kw)
+
+
+def linear_args():
+    return {"x": new(4, 16), "w": new(8, 16), "y": new(4, 8)}
+
+
+def test_names():
+    assert eas.ops.ACTIVATIONS == ("none", "relu", "gelu", "gelu_tanh", "silu", "sigmoid")
+    import eas.ops as direct
+
+    assert direct is eas.ops
+
+
+@pytest.mark.parametrize("change,error,match", [
+    ({"x": np.zeros((4, 16), np.float16)}, TypeError, "'x'"),
+    ({"x": "nothing"}, TypeError, "'x'"),
+    ({"x": eas.tensor(np.zeros((4, 16), np.float16))}, TypeError, "CUDA device"),
+    ({"w": new(8, 16, dtype=np.float32)}, TypeError, "float16"),
+    ({"x": new(4, 15)}, ValueError, "'x' has shape"),
+    ({"y": new(4, 9)}, ValueError, "'y' has shape"),
+    ({"y": new(5, 8)}, ValueError, "'y' has shape"),
+    ({"w": new(None, 16)}, ValueError, "matrix"),
+    ({"w": new(0, 16), "y": new(4, 0)}, ValueError, "at least one"),
+    ({"x": new(4, 0), "w": new(8, 0)}, ValueError, "at least one"),
+    ({"bias": new(None, 7)}, ValueError, "'bias'"),
+    ({"bias": new(1, 8)}, ValueError, "'bias'"),
+    ({"residual": new(1, 8)}, ValueError, "'residual'"),
+    ({"pre": new(4, 16)}, ValueError, "'pre'"),
+    ({"y": new(4, 8, device=1)}, ValueError, "different devices"),
+    ({"act": "swish"}, ValueError, "unknown activation"),
+    ({"_sync": 1}, TypeError, "_sync"),
+])
+def test_linear_refusals(change, error, match):
+    args = {**linear_args(), **change}
+    x, w, y = args.pop("x"), args.pop("w"), args.pop("y")
+    with pytest.raises(error, match=match):
+        eas.ops.linear(x, w, y, **args)
+
+
+def test_torch_refusals():
+    torch = pytest.importorskip("torch")
+    with pytest.raises(TypeError, match="CUDA device"):
+        eas.ops.linear(torch.zeros(4, 16, dtype=torch.float16), new(8, 16), new(4, 8))
+    with pytest.raises(TypeError, match="float16 or bfloat16"):
+        eas.ops.linear(torch.zeros(4, 16), new(8, 16), new(4, 8))
+
+
+@pytest.mark.parametrize("y", [
+    dev(4, 8, at=0x10000000),                  # x itself
+    dev(4, 8, at=0x10000000 + 4 * 16 * 2 - 2),  # x's last element
+    dev(4, 8, at=0x30000000),                  # the weight
+    dev(4, 8, at=0x40000000 + 2),              # the residual, one element off
+    dev(4, 8, at=0x50000000),                  # the bias
+    dev(4, 8, at=0x60000000 + 4 * 8),          # pre
+])
+def test_overlaps_are_refused(y):
+    with pytest.raises(ValueError, match="overlaps"):
+        eas.ops.linear(dev(4, 16), dev(8, 16, at=0x30000000), y, residual=dev(4, 8, at=0x40000000),
+                       bias=dev(None, 8, at=0x50000000), pre=dev(4, 8, at=0x60000000))
+
+
+def test_side_by_side_columns_do_not_overlap():
+    from easy_as_b200.ops import _Rows, _share
+
+    def cols(first, count, rows=4, ld=32):
+        return _Rows(0x1000 + 2 * first, rows, count, ld, (rows,), None)
+
+    assert not _share(cols(0, 8), cols(8, 8)) and not _share(cols(8, 8), cols(0, 8))
+    assert not _share(cols(24, 8), cols(32, 8))           # the next row's first columns, one row further
+    assert _share(cols(0, 9), cols(8, 8)) and _share(cols(8, 8), cols(0, 9))
+    assert _share(cols(30, 8), cols(0, 8))                # wraps into the next row
+    assert _share(cols(0, 8), cols(8, 8, ld=40))          # other pitches: not told apart
+    assert not _share(cols(0, 8, rows=0), cols(0, 8))
+
+
+def test_gated_refusals():
+    x, wg, wu, h = new(4, 16), new(8, 16), new(8, 16), new(4, 8)
+    with pytest.raises(ValueError, match="both of gate and up"):
+        eas.ops.gated(x, wg, wu, h, gate=new(4, 8))
+    with pytest.raises(ValueError, match="'w_up'"):
+        eas.ops.gated(x, wg, new(9, 16), h)
+    with pytest.raises(ValueError, match="'h'"):
+        eas.ops.gated(x, wg, wu, new(4, 16))
+    g = new(4, 8)
+    with pytest.raises(ValueError, match="overlaps"):
+        eas.ops.gated(x, wg, wu, h, gate=g, up=g)
+    with pytest.raises(ValueError, match="unknown activation"):
+        eas.ops.gated(x, wg, wu, h, act=None)
+
+
+def test_backward_refusals():
+    dy, x, w = new(4, 8), new(4, 16), new(8, 16)
+    with pytest.raises(ValueError, match="needs pre"):
+        eas.ops.linear_backward(dy, x, w, dx=new(4, 16), act="gelu")
+    with pytest.raises(ValueError, match="'dx'"):
+        eas.ops.linear_backward(dy, x, w, dx=new(4, 8))
+    with pytest.raises(ValueError, match="'dw'"):
+        eas.ops.linear_backward(dy, x, w, dw=new(16, 8))
+    with pytest.raises(ValueError, match="'dbias'"):
+        eas.ops.linear_backward(dy, x, w, dbias=new(None, 16))
+    with pytest.raises(ValueError, match="overlaps"):
+        eas.ops.linear_backward(dy, x, w, dx=x)
+    with pytest.raises(ValueError, match="overlaps"):
+        eas.ops.gated_backward(dy, x, w, new(8, 16), dy, dy, dw_gate=w)
+    with pytest.raises(ValueError, match="'gate'"):
+        eas.ops.gated_backward(dy, x, w, new(8, 16), x, dy, dx=new(4, 16))
+    eas.ops.linear_backward(dy, x, w)   # nothing asked for: nothing to do
+
+
+def _call(name, **change):
+    args = {"eas_linear": dict(dev=0, x=256, w=512, bias=None, residual=None, y=1024, pre=None, M=4, N=8, K=16, ldx=16,
+                               ldw=16, ldr=0, ldy=8, ldp=0, dtype=0, act=0, scratch=None, nbytes=0, stream=None),
+            "eas_gated": dict(dev=0, x=256, wg=512, wu=768, h=1024, gate=None, up=None, M=4, N=8, K=16, ldx=16, ldwg=16,
+                              ldwu=16, ldh=8, ldg=0, ldu=0, dtype=0, act=0, scratch=None, nbytes=0, stream=None),
+            "eas_linear_backward": dict(dev=0, dy=256, pre=512, x=768, w=1024, dx=2048, dw=4096, db=8192, M=4, N=8, K=16,
+                                        lddy=8, ldp=8, ldx=16, ldw=16, lddx=16, lddw=16, dtype=0, act=1, scratch=None,
+                                        nbytes=0, stream=None),
+            "eas_gated_backward": dict(dev=0, dh=256, gate=512, up=768, x=1024, wg=2048, wu=4096, dx=8192, dwg=16384,
+                                       dwu=32768, M=4, N=8, K=16, lddh=8, ldg=8, ldu=8, ldx=16, ldwg=16, ldwu=16,
+                                       lddx=16, lddwg=16, lddwu=16, dtype=0, act=1, scratch=None, nbytes=0,
+                                       stream=None)}[name]
+    assert set(change) <= set(args)
+    return getattr(cuda_ext.load(), name)(*{**args, **change}.values())
+
+
+@pytest.mark.parametrize("name", ["eas_linear", "eas_gated", "eas_linear_backward", "eas_gated_backward"])
+@pytest.mark.parametrize("change,match", [
+    ({"dtype": 2}, "dtype"), ({"dtype": -1}, "dtype"), ({"act": 6}, "activation"), ({"act": -1}, "activation"),
+    ({"N": 0}, "positive"), ({"K": 0}, "positive"), ({"M": 0xffffffff}, "exceeds"), ({"K": 0x80000000}, "exceeds"),
+    ({"x": None}, "null"),
+])
+def test_c_entries_check_their_arguments(name, change, match):
+    assert _call(name, **change) == cuda_ext.EAS_ERR_VALUE
+    assert match in cuda_ext.last_error() and name in cuda_ext.last_error()
+
+
+@pytest.mark.parametrize("name", ["eas_linear_backward", "eas_gated_backward"])
+def test_c_entries_want_their_scratch(name):
+    lib = cuda_ext.load()
+    need = ctypes.c_uint64()
+    op = 2 if name == "eas_linear_backward" else 3
+    assert lib.eas_dense_scratch(op, 4, 8, 16, 1, 7 if op == 2 else 3, 0, ctypes.byref(need)) == 0
+    assert need.value > 0 and need.value % 256 == 0
+    for scratch, nbytes in ((None, need.value), (65536, need.value - 1), (65536 + 16, need.value)):
+        assert _call(name, scratch=scratch, nbytes=nbytes) == cuda_ext.EAS_ERR_VALUE
+        assert "scratch" in cuda_ext.last_error()
+
+
+def test_scratch_query_checks_its_arguments():
+    lib = cuda_ext.load()
+    need = ctypes.c_uint64(5)
+    assert lib.eas_dense_scratch(4, 1, 1, 1, 0, 0, 0, ctypes.byref(need)) == cuda_ext.EAS_ERR_VALUE
+    assert lib.eas_dense_scratch(0, 1, 0, 1, 0, 0, 0, ctypes.byref(need)) == cuda_ext.EAS_ERR_VALUE
+    assert lib.eas_dense_scratch(0, 1, 1, 1, 0, 0, 0, None) == cuda_ext.EAS_ERR_VALUE
+    assert lib.eas_dense_scratch(2, 0, 1, 1, 0, 7, 15, ctypes.byref(need)) == 0 and need.value == 0
