@@ -12,97 +12,13 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "dense_internal.h"
 #include "dense_math.cuh"
 #include "eas_internal.h"
 
 namespace {
 
 using namespace dense;
-
-// C[m][n] = sum_t sum_k A_t[m][k] B_t[n][k], element strides for every operand
-struct Product {
-  const uint16_t* a[2];
-  const uint16_t* b[2];
-  int64_t a_m[2], a_k, b_n[2], b_k[2];
-  int M, N, K;
-  int terms;   // 1, or 2: two products summed
-  bool gated;  // one A, two B: the epilogue combines the two products
-  // epilogue
-  const uint16_t* bias;
-  const uint16_t* residual;
-  uint16_t* y;
-  uint16_t* pre;   // z (linear) or g (gated)
-  uint16_t* pre2;  // u (gated)
-  int64_t ldr, ldy, ldp, ldp2;
-  int act;
-  bool bf16;
-};
-
-constexpr int kT = 64, kTK = 16;
-
-// The plain tiled product: 64 x 64 outputs per block of 256 threads, 4 x 4 per thread, f32 FMAs.
-template <bool GATED>
-__global__ void __launch_bounds__(256) product_kernel(const Product p) {
-  __shared__ float sa[kTK][kT + 4];
-  __shared__ float sb[GATED ? 2 : 1][kTK][kT + 4];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int m0 = blockIdx.y * kT, n0 = blockIdx.x * kT;
-  float acc[GATED ? 2 : 1][4][4] = {};
-  const int terms = GATED ? 1 : p.terms;
-  for (int t = 0; t < terms; ++t) {
-    for (int k0 = 0; k0 < p.K; k0 += kTK) {
-      for (int i = threadIdx.x; i < kT * kTK; i += 256) {
-        int r, k;
-        if (p.a_k == 1) { k = i % kTK; r = i / kTK; } else { r = i % kT; k = i / kT; }
-        sa[k][r] = (m0 + r < p.M && k0 + k < p.K) ? to_f32(p.a[t][(m0 + r) * p.a_m[t] + (k0 + k) * p.a_k], p.bf16) : 0.0f;
-        if (p.b_k[0] == 1) { k = i % kTK; r = i / kTK; } else { r = i % kT; k = i / kT; }
-#pragma unroll
-        for (int h = 0; h < (GATED ? 2 : 1); ++h)
-          sb[h][k][r] = (n0 + r < p.N && k0 + k < p.K)
-                            ? to_f32(p.b[GATED ? h : t][(n0 + r) * p.b_n[GATED ? h : t] + (k0 + k) * p.b_k[GATED ? h : t]], p.bf16) : 0.0f;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < kTK; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int h = 0; h < (GATED ? 2 : 1); ++h)
-              acc[h][i][j] = fmaf(sa[k][ty * 4 + i], sb[h][k][tx * 4 + j], acc[h][i][j]);
-      __syncthreads();
-    }
-  }
-  with_act(p.act, [&](auto a) {
-    for (int i = 0; i < 4; ++i)
-      for (int j = 0; j < 4; ++j) {
-        const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-        if (m >= p.M || n >= p.N) continue;
-        float z = acc[0][i][j];
-        if (!GATED && p.bias) z += to_f32(p.bias[n], p.bf16);
-        if (p.pre) p.pre[m * p.ldp + n] = to_16(z, p.bf16);
-        float v = act<decltype(a)::value>(z);
-        if (GATED) {
-          const float u = acc[GATED ? 1 : 0][i][j];
-          if (p.pre2) p.pre2[m * p.ldp2 + n] = to_16(u, p.bf16);
-          v *= u;
-        } else if (p.residual) {
-          v += to_f32(p.residual[m * p.ldr + n], p.bf16);
-        }
-        p.y[m * p.ldy + n] = to_16(v, p.bf16);
-      }
-  });
-}
-
-int launch_product(const Product& p, cudaStream_t s, const char* who) {
-  const dim3 grid((p.N + kT - 1) / kT, (p.M + kT - 1) / kT);
-  if (p.gated)
-    product_kernel<true><<<grid, 256, 0, s>>>(p);
-  else
-    product_kernel<false><<<grid, 256, 0, s>>>(p);
-  return eas_cuda_check(cudaGetLastError(), who, EAS_ERR_LAUNCH);
-}
 
 // ---------------------------------------------------------------------------
 // the elementwise half of the backward pass
@@ -267,34 +183,43 @@ uint16_t* u16(void* p) { return static_cast<uint16_t*>(p); }
 enum { kDx = 1, kDw = 2, kDb = 4 };
 enum { kXOff = 1, kWOff = 2, kUpOff = 4, kDyOff = 8 };
 
-// Layout of the scratch of a backward pass: dz (or dg, du) in rows padded to 8 elements, then the
-// partial sums of db.
+// Layout of a call's scratch: operands that TMA cannot read in place, copied into rows padded to 8
+// elements; of a backward pass also dz (or dg, du) in such rows and the partial sums of db.
 struct Scratch {
-  uint64_t dz = 0, dz2 = 0, partial = 0, total = 0;
-  uint64_t ld = 0;
+  uint64_t x = 0, w = 0, up = 0, dz = 0, dz2 = 0, partial = 0, total = 0;
+  uint64_t ldk = 0, ldn = 0;  // padded pitches of rows of K and of N elements
   int rows = 0, blocks = 0;
   bool need_dz = false;
+
+  Scratch(uint32_t N, uint32_t K) : ldk(((uint64_t)K + 7) / 8 * 8), ldn(((uint64_t)N + 7) / 8 * 8) {}
+  uint64_t take(uint64_t bytes) {
+    const uint64_t at = total;
+    total += round256(bytes);
+    return at;
+  }
 };
 
-uint64_t take(Scratch& s, uint64_t bytes) {
-  const uint64_t at = s.total;
-  s.total += round256(bytes);
-  return at;
-}
-
-Scratch backward_scratch(bool gated, uint32_t M, uint32_t N, uint32_t K, int act, int outputs, int off) {
-  Scratch s;
-  s.ld = ((uint64_t)N + 7) / 8 * 8;
-  s.rows = rows_per_block((int)M, (int)N);
-  s.blocks = (int)(((uint64_t)M + s.rows - 1) / s.rows);
-  s.need_dz = gated || act != kNone || ((off & kDyOff) && (outputs & (kDx | kDw)));
-  if (s.need_dz) s.dz = take(s, (uint64_t)M * s.ld * 2);
-  if (gated) s.dz2 = take(s, (uint64_t)M * s.ld * 2);
-  if (outputs & kDb) s.partial = take(s, (uint64_t)s.blocks * N * 4);
+Scratch forward_scratch(bool gated, uint32_t M, uint32_t N, uint32_t K, int off) {
+  Scratch s(N, K);
+  if (off & kXOff) s.x = s.take(2 * (uint64_t)M * s.ldk);
+  if (off & kWOff) s.w = s.take(2 * (uint64_t)N * s.ldk);
+  if (gated && (off & kUpOff)) s.up = s.take(2 * (uint64_t)N * s.ldk);
   return s;
 }
 
-Scratch forward_scratch(bool gated, uint32_t M, uint32_t N, uint32_t K, int off) { return Scratch(); }
+Scratch backward_scratch(bool gated, uint32_t M, uint32_t N, uint32_t K, int act, int outputs, int off) {
+  Scratch s(N, K);
+  if ((outputs & kDw) && (off & kXOff)) s.x = s.take(2 * (uint64_t)M * s.ldk);
+  if ((outputs & kDx) && (off & kWOff)) s.w = s.take(2 * (uint64_t)N * s.ldk);
+  if (gated && (outputs & kDx) && (off & kUpOff)) s.up = s.take(2 * (uint64_t)N * s.ldk);
+  s.rows = rows_per_block((int)M, (int)N);
+  s.blocks = (int)(((uint64_t)M + s.rows - 1) / s.rows);
+  s.need_dz = (outputs & (kDx | kDw)) && (gated || act != kNone || (off & kDyOff));
+  if (s.need_dz) s.dz = s.take(2 * (uint64_t)M * s.ldn);
+  if (s.need_dz && gated) s.dz2 = s.take(2 * (uint64_t)M * s.ldn);
+  if (outputs & kDb) s.partial = s.take((uint64_t)s.blocks * N * 4);
+  return s;
+}
 
 int check_scratch(const char* who, const Scratch& s, const void* p, uint64_t bytes) {
   if (s.total && (!p || bytes < s.total || (reinterpret_cast<uintptr_t>(p) & 255)))
@@ -305,34 +230,46 @@ int check_scratch(const char* who, const Scratch& s, const void* p, uint64_t byt
 
 int off_mask(const void* p, uint64_t ld, int bit) { return vec_ok(p, ld) ? 0 : bit; }
 
-// dx = sum_t dz_t W_t and dW_t = dz_t^T x, from dz in memory
-int backward_products(const char* who, int terms, const uint16_t* const (&dz)[2], uint64_t lddz,
-                      const uint16_t* const (&w)[2], const uint64_t (&ldw)[2], const uint16_t* x, uint64_t ldx,
-                      uint16_t* dx, uint64_t lddx, uint16_t* const (&dw)[2], const uint64_t (&lddw)[2], uint32_t M,
-                      uint32_t N, uint32_t K, int dtype, cudaStream_t s) {
+// A matrix as a product's operand: itself, or its copy in scratch rows TMA can read.
+struct Operand {
+  const uint16_t* p;
+  uint64_t ld;
+};
+
+int operand(const void* src, uint64_t ld, uint32_t rows, uint32_t cols, bool off, void* scratch, uint64_t at,
+            uint64_t ld_pad, cudaStream_t s, Operand* out) {
+  *out = {u16(src), ld};
+  if (!off) return EAS_OK;
+  uint8_t* dst = static_cast<uint8_t*>(scratch) + at;
+  *out = {u16(dst), ld_pad};
+  return eas_pad_f16_2d(src, dst, rows, (uint32_t)ld_pad, ld, ld_pad, rows, cols, 1, 0, 0, s);
+}
+
+// dx = sum_t dz_t W_t and dW_t = dz_t^T x
+int backward_products(const char* who, int terms, const Operand (&dz)[2], const Operand (&w)[2], const Operand& x,
+                      void* dx, uint64_t lddx, void* const (&dw)[2], const uint64_t (&lddw)[2], uint32_t M, uint32_t N,
+                      uint32_t K, int dtype, cudaStream_t s) {
   if (dx) {
-    Product p = {};
-    for (int t = 0; t < 2; ++t) {
-      p.a[t] = dz[t], p.a_m[t] = (int64_t)lddz;
-      p.b[t] = w[t], p.b_n[t] = 1, p.b_k[t] = (int64_t)ldw[t];
-    }
-    p.a_k = 1;
-    p.M = M, p.N = K, p.K = N, p.terms = terms;
-    p.y = dx, p.ldy = lddx, p.bf16 = dtype == kBF16;
-    int rc = launch_product(p, s, who);
+    DenseProduct p;
+    for (int t = 0; t < terms; ++t) p.a[t] = dz[t].p, p.lda[t] = dz[t].ld, p.b[t] = w[t].p, p.ldb[t] = w[t].ld;
+    p.b_mn = true;
+    p.M = (int)M, p.N = (int)K, p.K = (int)N, p.terms = terms;
+    p.y[0] = u16(dx), p.ldy[0] = lddx, p.bf16 = dtype == kBF16;
+    int rc = dense_mma(p, s, who);
     if (rc) return rc;
   }
+  DenseProduct p;
+  p.batch = 0;
   for (int t = 0; t < terms; ++t) {
     if (!dw[t]) continue;
-    Product p = {};
-    p.a[0] = dz[t], p.a_m[0] = 1, p.a_k = (int64_t)lddz;
-    p.b[0] = x, p.b_n[0] = 1, p.b_k[0] = (int64_t)ldx;
-    p.M = N, p.N = K, p.K = M, p.terms = 1;
-    p.y = dw[t], p.ldy = lddw[t], p.bf16 = dtype == kBF16;
-    int rc = launch_product(p, s, who);
-    if (rc) return rc;
+    const int z = p.batch++;
+    p.a[z] = dz[t].p, p.lda[z] = dz[t].ld, p.y[z] = u16(dw[t]), p.ldy[z] = lddw[t];
   }
-  return EAS_OK;
+  if (!p.batch) return EAS_OK;
+  p.b[0] = x.p, p.ldb[0] = x.ld;
+  p.a_mn = p.b_mn = true;
+  p.M = (int)N, p.N = (int)K, p.K = (int)M, p.bf16 = dtype == kBF16;
+  return dense_mma(p, s, who);
 }
 
 }  // namespace
@@ -358,18 +295,22 @@ extern "C" int eas_linear(int dev, const void* x, const void* w, const void* bia
   int rc = check_sizes(who, M, N, K, dtype, act);
   if (rc || M == 0) return rc;
   if (!x || !w || !y) return eas_fail(EAS_ERR_VALUE, "%s: null operand", who);
-  const Scratch sc = forward_scratch(false, M, N, K, off_mask(x, ldx, kXOff) | off_mask(w, ldw, kWOff));
+  const int off = off_mask(x, ldx, kXOff) | off_mask(w, ldw, kWOff);
+  const Scratch sc = forward_scratch(false, M, N, K, off);
   if ((rc = check_scratch(who, sc, scratch, scratch_bytes))) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
   DeviceScope scope(dev);
   if (scope.rc) return scope.rc;
-  Product p = {};
-  p.a[0] = u16(x), p.b[0] = u16(w);
-  p.a_m[0] = (int64_t)ldx, p.a_k = 1, p.b_n[0] = (int64_t)ldw, p.b_k[0] = 1;
-  p.M = M, p.N = N, p.K = K, p.terms = 1;
-  p.bias = u16(bias), p.residual = u16(residual), p.y = u16(y), p.pre = u16(pre);
-  p.ldr = ldr, p.ldy = ldy, p.ldp = ldp;
+  Operand X, W;
+  if ((rc = operand(x, ldx, M, K, off & kXOff, scratch, sc.x, sc.ldk, s, &X))) return rc;
+  if ((rc = operand(w, ldw, N, K, off & kWOff, scratch, sc.w, sc.ldk, s, &W))) return rc;
+  DenseProduct p;
+  p.a[0] = X.p, p.lda[0] = X.ld, p.b[0] = W.p, p.ldb[0] = W.ld;
+  p.M = (int)M, p.N = (int)N, p.K = (int)K;
+  p.bias = u16(bias), p.residual = u16(residual), p.y[0] = u16(y), p.pre = u16(pre);
+  p.ldr = ldr, p.ldy[0] = ldy, p.ldp = ldp;
   p.act = act, p.bf16 = dtype == kBF16;
-  return launch_product(p, static_cast<cudaStream_t>(stream), who);
+  return dense_mma(p, s, who);
 }
 
 extern "C" int eas_gated(int dev, const void* x, const void* w_gate, const void* w_up, void* h, void* gate, void* up,
@@ -380,19 +321,24 @@ extern "C" int eas_gated(int dev, const void* x, const void* w_gate, const void*
   int rc = check_sizes(who, M, N, K, dtype, act);
   if (rc || M == 0) return rc;
   if (!x || !w_gate || !w_up || !h) return eas_fail(EAS_ERR_VALUE, "%s: null operand", who);
-  const Scratch sc = forward_scratch(true, M, N, K, off_mask(x, ldx, kXOff) | off_mask(w_gate, ldwg, kWOff) |
-                                                        off_mask(w_up, ldwu, kUpOff));
+  const int off = off_mask(x, ldx, kXOff) | off_mask(w_gate, ldwg, kWOff) | off_mask(w_up, ldwu, kUpOff);
+  const Scratch sc = forward_scratch(true, M, N, K, off);
   if ((rc = check_scratch(who, sc, scratch, scratch_bytes))) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
   DeviceScope scope(dev);
   if (scope.rc) return scope.rc;
-  Product p = {};
-  p.a[0] = u16(x), p.b[0] = u16(w_gate), p.b[1] = u16(w_up);
-  p.a_m[0] = (int64_t)ldx, p.a_k = 1, p.b_n[0] = (int64_t)ldwg, p.b_n[1] = (int64_t)ldwu, p.b_k[0] = p.b_k[1] = 1;
-  p.M = M, p.N = N, p.K = K, p.terms = 1, p.gated = true;
-  p.y = u16(h), p.pre = u16(gate), p.pre2 = u16(up);
-  p.ldy = ldh, p.ldp = ldg, p.ldp2 = ldu;
+  Operand X, G, U;
+  if ((rc = operand(x, ldx, M, K, off & kXOff, scratch, sc.x, sc.ldk, s, &X))) return rc;
+  if ((rc = operand(w_gate, ldwg, N, K, off & kWOff, scratch, sc.w, sc.ldk, s, &G))) return rc;
+  if ((rc = operand(w_up, ldwu, N, K, off & kUpOff, scratch, sc.up, sc.ldk, s, &U))) return rc;
+  DenseProduct p;
+  p.gated = true;
+  p.a[0] = X.p, p.lda[0] = X.ld, p.b[0] = G.p, p.ldb[0] = G.ld, p.b[1] = U.p, p.ldb[1] = U.ld;
+  p.M = (int)M, p.N = (int)N, p.K = (int)K;
+  p.y[0] = u16(h), p.pre = u16(gate), p.pre2 = u16(up);
+  p.ldy[0] = ldh, p.ldp = ldg, p.ldp2 = ldu;
   p.act = act, p.bf16 = dtype == kBF16;
-  return launch_product(p, static_cast<cudaStream_t>(stream), who);
+  return dense_mma(p, s, who);
 }
 
 extern "C" int eas_linear_backward(int dev, const void* dy, const void* pre, const void* x, const void* w, void* dx,
@@ -406,8 +352,8 @@ extern "C" int eas_linear_backward(int dev, const void* dy, const void* pre, con
     return eas_fail(EAS_ERR_VALUE, "%s: null operand", who);
   const int outputs = (dx ? kDx : 0) | (dw ? kDw : 0) | (db ? kDb : 0);
   if (!outputs) return EAS_OK;
-  const Scratch sc = backward_scratch(false, M, N, K, act, outputs,
-                                      off_mask(x, ldx, kXOff) | off_mask(w, ldw, kWOff) | off_mask(dy, lddy, kDyOff));
+  const int off = off_mask(x, ldx, kXOff) | off_mask(w, ldw, kWOff) | off_mask(dy, lddy, kDyOff);
+  const Scratch sc = backward_scratch(false, M, N, K, act, outputs, off);
   if (M && (rc = check_scratch(who, sc, scratch, scratch_bytes))) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   DeviceScope scope(dev);
@@ -418,12 +364,12 @@ extern "C" int eas_linear_backward(int dev, const void* dy, const void* pre, con
     return EAS_OK;
   }
   uint8_t* base = static_cast<uint8_t*>(scratch);
-  uint16_t* dz = sc.need_dz && (outputs & (kDx | kDw)) ? reinterpret_cast<uint16_t*>(base + sc.dz) : nullptr;
+  uint16_t* dz = sc.need_dz ? reinterpret_cast<uint16_t*>(base + sc.dz) : nullptr;
   float* partial = db ? reinterpret_cast<float*>(base + sc.partial) : nullptr;
   if (dz || db) {
     ActGrad g = {};
     g.dy = u16(dy), g.g = u16(pre), g.dg = dz, g.partial = partial;
-    g.lddy = lddy, g.ldg = ldp, g.ldo = sc.ld;
+    g.lddy = lddy, g.ldg = ldp, g.ldo = sc.ldn;
     g.M = M, g.N = N, g.rows_per_block = sc.rows, g.act = act, g.bf16 = dtype == kBF16;
     g.v_dy = vec_ok(dy, lddy), g.v_g = pre && vec_ok(pre, ldp), g.v_o = true;
     act_grad_kernel<false><<<dim3((N + 255) / 256, sc.blocks), 256, 0, s>>>(g);
@@ -433,8 +379,11 @@ extern "C" int eas_linear_backward(int dev, const void* dy, const void* pre, con
       if ((rc = eas_cuda_check(cudaGetLastError(), who, EAS_ERR_LAUNCH))) return rc;
     }
   }
-  return backward_products(who, 1, {dz ? dz : u16(dy), nullptr}, dz ? sc.ld : lddy, {u16(w), nullptr}, {ldw, 0},
-                           u16(x), ldx, u16(dx), lddx, {u16(dw), nullptr}, {lddw, 0}, M, N, K, dtype, s);
+  Operand X = {}, W = {};
+  if (dw && (rc = operand(x, ldx, M, K, off & kXOff, scratch, sc.x, sc.ldk, s, &X))) return rc;
+  if (dx && (rc = operand(w, ldw, N, K, off & kWOff, scratch, sc.w, sc.ldk, s, &W))) return rc;
+  const Operand DZ = dz ? Operand{dz, sc.ldn} : Operand{u16(dy), lddy};
+  return backward_products(who, 1, {DZ, {}}, {W, {}}, X, dx, lddx, {dw, nullptr}, {lddw, 0}, M, N, K, dtype, s);
 }
 
 extern "C" int eas_gated_backward(int dev, const void* dh, const void* gate, const void* up, const void* x,
@@ -450,9 +399,9 @@ extern "C" int eas_gated_backward(int dev, const void* dh, const void* gate, con
     return eas_fail(EAS_ERR_VALUE, "%s: null operand", who);
   const int outputs = (dx ? kDx : 0) | (dw_gate || dw_up ? kDw : 0);
   if (!outputs) return EAS_OK;
-  const Scratch sc = backward_scratch(true, M, N, K, act, outputs,
-                                      off_mask(x, ldx, kXOff) | off_mask(w_gate, ldwg, kWOff) |
-                                          off_mask(w_up, ldwu, kUpOff) | off_mask(dh, lddh, kDyOff));
+  const int off = off_mask(x, ldx, kXOff) | off_mask(w_gate, ldwg, kWOff) | off_mask(w_up, ldwu, kUpOff) |
+                  off_mask(dh, lddh, kDyOff);
+  const Scratch sc = backward_scratch(true, M, N, K, act, outputs, off);
   if (M && (rc = check_scratch(who, sc, scratch, scratch_bytes))) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   DeviceScope scope(dev);
@@ -463,15 +412,21 @@ extern "C" int eas_gated_backward(int dev, const void* dh, const void* gate, con
     return EAS_OK;
   }
   uint8_t* base = static_cast<uint8_t*>(scratch);
-  uint16_t* dg = reinterpret_cast<uint16_t*>(base + sc.dz);
+  uint16_t* dg = reinterpret_cast<uint16_t*>(base + sc.dz);  // need_dz: some output is asked for
   uint16_t* du = reinterpret_cast<uint16_t*>(base + sc.dz2);
   ActGrad g = {};
   g.dy = u16(dh), g.g = u16(gate), g.u = u16(up), g.dg = dg, g.du = du;
-  g.lddy = lddh, g.ldg = ldg, g.ldu = ldu, g.ldo = sc.ld;
+  g.lddy = lddh, g.ldg = ldg, g.ldu = ldu, g.ldo = sc.ldn;
   g.M = M, g.N = N, g.rows_per_block = sc.rows, g.act = act, g.bf16 = dtype == kBF16;
   g.v_dy = vec_ok(dh, lddh), g.v_g = vec_ok(gate, ldg), g.v_u = vec_ok(up, ldu), g.v_o = true;
   act_grad_kernel<true><<<dim3((N + 255) / 256, sc.blocks), 256, 0, s>>>(g);
   if ((rc = eas_cuda_check(cudaGetLastError(), who, EAS_ERR_LAUNCH))) return rc;
-  return backward_products(who, 2, {dg, du}, sc.ld, {u16(w_gate), u16(w_up)}, {ldwg, ldwu}, u16(x), ldx, u16(dx),
-                           lddx, {u16(dw_gate), u16(dw_up)}, {lddwg, lddwu}, M, N, K, dtype, s);
+  Operand X = {}, G = {}, U = {};
+  if ((outputs & kDw) && (rc = operand(x, ldx, M, K, off & kXOff, scratch, sc.x, sc.ldk, s, &X))) return rc;
+  if (dx) {
+    if ((rc = operand(w_gate, ldwg, N, K, off & kWOff, scratch, sc.w, sc.ldk, s, &G))) return rc;
+    if ((rc = operand(w_up, ldwu, N, K, off & kUpOff, scratch, sc.up, sc.ldk, s, &U))) return rc;
+  }
+  return backward_products(who, 2, {{dg, sc.ldn}, {du, sc.ldn}}, {G, U}, X, dx, lddx, {dw_gate, dw_up},
+                           {lddwg, lddwu}, M, N, K, dtype, s);
 }

@@ -1,0 +1,29 @@
+// dense_internal.h — the matrix products behind the dense-layer operators.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+// C = sum_t A_t B_t^T with an epilogue, on 16-bit matrices with f32 sums.
+//   plain   z[m][n] = sum_{t < terms} sum_k A_t[m][k] B_t[n][k];  y = act(z + bias) + residual
+//   gated   g = A_0 B_0^T, u = A_0 B_1^T;  y = act(g) u           (terms = 1)
+//   batch 2 two products with one B: y_z = A_z B_0^T, z = 0, 1    (plain, terms = 1)
+// A_t[m][k] is at a[t] + m lda[t] + k, or at a[t] + k lda[t] + m when a_mn; B_t likewise by n.
+// Operand bases and pitches are multiples of 16 bytes; those of the other arrays are arbitrary.
+struct DenseProduct {
+  const uint16_t* a[2] = {nullptr, nullptr};
+  const uint16_t* b[2] = {nullptr, nullptr};
+  uint64_t lda[2] = {0, 0}, ldb[2] = {0, 0};
+  bool a_mn = false, b_mn = false, gated = false;
+  int M = 0, N = 0, K = 0;
+  int terms = 1, batch = 1;
+  const uint16_t* bias = nullptr;
+  const uint16_t* residual = nullptr;
+  uint16_t* y[2] = {nullptr, nullptr};
+  uint16_t* pre = nullptr;   // z, or g
+  uint16_t* pre2 = nullptr;  // u
+  uint64_t ldr = 0, ldy[2] = {0, 0}, ldp = 0, ldp2 = 0;
+  int act = 0;
+  bool bf16 = false;
+};
+
+int dense_mma(const DenseProduct& p, cudaStream_t stream, const char* who);

@@ -1,0 +1,606 @@
+// dense_mma.cu — the dense layers' matrix products on tcgen05 (sm_100a).
+//
+// Operands are 16-bit matrices in either order: K-major (the contraction index is contiguous: x
+// and W of the forward products) or MN-major (the output's index is: W in dx = dz W, both operands
+// in dW = dz^T x).  TMA stages 64-deep k-blocks with 128-byte swizzle, the matrix instruction
+// reads either order through its descriptors, and TMA fills what lies outside a matrix with
+// zeros, so no size has to be a multiple of anything.
+//
+// A gated block is one product whose B tile is half gate rows and half up rows: the accumulator
+// then holds g and u of the same outputs side by side in one row of TMEM, and the epilogue of one
+// thread has both.  dx of a gated block is one product of two terms, whose k-blocks follow one
+// another into the same accumulator.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <cstdlib>
+#include <cstring>
+
+#include "dense_internal.h"
+#include "dense_math.cuh"
+#include "eas_internal.h"
+#include "tcgen05_ptx.cuh"
+
+namespace {
+
+using namespace tc;
+using namespace dense;
+
+constexpr int kBK = 64;  // one 128-byte swizzle row
+
+struct alignas(64) Params {
+  CUtensorMap a[2], b[2], y[2], pre, pre2;
+  const uint16_t* bias;
+  const uint16_t* residual;
+  uint16_t* y_ptr[2];
+  uint16_t* pre_ptr;
+  uint16_t* pre2_ptr;
+  int64_t ldr, ldy[2], ldp, ldp2;
+  int M, N;
+  int kb_term;   // k-blocks of one term
+  int kb_total;  // of all terms
+  int mt, nt, tiles;  // tiles along M and N, and of the whole launch
+  int act;
+  bool bf16, batch2, y_tma, pre_tma, pre2_tma, bias_vec, res_vec;
+  int* status;
+};
+
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster, int x,
+                                                 int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(x), "r"(y)
+               : "memory");
+}
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
+// The grid before this one in the stream may still be running: nothing of global memory is touched
+// before it has finished.  The next grid may be set up meanwhile, and waits in the same place.
+__device__ __forceinline__ void grid_order() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// Instruction descriptor, kind::f16: D = f32 (bits 4-5 = 1), A and B formats at bits 7-9 and 10-12
+// (f16 0, bf16 1), A and B major at bits 15 and 16 (1 = MN), N >> 3 at bits 17-22, M >> 4 at 24-28.
+__device__ __forceinline__ uint32_t instr_desc(int m, int n, bool a_mn, bool b_mn, bool bf16) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+template <int CG>
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Descriptor of the 16-deep step kk of a staged k-block.  K-major: rows of 128 bytes, 8 rows per
+// swizzle atom, the step is 32 bytes along the row.  MN-major: 64 k-rows of 64 elements (128
+// bytes) per 64-wide piece, 16 rows per step, the next piece kBK * 128 bytes on.
+template <bool MN>
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, int kk) {
+  return MN ? smem_desc(addr + kk * 2048, kBK * 128, 1024) : smem_desc(addr + kk * 32, 16, 1024);
+}
+
+// After an expired wait: copies in flight land before the CTA's shared memory is given up.
+__device__ __forceinline__ void settle() {
+  const long long t0 = clock64();
+  while (clock64() - t0 < 4000000) {
+  }
+}
+
+// ---------------------------------------------------------------------------
+// epilogue: 32 rows x 32 columns per warp at a time
+// ---------------------------------------------------------------------------
+//
+// Each lane holds one row of 32 f32 columns from TMEM.  Results go through a 2 KB box of the warp
+// (64-byte swizzle: 16-byte chunk j of row r lies at chunk j ^ (r / 2 & 3)) and leave by a TMA
+// store, which clips at the matrix's edges; arrays whose base or pitch TMA cannot take are written
+// from the box row by row, 32 neighbouring columns at a time.  Two boxes per warp take turns.
+
+struct Boxes {
+  uint8_t* base;
+  int n;
+};
+
+constexpr int kBoxBytes = 32 * 64;
+
+__device__ __forceinline__ uint8_t* box_chunk(uint8_t* box, int row, int chunk) {
+  return box + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+}
+
+__device__ __forceinline__ uint8_t* next_box(Boxes& bx, int lane) {
+  uint8_t* box = bx.base + (bx.n & 1) * kBoxBytes;
+  ++bx.n;
+  if (lane == 0) bulk_wait_read1();  // the store that last used this box has read it
+  __syncwarp();
+  return box;
+}
+
+__device__ __forceinline__ void put(Boxes& bx, int lane, const CUtensorMap* map, bool tma, uint16_t* ptr, int64_t ld,
+                                    int M, int N, int m0, int n0, const float (&v)[32], bool bf16) {
+  uint8_t* box = next_box(bx, lane);
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<uint4*>(box_chunk(box, lane, j)) =
+        make_uint4(pack2(v[8 * j], v[8 * j + 1], bf16), pack2(v[8 * j + 2], v[8 * j + 3], bf16),
+                   pack2(v[8 * j + 4], v[8 * j + 5], bf16), pack2(v[8 * j + 6], v[8 * j + 7], bf16));
+  if (tma) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) tma_store_2d(map, box, n0, m0);
+  } else {
+    __syncwarp();
+    const int rows = min(32, M - m0);
+    if (n0 + lane < N)
+      for (int r = 0; r < rows; ++r)
+        ptr[(int64_t)(m0 + r) * ld + n0 + lane] =
+            *reinterpret_cast<const uint16_t*>(box_chunk(box, r, lane >> 3) + (lane & 7) * 2);
+  }
+  if (lane == 0) bulk_commit();  // an empty group where nothing was stored: the boxes' turns count groups
+}
+
+// v += the residual's 32 x 32 piece
+__device__ __forceinline__ void add_residual(const Params& p, Boxes& bx, int lane, int m0, int n0, float (&v)[32]) {
+  uint4 w[4];
+  if (p.res_vec && n0 + 32 <= p.N) {
+    const int m = min(m0 + lane, p.M - 1);  // rows past the last are not stored
+    const uint4* src = reinterpret_cast<const uint4*>(p.residual + (int64_t)m * p.ldr + n0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = src[j];
+  } else {
+    uint8_t* box = next_box(bx, lane);
+    const int rows = min(32, p.M - m0);
+    for (int r = 0; r < rows; ++r)
+      *reinterpret_cast<uint16_t*>(box_chunk(box, r, lane >> 3) + (lane & 7) * 2) =
+          n0 + lane < p.N ? p.residual[(int64_t)(m0 + r) * p.ldr + n0 + lane] : (uint16_t)0;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4*>(box_chunk(box, lane, j));
+    if (lane == 0) bulk_commit();
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t q[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float lo, hi;
+      unpack2(q[i], lo, hi, p.bf16);
+      v[8 * j + 2 * i] += lo;
+      v[8 * j + 2 * i + 1] += hi;
+    }
+  }
+}
+
+__device__ __forceinline__ void add_bias(const Params& p, int n0, float (&v)[32]) {
+  if (p.bias_vec && n0 + 32 <= p.N) {
+    const uint4* src = reinterpret_cast<const uint4*>(p.bias + n0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint4 w = src[j];
+      const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float lo, hi;
+        unpack2(q[i], lo, hi, p.bf16);
+        v[8 * j + 2 * i] += lo;
+        v[8 * j + 2 * i + 1] += hi;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (n0 + j < p.N) v[j] += to_f32(p.bias[n0 + j], p.bf16);
+  }
+}
+
+// Finish 32 x 32 results from their sums: v = z, or v = g and u.
+template <bool GATED>
+__device__ __forceinline__ void finish(const Params& p, Boxes& bx, int lane, int z, int m0, int n0, float (&v)[32],
+                                       const float (&u)[GATED ? 32 : 1]) {
+  if (!GATED && p.bias) add_bias(p, n0, v);
+  if (p.pre_ptr) put(bx, lane, &p.pre, p.pre_tma, p.pre_ptr, p.ldp, p.M, p.N, m0, n0, v, p.bf16);
+  if constexpr (GATED) {
+    if (p.pre2_ptr) put(bx, lane, &p.pre2, p.pre2_tma, p.pre2_ptr, p.ldp2, p.M, p.N, m0, n0, u, p.bf16);
+  }
+  with_act(p.act, [&](auto a) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      v[j] = act<decltype(a)::value>(v[j]);
+      if constexpr (GATED) v[j] *= u[j];
+    }
+  });
+  if (!GATED && p.residual) add_residual(p, bx, lane, m0, n0, v);
+  put(bx, lane, &p.y[z], p.y_tma, p.y_ptr[z], p.ldy[z], p.M, p.N, m0, n0, v, p.bf16);
+}
+
+__device__ __forceinline__ void as_floats(const uint32_t (&r)[32], float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+}
+
+struct Tile {
+  int z, m, n;
+};
+
+// Tiles in groups of 16 along M, so that the tiles in flight share operands in L2.
+__device__ __forceinline__ Tile tile_at(const Params& p, int t) {
+  constexpr int kGroup = 16;
+  Tile c;
+  const int per_z = p.mt * p.nt;
+  c.z = t / per_z;
+  const int r = t - c.z * per_z;
+  const int g = r / (kGroup * p.nt);
+  const int first = g * kGroup;
+  const int size = min(kGroup, p.mt - first);
+  const int rr = r - g * kGroup * p.nt;
+  c.m = first + rr % size;
+  c.n = rr / size;
+  return c;
+}
+
+// ---------------------------------------------------------------------------
+// CTA-pair kernel: 256 x 256 tiles, two accumulators
+// ---------------------------------------------------------------------------
+//
+// A cluster of two CTAs, tcgen05.mma.cta_group::2 of M = 256, N = 256.  Each CTA stages its 128
+// rows of A and 128 of the tile's 256 B rows (gated: CTA 0 the gate's, CTA 1 the up projection's);
+// the leader issues the MMAs, and each CTA's TMEM receives its 128 rows of all 256 columns.  Two
+// accumulators take turns, so the epilogue of one tile runs under the main loop of the next.
+//   warp 0 TMA producer, warp 1 TMEM and (leader) MMA issue, warps 2-9 epilogue: two per TMEM
+//   quarter, one for each half of the columns.
+constexpr int kPairThreads = 320;
+constexpr int kPairStages = 6;
+constexpr int kPairStageBytes = 2 * 128 * kBK * 2;
+constexpr int kPairBoxes = kPairStages * kPairStageBytes;
+constexpr int kPairBars = kPairBoxes + 8 * 2 * kBoxBytes;
+constexpr int kPairSmem = kPairBars + (2 * kPairStages + 4) * 8 + 16 + 1024;
+static_assert(kPairSmem <= 232448, "shared memory over the 227 KB per-CTA limit");
+
+template <bool GATED, bool A_MN, bool B_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    dense_pair_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kPairBars);
+  uint64_t* empty = full + kPairStages;
+  uint64_t* acc_full = empty + kPairStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  uint32_t rank;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&full[s], 1);  // armed by the leader with both CTAs' bytes (the leader's copy is used)
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 16);  // 8 epilogue warps x 2 CTAs (the leader's copy is used)
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    prefetch_map(&p.a[0]);
+    prefetch_map(&p.b[0]);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the peer's barriers are initialised before anyone signals them
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_order();
+
+  const int cid = blockIdx.x >> 1, ncl = gridDim.x >> 1;
+  const int kTileN = GATED ? 128 : 256;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0;
+      for (int t = cid; t < p.tiles && !*abort_flag; t += ncl) {
+        const Tile c = tile_at(p, t);
+        const int m0 = c.m * 256 + 128 * (int)rank;
+        const int n0 = c.n * kTileN + (GATED ? 0 : 128 * (int)rank);
+        for (int kb = 0; kb < p.kb_total; ++kb) {
+          if (!mbar_wait(&empty[s], ph ^ 1, abort_flag)) break;
+          const int term = kb >= p.kb_term ? 1 : 0;
+          const int k0 = (kb - term * p.kb_term) * kBK;
+          const CUtensorMap* ma = &p.a[p.batch2 ? c.z : term];
+          const CUtensorMap* mb = &p.b[GATED ? (int)rank : term];
+          const uint32_t fl = mapa_rank(smem_u32(&full[s]), 0);
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * kPairStageBytes);
+          uint8_t* sa = smem + s * kPairStageBytes;
+          uint8_t* sb = sa + 128 * kBK * 2;
+          if (A_MN) {
+            tma_load_2d_pair(sa, ma, fl, m0, k0);
+            tma_load_2d_pair(sa + kBK * 128, ma, fl, m0 + 64, k0);
+          } else {
+            tma_load_2d_pair(sa, ma, fl, k0, m0);
+          }
+          if (B_MN) {
+            tma_load_2d_pair(sb, mb, fl, n0, k0);
+            tma_load_2d_pair(sb + kBK * 128, mb, fl, n0 + 64, k0);
+          } else {
+            tma_load_2d_pair(sb, mb, fl, k0, n0);
+          }
+          if (++s == kPairStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = instr_desc(256, 256, A_MN, B_MN, p.bf16);
+      int s = 0, local = 0;
+      uint32_t ph = 0;
+      for (int t = cid; t < p.tiles && !*abort_flag; t += ncl, ++local) {
+        const int buf = local & 1;
+        if (!mbar_wait_cl(&acc_empty[buf], ((local >> 1) & 1) ^ 1, abort_flag)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + buf * 256;
+        bool ok = true;
+        for (int kb = 0; kb < p.kb_total; ++kb) {
+          if (!mbar_wait(&full[s], ph, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + s * kPairStageBytes), sb = sa + 128 * kBK * 2;
+#pragma unroll
+          for (int kk = 0; kk < kBK / 16; ++kk)
+            mma_f16<2>(d, operand_desc<A_MN>(sa, kk), operand_desc<B_MN>(sb, kk), idesc, (kb | kk) ? 1u : 0u);
+          asm volatile(
+              "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::
+                  "r"(smem_u32(&empty[s])),
+              "h"((uint16_t)3)
+              : "memory");
+          if (++s == kPairStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+        if (!ok) break;
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                smem_u32(&acc_full[buf])),
+            "h"((uint16_t)3)
+            : "memory");
+      }
+    }
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    Boxes bx = {smem + kPairBoxes + (warp - 2) * 2 * kBoxBytes, 0};
+    const uint32_t leader[2] = {mapa_rank(smem_u32(&acc_empty[0]), 0), mapa_rank(smem_u32(&acc_empty[1]), 0)};
+    int local = 0;
+    for (int t = cid; t < p.tiles && !*abort_flag; t += ncl, ++local) {
+      const int buf = local & 1;
+      if (!mbar_wait(&acc_full[buf], (local >> 1) & 1, abort_flag)) break;
+      tc_fence_after();
+      const Tile c = tile_at(p, t);
+      const int m0 = c.m * 256 + 128 * (int)rank + q * 32;
+      const uint32_t acc = tmem + buf * 256 + ((uint32_t)(q * 32) << 16);
+      constexpr int kCols = GATED ? 64 : 128;  // of this warp
+      if (m0 < p.M) {
+#pragma unroll 1
+        for (int cc = 0; cc < kCols; cc += 32) {
+          const int col = half * kCols + cc, n0 = c.n * kTileN + col;
+          if (n0 >= p.N) break;
+          uint32_t r[32];
+          float v[32], u[GATED ? 32 : 1];
+          tmem_ld32(acc + col, r);
+          as_floats(r, v);
+          if constexpr (GATED) {
+            tmem_ld32(acc + 128 + col, r);
+            as_floats(r, u);
+          }
+          finish<GATED>(p, bx, lane, c.z, m0, n0, v, u);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader[buf]) : "memory");
+    }
+    if (lane == 0) bulk_wait_all0();  // the stores are done before the CTA's shared memory goes away
+  }
+
+  __syncwarp();
+  if (*abort_flag) settle();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the pair leaves together: no MMA still targets the peer's TMEM
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+  if (threadIdx.x == 0 && *abort_flag && p.status) *p.status = EAS_ERR_TIMEOUT;
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+// A row-major matrix [rows][cols] of 16-bit values for TMA boxes of box_rows x box_cols.
+int encode(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows,
+           uint32_t box_cols, CUtensorMapSwizzle swizzle, const char* who) {
+  const cuuint64_t dims[2] = {cols, rows};
+  const cuuint64_t strides[1] = {ld * 2};
+  const cuuint32_t box[2] = {box_cols, box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  // 16-bit words are copied as they are, whichever of the two types they hold; zeros fill the outside
+  return eas_drv_check(
+      g_drv.tensorMapEncodeTiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dims, strides, box,
+                                 estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
+      who, EAS_ERR_VALUE);
+}
+
+bool aligned16(const void* p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld & 7) == 0; }
+
+bool pdl_on() {
+  static const bool on = [] {
+    const char* e = getenv("EAS_PDL");
+    return !(e && (e[0] == '0' || e[0] == 0 || !strcmp(e, "off")));
+  }();
+  return on;
+}
+
+int sm_count(int dev) {
+  static int cached[64] = {0};
+  if (dev < 0 || dev >= 64) return 148;
+  if (!cached[dev]) cudaDeviceGetAttribute(&cached[dev], cudaDevAttrMultiProcessorCount, dev);
+  return cached[dev];
+}
+
+// Operand maps (b_rows: rows of B per box), epilogue arrays, and the tile grid of tile_m x tile_n outputs.
+int fill(Params& q, const DenseProduct& p, int b_rows, int tile_m, int tile_n, const char* who) {
+  int rc = EAS_OK;
+  const int na = p.terms > 1 || p.batch > 1 ? 2 : 1;
+  const int nb = p.terms > 1 || p.gated ? 2 : 1;
+  for (int t = 0; t < na && !rc; ++t)
+    rc = p.a_mn ? encode(&q.a[t], p.a[t], p.K, p.M, p.lda[t], kBK, 64, CU_TENSOR_MAP_SWIZZLE_128B, who)
+                : encode(&q.a[t], p.a[t], p.M, p.K, p.lda[t], 128, kBK, CU_TENSOR_MAP_SWIZZLE_128B, who);
+  for (int t = 0; t < nb && !rc; ++t)
+    rc = p.b_mn ? encode(&q.b[t], p.b[t], p.K, p.N, p.ldb[t], kBK, 64, CU_TENSOR_MAP_SWIZZLE_128B, who)
+                : encode(&q.b[t], p.b[t], p.N, p.K, p.ldb[t], b_rows, kBK, CU_TENSOR_MAP_SWIZZLE_128B, who);
+  if (rc) return rc;
+  q.y_tma = aligned16(p.y[0], p.ldy[0]) && (p.batch < 2 || aligned16(p.y[1], p.ldy[1]));
+  for (int z = 0; z < p.batch && q.y_tma && !rc; ++z)
+    rc = encode(&q.y[z], p.y[z], p.M, p.N, p.ldy[z], 32, 32, CU_TENSOR_MAP_SWIZZLE_64B, who);
+  if (!rc && p.pre && (q.pre_tma = aligned16(p.pre, p.ldp)))
+    rc = encode(&q.pre, p.pre, p.M, p.N, p.ldp, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B, who);
+  if (!rc && p.pre2 && (q.pre2_tma = aligned16(p.pre2, p.ldp2)))
+    rc = encode(&q.pre2, p.pre2, p.M, p.N, p.ldp2, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B, who);
+  if (rc) return rc;
+  q.bias = p.bias, q.residual = p.residual;
+  q.bias_vec = (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0;
+  q.res_vec = aligned16(p.residual, p.ldr);
+  for (int z = 0; z < 2; ++z) q.y_ptr[z] = p.y[z], q.ldy[z] = (int64_t)p.ldy[z];
+  q.pre_ptr = p.pre, q.pre2_ptr = p.pre2;
+  q.ldr = (int64_t)p.ldr, q.ldp = (int64_t)p.ldp, q.ldp2 = (int64_t)p.ldp2;
+  q.M = p.M, q.N = p.N;
+  q.kb_term = (p.K + kBK - 1) / kBK;
+  if ((int64_t)q.kb_term * p.terms > 0x7fffffff) return eas_fail(EAS_ERR_VALUE, "%s: too many products in a sum", who);
+  q.kb_total = q.kb_term * p.terms;
+  const int64_t mt = ((int64_t)p.M + tile_m - 1) / tile_m, nt = ((int64_t)p.N + tile_n - 1) / tile_n;
+  if (mt * nt * p.batch > 0x3fffffff) return eas_fail(EAS_ERR_VALUE, "%s: too many output tiles", who);
+  q.mt = (int)mt, q.nt = (int)nt, q.tiles = (int)(mt * nt * p.batch);
+  q.batch2 = p.batch > 1;
+  q.act = p.act, q.bf16 = p.bf16;
+  return EAS_OK;
+}
+
+int launch(const void* kernel, int blocks, int cluster, int threads, int smem, cudaStream_t s, Params& q,
+           const char* who) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (cluster) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = (unsigned)cluster;
+    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pdl_on()) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = (unsigned)n;
+  void* args[] = {&q};
+  return eas_cuda_check(cudaLaunchKernelExC(&cfg, kernel, args), who, EAS_ERR_LAUNCH);
+}
+
+// Shared-memory opt-in and co-resident clusters of a kernel, once per device.
+struct KernelState {
+  int pairs[64] = {0};
+};
+
+template <bool GATED, bool A_MN, bool B_MN>
+int launch_pair(Params& q, int dev, cudaStream_t s, const char* who) {
+  static KernelState st;
+  const void* kernel = reinterpret_cast<const void*>(&dense_pair_kernel<GATED, A_MN, B_MN>);
+  const int slot = dev >= 0 && dev < 64 ? dev : 0;
+  if (!st.pairs[slot]) {
+    int rc = eas_cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem), who,
+                            EAS_ERR_LAUNCH);
+    if (rc) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * (sm_count(dev) / 2)), 1, 1);
+    cfg.blockDim = dim3(kPairThreads, 1, 1);
+    cfg.dynamicSmemBytes = kPairSmem;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = sm_count(dev) / 2;
+    }
+    st.pairs[slot] = n;
+  }
+  const int pairs = q.tiles < st.pairs[slot] ? q.tiles : st.pairs[slot];
+  return launch(kernel, 2 * pairs, 0, kPairThreads, kPairSmem, s, q, who);
+}
+
+}  // namespace
+
+int dense_mma(const DenseProduct& p, cudaStream_t stream, const char* who) {
+  int dev = 0;
+  int rc = eas_cuda_check(cudaGetDevice(&dev), who, EAS_ERR_UNAVAILABLE);
+  if (rc) return rc;
+  Params q = {};
+  q.status = eas_native_status_dev(dev);
+  rc = fill(q, p, 128, 256, p.gated ? 128 : 256, who);
+  if (rc) return rc;
+  if (p.gated) return launch_pair<true, false, false>(q, dev, stream, who);
+  if (p.a_mn) return launch_pair<false, true, true>(q, dev, stream, who);
+  if (p.b_mn) return launch_pair<false, false, true>(q, dev, stream, who);
+  return launch_pair<false, false, false>(q, dev, stream, who);
+}

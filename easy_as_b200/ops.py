@@ -193,7 +193,20 @@ class _Call:
                     else:
                         ptr, owner = rt.scratch(device, stream, self.what, nbytes)
             cuda_ext.check(getattr(lib, entry)(device, *head, *tail, ptr, nbytes, stream), self.what)
-            rt.finish_native(device, stream, (self.ins, self.outs, owner), sync, capturing)
+            keep = None
+            if not (sync or capturing):
+                # buffers must outlive the launch: torch's allocator learns which stream uses them (its
+                # scratch is that stream's already), the others are kept until it is done
+                bufs = [r.keep for r in self.ins] + [r.keep for _n, r in self.outs]
+                if torch is not None:
+                    on = torch.cuda.current_stream(device)
+                    for b in bufs:
+                        if type(b) is not Tensor:
+                            b.record_stream(on)
+                keep = [b for b in bufs if type(b) is Tensor]
+                if torch is None and owner is not None:
+                    keep.append(owner)
+            rt.finish_native(device, stream, keep, sync, capturing)
 
 
 def _share(a: _Rows, b: _Rows) -> bool:

@@ -472,6 +472,50 @@ def test_streams(cuda_rt):
     assert cuda_rt.in_flight() == 0
 
 
+def test_buffers_of_another_stream(cuda_rt):
+    """Buffers allocated on the default stream, used in another one and dropped while it is busy: their memory is not
+    handed out again before the call is done."""
+    m, n, k, dtype = 256, 512, 512, torch.bfloat16
+    x, w = normal(gen(0), m, k, dtype), normal(gen(1), n, k, dtype, k ** -0.5)
+    want = torch.empty(m, n, device="cuda", dtype=dtype)
+    eas.ops.linear(x, w, want, act="silu")
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        y = torch.empty_like(want)
+        mine = x.clone()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            eas.ops.linear(mine, w, y, act="silu", _sync=False)
+        del mine
+        junk = [torch.full_like(x, float("nan")) for _ in range(4)]   # would take the dropped block
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+        del junk
+    cuda_rt.synchronize()
+
+
+def test_memory_does_not_pile_up(cuda_rt):
+    """Calls that run ahead of the GPU hold neither their scratch nor their callers' dropped buffers."""
+    m, n, k, dtype = 2048, 2048, 256, torch.float16
+    g = gen(0)
+    x, w, dy, pre = (normal(g, *s, dtype) for s in ((m, k), (n, k), (m, n), (m, n)))
+    dx = torch.empty_like(x)
+
+    def step():
+        eas.ops.linear_backward(dy.clone(), x, w, dx=dx, act="gelu", pre=pre, _sync=False)
+
+    step()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    for _ in range(100):
+        step()
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before <= 4 * dy.numel() * 2
+    cuda_rt.synchronize()
+
+
 def test_eas_tensors(cuda_rt):
     """eas.Tensor buffers (f16) give what torch tensors give, mixed with them too."""
     m, n, k = 33, 136, 72
