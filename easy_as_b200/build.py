@@ -32,7 +32,7 @@ def sources() -> list[Path]:
 
 
 def _flags(ptxas_verbose: bool = False) -> list[str]:
-    return [*ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC", "-cudart", "static",
+    return [*ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC", "-cudart", "static", "-t0",
             *(["-Xptxas", "-v"] if ptxas_verbose else [])]
 
 

@@ -201,6 +201,7 @@ struct Scratch {
 
 Scratch forward_scratch(bool gated, uint32_t M, uint32_t N, uint32_t K, int off) {
   Scratch s(N, K);
+  if (dense_rows_fit((int)M, (int)K)) return s;
   if (off & kXOff) s.x = s.take(2 * (uint64_t)M * s.ldk);
   if (off & kWOff) s.w = s.take(2 * (uint64_t)N * s.ldk);
   if (gated && (off & kUpOff)) s.up = s.take(2 * (uint64_t)N * s.ldk);
@@ -287,15 +288,21 @@ extern "C" int eas_dense_scratch(int op, uint32_t M, uint32_t N, uint32_t K, int
   return EAS_OK;
 }
 
-extern "C" int eas_linear(int dev, const void* x, const void* w, const void* bias, const void* residual, void* y,
-                          void* pre, uint32_t M, uint32_t N, uint32_t K, uint64_t ldx, uint64_t ldw, uint64_t ldr,
-                          uint64_t ldy, uint64_t ldp, int dtype, int act, void* scratch, uint64_t scratch_bytes,
-                          void* stream) {
+extern "C" int eas_linear(const eas_linear_args* args, void* stream) {
   const char* who = "eas_linear";
+  if (!args) return eas_fail(EAS_ERR_VALUE, "%s: null arguments", who);
+  const void *const x = args->x, *const w = args->w, *const bias = args->bias, *const residual = args->residual;
+  void *const y = args->y, *const pre = args->pre;
+  const uint64_t ldx = args->ldx, ldw = args->ldw, ldr = args->ldr, ldy = args->ldy, ldp = args->ldp;
+  const uint32_t M = args->M, N = args->N, K = args->K;
+  const int dev = args->dev, dtype = args->dtype, act = args->act;
+  void* const scratch = args->scratch;
+  const uint64_t scratch_bytes = args->scratch_bytes;
   int rc = check_sizes(who, M, N, K, dtype, act);
   if (rc || M == 0) return rc;
   if (!x || !w || !y) return eas_fail(EAS_ERR_VALUE, "%s: null operand", who);
-  const int off = off_mask(x, ldx, kXOff) | off_mask(w, ldw, kWOff);
+  const bool few = dense_rows_fit((int)M, (int)K);
+  const int off = few ? 0 : off_mask(x, ldx, kXOff) | off_mask(w, ldw, kWOff);
   const Scratch sc = forward_scratch(false, M, N, K, off);
   if ((rc = check_scratch(who, sc, scratch, scratch_bytes))) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -310,18 +317,24 @@ extern "C" int eas_linear(int dev, const void* x, const void* w, const void* bia
   p.bias = u16(bias), p.residual = u16(residual), p.y[0] = u16(y), p.pre = u16(pre);
   p.ldr = ldr, p.ldy[0] = ldy, p.ldp = ldp;
   p.act = act, p.bf16 = dtype == kBF16;
-  return dense_mma(p, s, who);
+  return few ? dense_rows(p, s, who) : dense_mma(p, s, who);
 }
 
-extern "C" int eas_gated(int dev, const void* x, const void* w_gate, const void* w_up, void* h, void* gate, void* up,
-                         uint32_t M, uint32_t N, uint32_t K, uint64_t ldx, uint64_t ldwg, uint64_t ldwu, uint64_t ldh,
-                         uint64_t ldg, uint64_t ldu, int dtype, int act, void* scratch, uint64_t scratch_bytes,
-                         void* stream) {
+extern "C" int eas_gated(const eas_gated_args* args, void* stream) {
   const char* who = "eas_gated";
+  if (!args) return eas_fail(EAS_ERR_VALUE, "%s: null arguments", who);
+  const void *const x = args->x, *const w_gate = args->w_gate, *const w_up = args->w_up;
+  void *const h = args->h, *const gate = args->gate, *const up = args->up;
+  const uint64_t ldx = args->ldx, ldwg = args->ldwg, ldwu = args->ldwu, ldh = args->ldh, ldg = args->ldg, ldu = args->ldu;
+  const uint32_t M = args->M, N = args->N, K = args->K;
+  const int dev = args->dev, dtype = args->dtype, act = args->act;
+  void* const scratch = args->scratch;
+  const uint64_t scratch_bytes = args->scratch_bytes;
   int rc = check_sizes(who, M, N, K, dtype, act);
   if (rc || M == 0) return rc;
   if (!x || !w_gate || !w_up || !h) return eas_fail(EAS_ERR_VALUE, "%s: null operand", who);
-  const int off = off_mask(x, ldx, kXOff) | off_mask(w_gate, ldwg, kWOff) | off_mask(w_up, ldwu, kUpOff);
+  const bool few = dense_rows_fit((int)M, (int)K);
+  const int off = few ? 0 : off_mask(x, ldx, kXOff) | off_mask(w_gate, ldwg, kWOff) | off_mask(w_up, ldwu, kUpOff);
   const Scratch sc = forward_scratch(true, M, N, K, off);
   if ((rc = check_scratch(who, sc, scratch, scratch_bytes))) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -338,14 +351,19 @@ extern "C" int eas_gated(int dev, const void* x, const void* w_gate, const void*
   p.y[0] = u16(h), p.pre = u16(gate), p.pre2 = u16(up);
   p.ldy[0] = ldh, p.ldp = ldg, p.ldp2 = ldu;
   p.act = act, p.bf16 = dtype == kBF16;
-  return dense_mma(p, s, who);
+  return few ? dense_rows(p, s, who) : dense_mma(p, s, who);
 }
 
-extern "C" int eas_linear_backward(int dev, const void* dy, const void* pre, const void* x, const void* w, void* dx,
-                                   void* dw, void* db, uint32_t M, uint32_t N, uint32_t K, uint64_t lddy, uint64_t ldp,
-                                   uint64_t ldx, uint64_t ldw, uint64_t lddx, uint64_t lddw, int dtype, int act,
-                                   void* scratch, uint64_t scratch_bytes, void* stream) {
+extern "C" int eas_linear_backward(const eas_linear_backward_args* args, void* stream) {
   const char* who = "eas_linear_backward";
+  if (!args) return eas_fail(EAS_ERR_VALUE, "%s: null arguments", who);
+  const void *const dy = args->dy, *const pre = args->pre, *const x = args->x, *const w = args->w;
+  void *const dx = args->dx, *const dw = args->dw, *const db = args->db;
+  const uint64_t lddy = args->lddy, ldp = args->ldp, ldx = args->ldx, ldw = args->ldw, lddx = args->lddx, lddw = args->lddw;
+  const uint32_t M = args->M, N = args->N, K = args->K;
+  const int dev = args->dev, dtype = args->dtype, act = args->act;
+  void* const scratch = args->scratch;
+  const uint64_t scratch_bytes = args->scratch_bytes;
   int rc = check_sizes(who, M, N, K, dtype, act);
   if (rc) return rc;
   if ((M && !dy) || (M && act != kNone && !pre) || (dx && !w) || (M && dw && !x))
@@ -386,13 +404,16 @@ extern "C" int eas_linear_backward(int dev, const void* dy, const void* pre, con
   return backward_products(who, 1, {DZ, {}}, {W, {}}, X, dx, lddx, {dw, nullptr}, {lddw, 0}, M, N, K, dtype, s);
 }
 
-extern "C" int eas_gated_backward(int dev, const void* dh, const void* gate, const void* up, const void* x,
-                                  const void* w_gate, const void* w_up, void* dx, void* dw_gate, void* dw_up,
-                                  uint32_t M, uint32_t N, uint32_t K, uint64_t lddh, uint64_t ldg, uint64_t ldu,
-                                  uint64_t ldx, uint64_t ldwg, uint64_t ldwu, uint64_t lddx, uint64_t lddwg,
-                                  uint64_t lddwu, int dtype, int act, void* scratch, uint64_t scratch_bytes,
-                                  void* stream) {
+extern "C" int eas_gated_backward(const eas_gated_backward_args* args, void* stream) {
   const char* who = "eas_gated_backward";
+  if (!args) return eas_fail(EAS_ERR_VALUE, "%s: null arguments", who);
+  const void *const dh = args->dh, *const gate = args->gate, *const up = args->up, *const x = args->x, *const w_gate = args->w_gate, *const w_up = args->w_up;
+  void *const dx = args->dx, *const dw_gate = args->dw_gate, *const dw_up = args->dw_up;
+  const uint64_t lddh = args->lddh, ldg = args->ldg, ldu = args->ldu, ldx = args->ldx, ldwg = args->ldwg, ldwu = args->ldwu, lddx = args->lddx, lddwg = args->lddwg, lddwu = args->lddwu;
+  const uint32_t M = args->M, N = args->N, K = args->K;
+  const int dev = args->dev, dtype = args->dtype, act = args->act;
+  void* const scratch = args->scratch;
+  const uint64_t scratch_bytes = args->scratch_bytes;
   int rc = check_sizes(who, M, N, K, dtype, act);
   if (rc) return rc;
   if ((M && (!dh || !gate || !up)) || (dx && (!w_gate || !w_up)) || (M && (dw_gate || dw_up) && !x))

@@ -27,3 +27,9 @@ struct DenseProduct {
 };
 
 int dense_mma(const DenseProduct& p, cudaStream_t stream, const char* who);
+
+// The same for the forward products (K-major operands, one term, one product) of at most kDenseRows
+// rows that fit in shared memory; operands of any alignment.
+constexpr int kDenseRows = 8;
+bool dense_rows_fit(int M, int K);
+int dense_rows(const DenseProduct& p, cudaStream_t stream, const char* who);

@@ -14,10 +14,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <cstdlib>
-#include <cstring>
-
 #include "dense_internal.h"
+#include "dense_launch.h"
 #include "dense_math.cuh"
 #include "eas_internal.h"
 #include "tcgen05_ptx.cuh"
@@ -41,26 +39,64 @@ struct alignas(64) Params {
   int kb_term;   // k-blocks of one term
   int kb_total;  // of all terms
   int mt, nt, tiles;  // tiles along M and N, and of the whole launch
+  int split;          // CTAs of a cluster that share a tile's k-blocks
   int act;
   bool bf16, batch2, y_tma, pre_tma, pre2_tma, bias_vec, res_vec;
   int* status;
 };
 
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+// The producer and MMA warps run their loops whole, one elected lane issuing: every address and
+// descriptor is then uniform over the warp and stays in uniform registers, which these
+// instructions want.  (Issued from a branch of one lane they came from vector registers, and a
+// k-block took 566 cycles to issue whatever its tile: 300 ns per k-block, above the 270 ns that
+// a 256 x 256 x 64 pair k-block computes.)
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
-          smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y)
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}" ::
+          "r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
       : "memory");
 }
 
-__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster, int x,
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar_cluster, int x,
                                                  int y) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
-      "[%2];" ::"r"(smem_u32(dst)),
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+      "%4}], [%2];\n\t}" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y)
       : "memory");
+}
+
+__device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+      "r"(bytes)
+      : "memory");
+}
+
+// Arrive on `bar` when the MMAs issued so far are done; CG = 2: in both CTAs of the pair.
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::
+            "r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+        : "memory");
 }
 
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
@@ -88,31 +124,62 @@ __device__ __forceinline__ uint32_t instr_desc(int m, int n, bool a_mn, bool b_m
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-template <int CG>
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Descriptor of a staged k-block.  K-major: rows of 128 bytes, 8 rows per swizzle atom; a step of
+// 16 is 32 bytes along the row.  MN-major: 64 k-rows of 64 elements (128 bytes) per 64-wide piece,
+// the next piece kBK * 128 bytes on; a step is 16 rows.  Descriptors count in 16-byte units.
+template <bool MN>
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
+  return MN ? smem_desc(addr, kBK * 128, 1024) : smem_desc(addr, 16, 1024);
+}
+template <bool MN>
+constexpr int kStep = MN ? 2048 / 16 : 32 / 16;
+
+// The four 16-deep MMAs of a k-block; the first overwrites D unless `accumulate`.
+#define EAS_MMA_KBLOCK(GROUP)                                                                            \
+  asm volatile(                                                                                          \
+      "{\n\t.reg .pred e, p, t;\n\t.reg .b64 a, b;\n\t"                                                  \
+      "elect.sync _|e, 0xffffffff;\n\t"                                                                  \
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"                                                \
+      "@e tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], %1, %2, %3, p;\n\t"                           \
+      "add.s64 a, %1, %5;\n\tadd.s64 b, %2, %6;\n\t"                                                     \
+      "@e tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], a, b, %3, t;\n\t"                             \
+      "add.s64 a, a, %5;\n\tadd.s64 b, b, %6;\n\t"                                                       \
+      "@e tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], a, b, %3, t;\n\t"                             \
+      "add.s64 a, a, %5;\n\tadd.s64 b, b, %6;\n\t"                                                       \
+      "@e tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], a, b, %3, t;\n\t}" ::"r"(d),                  \
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "n"(kStep<A_MN>), "n"(kStep<B_MN>)          \
+      : "memory")
+
+template <int CG, bool A_MN, bool B_MN>
+__device__ __forceinline__ void mma_kblock(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
   if constexpr (CG == 2)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
+    EAS_MMA_KBLOCK("2");
   else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
+    EAS_MMA_KBLOCK("1");
+}
+#undef EAS_MMA_KBLOCK
+
+// A whole warp's bounded wait (tc::mbar_wait is one thread's): the same answer in every lane, so
+// that the warp leaves its loop together when a wait expires.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  auto done = [&]() {
+    return __all_sync(0xffffffffu, CLUSTER ? mbar_try_wait_cl(smem_u32(bar), parity) : mbar_try_wait(bar, parity));
+  };
+  if (done()) return true;
+  const long long t0 = clock64();
+  while (!done()) {
+    const bool expired = clock64() - t0 > kWaitBudget;
+    if (__any_sync(0xffffffffu, expired || *abort_flag)) {
+      *abort_flag = 1;
+      return false;
+    }
+  }
+  return true;
 }
 
-// Descriptor of the 16-deep step kk of a staged k-block.  K-major: rows of 128 bytes, 8 rows per
-// swizzle atom, the step is 32 bytes along the row.  MN-major: 64 k-rows of 64 elements (128
-// bytes) per 64-wide piece, 16 rows per step, the next piece kBK * 128 bytes on.
-template <bool MN>
-__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, int kk) {
-  return MN ? smem_desc(addr + kk * 2048, kBK * 128, 1024) : smem_desc(addr + kk * 32, 16, 1024);
-}
+__device__ __forceinline__ bool going(volatile int* abort_flag) { return !__any_sync(0xffffffffu, *abort_flag); }
 
 // After an expired wait: copies in flight land before the CTA's shared memory is given up.
 __device__ __forceinline__ void settle() {
@@ -300,7 +367,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);  // uniform
   const int lane = threadIdx.x & 31;
   uint32_t rank;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -329,86 +396,77 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   __syncthreads();
   cluster_sync_all();  // the peer's barriers are initialised before anyone signals them
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   grid_order();
 
   const int cid = blockIdx.x >> 1, ncl = gridDim.x >> 1;
   const int kTileN = GATED ? 128 : 256;
 
+  const uint32_t ring = smem_u32(smem), full0 = smem_u32(full), empty0 = smem_u32(empty);
+
   if (warp == 0) {
-    if (lane == 0) {
-      int s = 0;
-      uint32_t ph = 0;
-      for (int t = cid; t < p.tiles && !*abort_flag; t += ncl) {
-        const Tile c = tile_at(p, t);
-        const int m0 = c.m * 256 + 128 * (int)rank;
-        const int n0 = c.n * kTileN + (GATED ? 0 : 128 * (int)rank);
-        for (int kb = 0; kb < p.kb_total; ++kb) {
-          if (!mbar_wait(&empty[s], ph ^ 1, abort_flag)) break;
-          const int term = kb >= p.kb_term ? 1 : 0;
-          const int k0 = (kb - term * p.kb_term) * kBK;
-          const CUtensorMap* ma = &p.a[p.batch2 ? c.z : term];
-          const CUtensorMap* mb = &p.b[GATED ? (int)rank : term];
-          const uint32_t fl = mapa_rank(smem_u32(&full[s]), 0);
-          if (rank == 0) mbar_expect_tx(&full[s], 2 * kPairStageBytes);
-          uint8_t* sa = smem + s * kPairStageBytes;
-          uint8_t* sb = sa + 128 * kBK * 2;
-          if (A_MN) {
-            tma_load_2d_pair(sa, ma, fl, m0, k0);
-            tma_load_2d_pair(sa + kBK * 128, ma, fl, m0 + 64, k0);
-          } else {
-            tma_load_2d_pair(sa, ma, fl, k0, m0);
-          }
-          if (B_MN) {
-            tma_load_2d_pair(sb, mb, fl, n0, k0);
-            tma_load_2d_pair(sb + kBK * 128, mb, fl, n0 + 64, k0);
-          } else {
-            tma_load_2d_pair(sb, mb, fl, k0, n0);
-          }
-          if (++s == kPairStages) {
-            s = 0;
-            ph ^= 1;
-          }
+    const uint32_t leader_full = mapa_rank(full0, 0);
+    int s = 0;
+    uint32_t ph = 0;
+    for (int t = cid; t < p.tiles && going(abort_flag); t += ncl) {
+      const Tile c = tile_at(p, t);
+      const int m0 = c.m * 256 + 128 * (int)rank;
+      const int n0 = c.n * kTileN + (GATED ? 0 : 128 * (int)rank);
+      int term = 0, k0 = 0;
+      for (int kb = 0; kb < p.kb_total; ++kb) {
+        if (!warp_wait(&empty[s], ph ^ 1, abort_flag)) break;
+        if (kb == p.kb_term) term = 1, k0 = 0;
+        const CUtensorMap* ma = &p.a[p.batch2 ? c.z : term];
+        const CUtensorMap* mb = &p.b[GATED ? (int)rank : term];
+        const uint32_t fl = leader_full + s * 8;
+        if (rank == 0) expect_tx(full0 + s * 8, 2 * kPairStageBytes);
+        const uint32_t sa = ring + s * kPairStageBytes, sb = sa + 128 * kBK * 2;
+        if (A_MN) {
+          tma_load_2d_pair(sa, ma, fl, m0, k0);
+          tma_load_2d_pair(sa + kBK * 128, ma, fl, m0 + 64, k0);
+        } else {
+          tma_load_2d_pair(sa, ma, fl, k0, m0);
+        }
+        if (B_MN) {
+          tma_load_2d_pair(sb, mb, fl, n0, k0);
+          tma_load_2d_pair(sb + kBK * 128, mb, fl, n0 + 64, k0);
+        } else {
+          tma_load_2d_pair(sb, mb, fl, k0, n0);
+        }
+        k0 += kBK;
+        if (++s == kPairStages) {
+          s = 0;
+          ph ^= 1;
         }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       const uint32_t idesc = instr_desc(256, 256, A_MN, B_MN, p.bf16);
+      const uint64_t a0 = operand_desc<A_MN>(ring), b0 = operand_desc<B_MN>(ring + 128 * kBK * 2);
       int s = 0, local = 0;
       uint32_t ph = 0;
-      for (int t = cid; t < p.tiles && !*abort_flag; t += ncl, ++local) {
+      for (int t = cid; t < p.tiles && going(abort_flag); t += ncl, ++local) {
         const int buf = local & 1;
-        if (!mbar_wait_cl(&acc_empty[buf], ((local >> 1) & 1) ^ 1, abort_flag)) break;
+        if (!warp_wait<true>(&acc_empty[buf], ((local >> 1) & 1) ^ 1, abort_flag)) break;
         tc_fence_after();
         const uint32_t d = tmem + buf * 256;
         bool ok = true;
         for (int kb = 0; kb < p.kb_total; ++kb) {
-          if (!mbar_wait(&full[s], ph, abort_flag)) {
+          if (!warp_wait(&full[s], ph, abort_flag)) {
             ok = false;
             break;
           }
-          tc_fence_after();
-          const uint32_t sa = smem_u32(smem + s * kPairStageBytes), sb = sa + 128 * kBK * 2;
-#pragma unroll
-          for (int kk = 0; kk < kBK / 16; ++kk)
-            mma_f16<2>(d, operand_desc<A_MN>(sa, kk), operand_desc<B_MN>(sb, kk), idesc, (kb | kk) ? 1u : 0u);
-          asm volatile(
-              "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::
-                  "r"(smem_u32(&empty[s])),
-              "h"((uint16_t)3)
-              : "memory");
+          const uint64_t at = (uint64_t)(s * (kPairStageBytes / 16));
+          mma_kblock<2, A_MN, B_MN>(d, a0 + at, b0 + at, idesc, kb);
+          commit<2>(empty0 + s * 8);
           if (++s == kPairStages) {
             s = 0;
             ph ^= 1;
           }
         }
         if (!ok) break;
-        asm volatile(
-            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-                smem_u32(&acc_full[buf])),
-            "h"((uint16_t)3)
-            : "memory");
+        commit<2>(smem_u32(&acc_full[buf]));
       }
     }
   } else {
@@ -416,9 +474,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     Boxes bx = {smem + kPairBoxes + (warp - 2) * 2 * kBoxBytes, 0};
     const uint32_t leader[2] = {mapa_rank(smem_u32(&acc_empty[0]), 0), mapa_rank(smem_u32(&acc_empty[1]), 0)};
     int local = 0;
-    for (int t = cid; t < p.tiles && !*abort_flag; t += ncl, ++local) {
+    for (int t = cid; t < p.tiles && going(abort_flag); t += ncl, ++local) {
       const int buf = local & 1;
-      if (!mbar_wait(&acc_full[buf], (local >> 1) & 1, abort_flag)) break;
+      if (!warp_wait(&acc_full[buf], (local >> 1) & 1, abort_flag)) break;
       tc_fence_after();
       const Tile c = tile_at(p, t);
       const int m0 = c.m * 256 + 128 * (int)rank + q * 32;
@@ -461,6 +519,211 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 }
 
 // ---------------------------------------------------------------------------
+// single-CTA kernel: 128 x BN tiles, K split over a cluster
+// ---------------------------------------------------------------------------
+//
+// For outputs of too few 256 x 256 tiles.  One tile per cluster of S CTAs (S = 1, 2, 4, 8), each
+// with its share of the k-blocks; two CTAs fit on an SM, so one's epilogue runs beside the
+// other's main loop.  With S > 1 every CTA leaves its f32 sums in shared memory (column-major, over
+// the ring, which is idle by then), and the cluster's warps share out the 32 x 32 pieces: a piece is
+// summed over the CTAs in their order, through distributed shared memory, and finished.  No
+// workspace, no atomics: the same bits on every run.
+//   warp 0 TMA producer, warp 1 TMEM and MMA issue, warps 2-5 epilogue (one per TMEM quarter).
+//
+// Shapes: AR rows of A are staged (64 when the matrix has no more: the MMA then reads the rows
+// behind them too, whatever they hold, into accumulator rows that nobody looks at).  DEEP rings
+// take the whole SM, for launches of no more CTAs than SMs; else two CTAs share one.
+constexpr int kTileThreads = 192;
+template <int BN, int AR, bool DEEP>
+struct TileShape {
+  static constexpr int kABytes = AR * kBK * 2;
+  static constexpr int kStageBytes = kABytes + BN * kBK * 2;
+  static constexpr int kStages = (DEEP ? 196608 : 98304) / kStageBytes;
+  static constexpr int kRing = kStages * kStageBytes;
+  static constexpr int kOver = 128 * kBK * 2 > kStageBytes ? 128 * kBK * 2 - kStageBytes : 0;  // read past the ring
+  static constexpr int kBoxes = 128 * BN * 4;  // after the partial sums, over the ring
+  static constexpr int kBars = kRing + kOver;
+  static constexpr int kSmem = kBars + (2 * kStages + 1) * 8 + 16 + 1024;
+  static_assert(kBoxes + 4 * 2 * kBoxBytes <= kRing, "partial sums and boxes lie over the ring");
+  static_assert(kSmem <= (DEEP ? 232448 : 115000), "shared memory");
+};
+
+template <int BN, int AR, bool DEEP, bool GATED, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(const __grid_constant__ Params p) {
+  static_assert(AR == 128 || !A_MN, "MN-major A comes in 64-wide pieces of all 128 rows");
+  using L = TileShape<BN, AR, DEEP>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);
+  uint64_t* empty = full + L::kStages;
+  uint64_t* acc_full = empty + L::kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);  // uniform
+  const int lane = threadIdx.x & 31;
+  const int S = p.split;
+  const int rank = (int)blockIdx.x % S;  // consecutive blocks form a cluster
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < L::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    prefetch_map(&p.a[0]);
+    prefetch_map(&p.b[0]);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(BN)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  grid_order();
+
+  constexpr int kTileN = GATED ? BN / 2 : BN;
+  const Tile c = tile_at(p, (int)blockIdx.x / S);
+  const int m0 = c.m * 128, n0 = c.n * kTileN;
+  const int kb_lo = (int)((int64_t)rank * p.kb_total / S), kb_hi = (int)((int64_t)(rank + 1) * p.kb_total / S);
+
+  const uint32_t ring = smem_u32(smem), full0 = smem_u32(full), empty0 = smem_u32(empty);
+
+  if (warp == 0) {
+    int s = 0;
+    uint32_t ph = 0;
+    for (int kb = kb_lo; kb < kb_hi; ++kb) {
+      if (!warp_wait(&empty[s], ph ^ 1, abort_flag)) break;
+      const uint32_t fl = full0 + s * 8;
+      expect_tx(fl, L::kStageBytes);
+      const int term = kb >= p.kb_term ? 1 : 0;
+      const int k0 = (kb - term * p.kb_term) * kBK;
+      const CUtensorMap* ma = &p.a[p.batch2 ? c.z : term];
+      const uint32_t sa = ring + s * L::kStageBytes, sb = sa + L::kABytes;
+      if (A_MN) {
+        tma_load_2d(sa, ma, fl, m0, k0);
+        tma_load_2d(sa + kBK * 128, ma, fl, m0 + 64, k0);
+      } else {
+        tma_load_2d(sa, ma, fl, k0, m0);
+      }
+      if (GATED) {
+        tma_load_2d(sb, &p.b[0], fl, k0, n0);
+        tma_load_2d(sb + kTileN * 128, &p.b[1], fl, k0, n0);
+      } else if (B_MN) {
+#pragma unroll
+        for (int j = 0; j < BN / 64; ++j) tma_load_2d(sb + j * kBK * 128, &p.b[term], fl, n0 + 64 * j, k0);
+      } else {
+        tma_load_2d(sb, &p.b[term], fl, k0, n0);
+      }
+      if (++s == L::kStages) {
+        s = 0;
+        ph ^= 1;
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t idesc = instr_desc(128, BN, A_MN, B_MN, p.bf16);
+    const uint64_t a0 = operand_desc<A_MN>(ring), b0 = operand_desc<B_MN>(ring + L::kABytes);
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int kb = kb_lo; kb < kb_hi; ++kb) {
+      if (!warp_wait(&full[s], ph, abort_flag)) {
+        ok = false;
+        break;
+      }
+      const uint64_t at = (uint64_t)(s * (L::kStageBytes / 16));
+      mma_kblock<1, A_MN, B_MN>(tmem, a0 + at, b0 + at, idesc, kb - kb_lo);
+      commit<1>(empty0 + s * 8);
+      if (++s == L::kStages) {
+        s = 0;
+        ph ^= 1;
+      }
+    }
+    if (ok) commit<1>(smem_u32(acc_full));
+  } else if (warp_wait(acc_full, 0, abort_flag)) {
+    // every MMA has read its operands: the ring is free
+    tc_fence_after();
+    const int q = warp & 3;
+    const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16);
+    if (S == 1) {
+      Boxes bx = {smem + L::kBoxes + q * 2 * kBoxBytes, 0};
+      if (m0 + q * 32 < p.M) {
+#pragma unroll 1
+        for (int cc = 0; cc < kTileN && n0 + cc < p.N; cc += 32) {
+          uint32_t r[32];
+          float v[32], u[GATED ? 32 : 1];
+          tmem_ld32(acc + cc, r);
+          as_floats(r, v);
+          if constexpr (GATED) {
+            tmem_ld32(acc + kTileN + cc, r);
+            as_floats(r, u);
+          }
+          finish<GATED>(p, bx, lane, c.z, m0 + q * 32, n0 + cc, v, u);
+        }
+      }
+      if (lane == 0) bulk_wait_all0();
+    } else if (m0 + q * 32 < p.M) {
+      float* part = reinterpret_cast<float*>(smem) + q * 32 + lane;
+#pragma unroll 1
+      for (int cc = 0; cc < BN; cc += 32) {
+        uint32_t r[32];
+        tmem_ld32(acc + cc, r);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) part[(cc + j) * 128] = __uint_as_float(r[j]);
+      }
+    }
+  }
+
+  __syncwarp();
+  if (*abort_flag) settle();
+  if (S > 1) {
+    cluster_sync_all();  // every CTA's sums are in its shared memory
+    if (warp >= 2) {
+      const int e = warp - 2;
+      Boxes bx = {smem + L::kBoxes + e * 2 * kBoxBytes, 0};
+      const int quarters = min(4, (p.M - m0 + 31) / 32);
+      const int pieces = min(kTileN, p.N - n0 + 31) / 32 * quarters;
+      for (int i = rank + e * S; i < pieces; i += 4 * S) {
+        const int q = i % quarters, cc = i / quarters * 32;
+        const uint32_t at = smem_u32(smem) + (uint32_t)(cc * 128 + q * 32 + lane) * 4;
+        float v[32], u[GATED ? 32 : 1];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = 0;
+        if constexpr (GATED) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) u[j] = 0;
+        }
+        for (int s = 0; s < S; ++s) {
+          const uint32_t from = mapa_rank(at, (uint32_t)s);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += ld_cluster_f32(from + j * 512);
+          if constexpr (GATED) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) u[j] += ld_cluster_f32(from + (kTileN + j) * 512);
+          }
+        }
+        finish<GATED>(p, bx, lane, c.z, m0 + q * 32, n0 + cc, v, u);
+      }
+      if (lane == 0) bulk_wait_all0();
+    }
+    __syncwarp();
+    cluster_sync_all();  // nobody leaves while its sums are being read
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(BN) : "memory");
+  }
+  if (threadIdx.x == 0 && *abort_flag && p.status) *p.status = EAS_ERR_TIMEOUT;
+}
+
+// ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 
@@ -481,29 +744,14 @@ int encode(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uin
 
 bool aligned16(const void* p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld & 7) == 0; }
 
-bool pdl_on() {
-  static const bool on = [] {
-    const char* e = getenv("EAS_PDL");
-    return !(e && (e[0] == '0' || e[0] == 0 || !strcmp(e, "off")));
-  }();
-  return on;
-}
-
-int sm_count(int dev) {
-  static int cached[64] = {0};
-  if (dev < 0 || dev >= 64) return 148;
-  if (!cached[dev]) cudaDeviceGetAttribute(&cached[dev], cudaDevAttrMultiProcessorCount, dev);
-  return cached[dev];
-}
-
-// Operand maps (b_rows: rows of B per box), epilogue arrays, and the tile grid of tile_m x tile_n outputs.
-int fill(Params& q, const DenseProduct& p, int b_rows, int tile_m, int tile_n, const char* who) {
+// Operand maps (a_rows, b_rows: rows of a K-major operand per box), epilogue arrays, and the tile grid of tile_m x tile_n outputs.
+int fill(Params& q, const DenseProduct& p, int a_rows, int b_rows, int tile_m, int tile_n, const char* who) {
   int rc = EAS_OK;
   const int na = p.terms > 1 || p.batch > 1 ? 2 : 1;
   const int nb = p.terms > 1 || p.gated ? 2 : 1;
   for (int t = 0; t < na && !rc; ++t)
     rc = p.a_mn ? encode(&q.a[t], p.a[t], p.K, p.M, p.lda[t], kBK, 64, CU_TENSOR_MAP_SWIZZLE_128B, who)
-                : encode(&q.a[t], p.a[t], p.M, p.K, p.lda[t], 128, kBK, CU_TENSOR_MAP_SWIZZLE_128B, who);
+                : encode(&q.a[t], p.a[t], p.M, p.K, p.lda[t], a_rows, kBK, CU_TENSOR_MAP_SWIZZLE_128B, who);
   for (int t = 0; t < nb && !rc; ++t)
     rc = p.b_mn ? encode(&q.b[t], p.b[t], p.K, p.N, p.ldb[t], kBK, 64, CU_TENSOR_MAP_SWIZZLE_128B, who)
                 : encode(&q.b[t], p.b[t], p.N, p.K, p.ldb[t], b_rows, kBK, CU_TENSOR_MAP_SWIZZLE_128B, who);
@@ -534,32 +782,6 @@ int fill(Params& q, const DenseProduct& p, int b_rows, int tile_m, int tile_n, c
   return EAS_OK;
 }
 
-int launch(const void* kernel, int blocks, int cluster, int threads, int smem, cudaStream_t s, Params& q,
-           const char* who) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks, 1, 1);
-  cfg.blockDim = dim3((unsigned)threads, 1, 1);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = s;
-  cudaLaunchAttribute at[2];
-  int n = 0;
-  if (cluster) {
-    at[n].id = cudaLaunchAttributeClusterDimension;
-    at[n].val.clusterDim.x = (unsigned)cluster;
-    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  if (pdl_on()) {
-    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
-  cfg.attrs = at;
-  cfg.numAttrs = (unsigned)n;
-  void* args[] = {&q};
-  return eas_cuda_check(cudaLaunchKernelExC(&cfg, kernel, args), who, EAS_ERR_LAUNCH);
-}
-
 // Shared-memory opt-in and co-resident clusters of a kernel, once per device.
 struct KernelState {
   int pairs[64] = {0};
@@ -575,18 +797,96 @@ int launch_pair(Params& q, int dev, cudaStream_t s, const char* who) {
                             EAS_ERR_LAUNCH);
     if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(2 * (sm_count(dev) / 2)), 1, 1);
+    cfg.gridDim = dim3((unsigned)(2 * (dense_sms(dev) / 2)), 1, 1);
     cfg.blockDim = dim3(kPairThreads, 1, 1);
     cfg.dynamicSmemBytes = kPairSmem;
     int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
       cudaGetLastError();
-      n = sm_count(dev) / 2;
+      n = dense_sms(dev) / 2;
     }
     st.pairs[slot] = n;
   }
   const int pairs = q.tiles < st.pairs[slot] ? q.tiles : st.pairs[slot];
-  return launch(kernel, 2 * pairs, 0, kPairThreads, kPairSmem, s, q, who);
+  return dense_launch(kernel, 2 * pairs, 0, kPairThreads, kPairSmem, s, &q, who);
+}
+
+template <int BN, int AR, bool DEEP, bool GATED, bool A_MN, bool B_MN>
+int launch_tile(Params& q, int dev, cudaStream_t s, const char* who) {
+  static bool ready[64] = {false};
+  using L = TileShape<BN, AR, DEEP>;
+  const void* kernel = reinterpret_cast<const void*>(&dense_tile_kernel<BN, AR, DEEP, GATED, A_MN, B_MN>);
+  const int slot = dev >= 0 && dev < 64 ? dev : 0;
+  if (!ready[slot]) {
+    int rc = eas_cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem), who,
+                            EAS_ERR_LAUNCH);
+    if (rc) return rc;
+    ready[slot] = true;
+  }
+  return dense_launch(kernel, q.tiles * q.split, q.split > 1 ? q.split : 0, kTileThreads, L::kSmem, s, &q, who);
+}
+
+struct Choice {
+  int bn;     // 0: the pair kernel, else the single-CTA kernel's tile width
+  int split;  // CTAs that share a tile's k-blocks
+  int ar;     // rows of A staged
+  bool deep;  // one CTA per SM
+};
+
+// The shape of least estimated time, in microseconds as measured on one B200 at 1.9 GHz (bf16,
+// operands from HBM; the sweep behind the constants is in the comments).  A step is one 64-deep
+// k-block of one CTA or pair.
+//   pair, 256 x 256        5.5 + rounds x k-blocks x 0.31   (4096^3: 94 us; 512 x 4096 x 4096: 25.3)
+//   one CTA per SM         4.5 + k-blocks x step, step 0.15 (BN 64) or 0.205 (128), 0.115 or 0.155 with
+//                          64 rows of A   (64 x 4096 x 4096: 12.3 BN 64, 15.0 BN 128)
+//   two CTAs per SM        4.0 + CTAs per SM x (k-blocks x step + 0.6 or 0.9), step 0.2 or 0.26
+//                          (2048^3: 25.1 BN 64, 17.5 BN 128)
+//   a split over 2 or 4    2 or 2.8 more for the exchange, and only while all CTAs are resident at
+//                          once (16 x 4096 x 4096, BN 64: 11.9 whole, 10.2 split in 2, 17.9 in 8)
+Choice choose(const DenseProduct& p, int sms) {
+  const int64_t kb = (int64_t)((p.K + kBK - 1) / kBK) * p.terms;
+  const int pairs = sms / 2 > 0 ? sms / 2 : 1;
+  auto tiles_of = [&](int m, int width) {
+    const int n = p.gated ? width / 2 : width;
+    return (int64_t)((p.M + (int64_t)m - 1) / m) * ((p.N + (int64_t)n - 1) / n) * p.batch;
+  };
+  Choice best = {0, 1, 128, false};
+  double best_us = 5.5 + (double)((tiles_of(256, 256) + pairs - 1) / pairs) * kb * 0.31;
+  for (int bn = 64; bn <= 128; bn += 64) {
+    const int64_t tiles = tiles_of(128, bn);
+    for (int split = 1; split <= 4; split *= 2) {
+      const int64_t ctas = tiles * split;
+      if (split > 1 && (ctas > sms * 7 / 8 || kb < 2 * split)) break;
+      Choice c = {bn, split, 128, ctas <= sms};
+      double us;
+      if (c.deep) {
+        if (p.M <= 64 && !p.a_mn) c.ar = 64;
+        const double step = bn == 64 ? (c.ar == 64 ? 0.115 : 0.15) : (c.ar == 64 ? 0.155 : 0.205);
+        us = 4.5 + (double)((kb + split - 1) / split) * step + (split == 1 ? 0 : split == 2 ? 2 : 2.8);
+      } else {
+        double per_sm = (double)ctas / sms;
+        if (per_sm < 1.8) per_sm = 1.8;  // some SM has two
+        us = 4.0 + per_sm * (kb * (bn == 64 ? 0.2 : 0.26) + (bn == 64 ? 0.6 : 0.9));
+      }
+      if (us < best_us) best = c, best_us = us;
+    }
+  }
+  return best;
+}
+
+template <bool GATED, bool A_MN, bool B_MN>
+int launch_choice(const Choice& c, Params& q, int dev, cudaStream_t s, const char* who) {
+  if (c.bn == 0) return launch_pair<GATED, A_MN, B_MN>(q, dev, s, who);
+  if constexpr (!A_MN) {
+    if (c.ar == 64)
+      return c.bn == 64 ? launch_tile<64, 64, true, GATED, A_MN, B_MN>(q, dev, s, who)
+                        : launch_tile<128, 64, true, GATED, A_MN, B_MN>(q, dev, s, who);
+  }
+  if (c.bn == 64)
+    return c.deep ? launch_tile<64, 128, true, GATED, A_MN, B_MN>(q, dev, s, who)
+                  : launch_tile<64, 128, false, GATED, A_MN, B_MN>(q, dev, s, who);
+  return c.deep ? launch_tile<128, 128, true, GATED, A_MN, B_MN>(q, dev, s, who)
+                : launch_tile<128, 128, false, GATED, A_MN, B_MN>(q, dev, s, who);
 }
 
 }  // namespace
@@ -595,12 +895,16 @@ int dense_mma(const DenseProduct& p, cudaStream_t stream, const char* who) {
   int dev = 0;
   int rc = eas_cuda_check(cudaGetDevice(&dev), who, EAS_ERR_UNAVAILABLE);
   if (rc) return rc;
+  const Choice c = choose(p, dense_sms(dev));
   Params q = {};
   q.status = eas_native_status_dev(dev);
-  rc = fill(q, p, 128, 256, p.gated ? 128 : 256, who);
+  q.split = c.split;
+  const int width = c.bn ? c.bn : 256;  // of the accumulator: a gated tile has half as many outputs
+  const int b_rows = !c.bn ? 128 : (p.gated ? c.bn / 2 : c.bn);
+  rc = fill(q, p, c.ar, b_rows, c.bn ? 128 : 256, p.gated ? width / 2 : width, who);
   if (rc) return rc;
-  if (p.gated) return launch_pair<true, false, false>(q, dev, stream, who);
-  if (p.a_mn) return launch_pair<false, true, true>(q, dev, stream, who);
-  if (p.b_mn) return launch_pair<false, false, true>(q, dev, stream, who);
-  return launch_pair<false, false, false>(q, dev, stream, who);
+  if (p.gated) return launch_choice<true, false, false>(c, q, dev, stream, who);
+  if (p.a_mn) return launch_choice<false, true, true>(c, q, dev, stream, who);
+  if (p.b_mn) return launch_choice<false, false, true>(c, q, dev, stream, who);
+  return launch_choice<false, false, false>(c, q, dev, stream, who);
 }

@@ -1,0 +1,336 @@
+// dense_rows.cu — the dense layers' forward products for a few rows (decoding steps).
+//
+//   plain   z[m][n] = sum_k x[m][k] W[n][k];  y = act(z + bias) + residual
+//   gated   g = x Wg^T, u = x Wu^T;  y = act(g) u
+//
+// With so few rows the product reads W once and does almost nothing with it: the bound is HBM, and
+// what counts is to keep bytes under way with few instructions.  Each warp copies 16 rows x 64 values
+// at a time into a queue of its own in shared memory (cp.async), several pieces ahead, and
+// hands them to mma.sync from there.  A warp reads only what it copied itself, so the queue needs
+// no barrier between warps.  x lies in shared memory whole.  Rows of W are the instruction's 16 rows (gated: 8 of the gate, 8 of the up projection),
+// rows of x its 8 columns.  Its k order is a convention between the two operands: lane t of a quad
+// takes k = 8t .. 8t+7 of 32, as it lies in memory, and hands words 0-1 to one m16n8k16 and words
+// 2-3 to the next, on both operands alike.  Rows that do not start on 16 bytes are loaded straight
+// into registers, value by value.
+//
+// Two blocks of 8 warps stay on each SM (or one of 16, where x needs the room), each with an equal
+// share of W's rows (N / 296 of them, give or take one, so that no SM has more to read than another), in tiles of at most 16 (gated: 8 of
+// each weight).  The warps take every 8th (16th) 64-wide piece of K, and the queue runs on over the
+// tiles' ends.  Where a share would be too few rows for a tile, the CTAs of a cluster share the
+// rows of several and split K.  The sums of the warps, then of the cluster's CTAs, are added in a
+// fixed order through (distributed) shared memory, so results are the same bits on every run.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "dense_internal.h"
+#include "dense_launch.h"
+#include "dense_math.cuh"
+#include "eas_internal.h"
+#include "tcgen05_ptx.cuh"
+
+namespace {
+
+using namespace dense;
+
+struct RowsParams {
+  const uint16_t* x;
+  const uint16_t* w[2];
+  const uint16_t* bias;
+  const uint16_t* residual;
+  uint16_t* y;
+  uint16_t* pre;
+  uint16_t* pre2;
+  int64_t ldx, ldw[2], ldr, ldy, ldp, ldp2;
+  int M, N, K, split, act;
+};
+
+template <bool BF16>
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// 8 values of a row, of which `n` are left: zeros past them.
+__device__ __forceinline__ uint4 load8(const uint16_t* p, int n) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t lo = 2 * j < n ? __ldg(p + 2 * j) : 0, hi = 2 * j + 1 < n ? __ldg(p + 2 * j + 1) : 0;
+    w[j] = lo | (hi << 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const uint16_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// Copy 16 bytes past L1, of which the row has `n` values left: zeros past them.
+__device__ __forceinline__ void copy8(uint32_t dst, const uint16_t* src, int n) {
+  const int bytes = n >= 8 ? 16 : n > 0 ? 2 * n : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
+constexpr int kPiece = 64;       // values of K per row and piece
+constexpr int kSlot = 16 * 128;  // a piece of 16 rows of W
+constexpr int kPieces = 4;       // per warp
+constexpr int kDepth = kPieces - 1;  // under way while one is consumed
+
+// W warps per block, and of x in shared memory: two blocks of 8 warps per SM, or one of 16 with twice
+// the room for x.
+template <int W>
+struct Shape {
+  static constexpr int kQueue = W * kPieces * kSlot;  // 64 or 128 KB
+  static constexpr int kMostX = W == 8 ? 40960 : 81920;
+};
+
+// x in shared memory: rows of whole pieces, 64 bytes apart modulo 128, so that the quads of a
+// quarter warp read different banks.
+__host__ __device__ constexpr int64_t x_pitch(int64_t K) { return (K + kPiece - 1) / kPiece * (2 * kPiece) + 64; }
+
+// VEC: rows of x and W start on 16 bytes.
+template <int kWarps, bool GATED, bool VEC, bool BF16>
+__global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
+    dense_rows_kernel(const __grid_constant__ RowsParams p) {
+  constexpr int kTile = GATED ? 8 : 16;  // outputs; always 16 rows of W
+  constexpr int kRows = kDenseRows, kCols = 16;
+  extern __shared__ __align__(128) uint8_t queue[];
+  __shared__ float part[2][kWarps][kRows][kCols + 1];  // tiles take turns
+  __shared__ float sums[kRows][kCols + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int S = p.split;
+  const int rank = (int)blockIdx.x % S;
+  const int64_t group = blockIdx.x / S, groups = gridDim.x / S;
+  const int lo = (int)(group * p.N / groups), hi = (int)((group + 1) * p.N / groups);
+  const int tiles = (hi - lo + kTile - 1) / kTile;
+  auto tile_row = [&](int j) { return lo + (int)((int64_t)j * (hi - lo) / max(tiles, 1)); };  // equal tiles
+  const int stride = kPiece * kWarps * S;
+  const int first = kPiece * (rank * kWarps + warp);
+
+  // Copies go 4 rows of W at a time, 8 lanes and so a whole 128-byte line per row (64 bytes of each
+  // row at a time, the way the lanes read them, every line crossed from L2 twice: 273 MB for 134).
+  // Chunk c of a row lies at place c ^ 4 (row & 1), so that two rows' quads read different banks.
+  // Rows past the tile are not copied: whatever their place in the queue holds reaches only sums
+  // that nobody looks at.
+  const int c8 = lane & 7, r8 = lane >> 3;
+  const uint16_t* w[4];
+  int have = 0;
+  auto aim = [&](int n0, int n1) {
+    have = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int h = GATED ? i >> 1 : 0, n = n0 + r8 + 4 * (GATED ? i & 1 : i);
+      have |= (n < n1 ? 1 : 0) << i;
+      w[i] = p.w[h] + (int64_t)(n < n1 ? n : n0) * p.ldw[h] + 8 * c8;
+    }
+  };
+  const int xrow = min(g, p.M - 1);
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  const uint32_t mine = tc::smem_u32(queue) + warp * (kPieces * kSlot);
+  const uint32_t put = mine + r8 * 128 + ((c8 ^ (4 * (r8 & 1))) << 4);  // + 512 per 4 rows
+  const uint32_t take = mine + g * 128 + ((t ^ (4 * (g & 1))) << 4);    // v = 1: ^ 64; row g + 8: + 1024
+  const int64_t pitch = x_pitch(p.K);
+  const uint32_t xs = tc::smem_u32(queue) + Shape<kWarps>::kQueue;
+  const uint32_t xmine = xs + (uint32_t)(xrow * pitch) + 16 * t;
+  int in_tile = 0, in_k = first, in_slot = 0, out_slot = 0;
+  if (tiles > 0) aim(tile_row(0), tile_row(1));
+  auto issue = [&]() {  // always one group, empty past the end: the waits count groups
+    if (VEC && in_tile < tiles && in_k < p.K) {
+      const uint32_t at = put + in_slot * kSlot;
+      if (in_k + kPiece <= p.K) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (have >> i & 1) copy16(at + i * 512, w[i] + in_k);
+      } else {  // zeros past the end of K
+        const int left = p.K - in_k - 8 * c8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) copy8(at + i * 512, w[i] + (left > 0 ? in_k : 0), left);
+      }
+      in_slot = in_slot == kDepth ? 0 : in_slot + 1;
+      in_k += stride;
+      if (in_k >= p.K) {
+        in_k = first;
+        if (++in_tile < tiles) aim(tile_row(in_tile), tile_row(in_tile + 1));
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if constexpr (VEC) {
+    // x once per block: from every warp's piece it would be read by all SMs at the same time, and
+    // its few lines of L2 were what the kernel waited for (4 rows: 44 us where one took 34)
+    const int words = (int)((pitch - 64) / 16);
+    for (int e = threadIdx.x; e < p.M * words; e += kWarps * 32) {
+      const int r = e / words, c = e % words;
+      const int left = p.K - 8 * c;
+      copy8(xs + (uint32_t)(r * pitch) + 16 * c, p.x + (int64_t)r * p.ldx + (left > 0 ? 8 * c : 0), left);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    for (int i = 0; i < kDepth; ++i) issue();
+    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth) : "memory");
+    __syncthreads();
+  }
+
+  for (int j = 0; j < tiles; ++j) {
+    const int n0 = tile_row(j), width = tile_row(j + 1) - n0;
+    const uint16_t* row[2];  // of this lane's values of W, where they are loaded one by one
+    if (!VEC) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int n = n0 + min(GATED ? g : 8 * i + g, width - 1);
+        row[i] = p.w[GATED ? i : 0] + (int64_t)n * p.ldw[GATED ? i : 0] + 8 * t;
+      }
+    }
+    float acc[4] = {};
+    for (int k = first; k < p.K; k += stride) {
+      uint32_t at = 0;
+      if constexpr (VEC) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+        __syncwarp();  // the piece is here, and everyone has read the one before it
+        issue();
+        at = take + out_slot * kSlot;
+        out_slot = out_slot == kDepth ? 0 : out_slot + 1;
+      }
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        uint4 a[2], b;
+        if constexpr (VEC) {
+          a[0] = lds128((at ^ (v * 64)));
+          a[1] = lds128((at ^ (v * 64)) + 1024);
+          b = lds128(xmine + 2 * k + v * 64);
+        } else {
+          const int left = p.K - k - 32 * v - 8 * t;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) a[i] = load8(row[i] + k + 32 * v, left);
+          b = load8(p.x + (int64_t)xrow * p.ldx + 8 * t + k + 32 * v, left);
+        }
+        const uint32_t a0[4] = {a[0].x, a[1].x, a[0].y, a[1].y};
+        const uint32_t a1[4] = {a[0].z, a[1].z, a[0].w, a[1].w};
+        mma_16816<BF16>(acc, a0, b.x, b.y);
+        mma_16816<BF16>(acc, a1, b.z, b.w);
+      }
+    }
+    auto& mine_part = part[j & 1];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) mine_part[warp][2 * t + (c & 1)][8 * (c >> 1) + g] = acc[c];
+    __syncthreads();
+    const int rows = p.M;
+    if (S > 1) {
+      for (int e = threadIdx.x; e < rows * kCols; e += kWarps * 32) {
+        float s = 0;
+#pragma unroll
+        for (int v = 0; v < kWarps; ++v) s += mine_part[v][e / kCols][e % kCols];
+        sums[e / kCols][e % kCols] = s;
+      }
+      tc::cluster_sync_all();
+    }
+    // this CTA's share of the tile's outputs
+    const int e = threadIdx.x * S + rank;
+    const int r = e / kTile, c = e % kTile, n = n0 + c;
+    if (r < rows && c < width) {
+      float z = 0, u = 0;
+      if (S == 1) {
+#pragma unroll
+        for (int v = 0; v < kWarps; ++v) {
+          z += mine_part[v][r][c];
+          if (GATED) u += mine_part[v][r][c + 8];
+        }
+      } else {
+        const uint32_t at = tc::smem_u32(&sums[r][c]);
+        for (int s = 0; s < S; ++s) {
+          const uint32_t from = tc::mapa_rank(at, (uint32_t)s);
+          z += tc::ld_cluster_f32(from);
+          if (GATED) u += tc::ld_cluster_f32(from + 4 * 8);
+        }
+      }
+      if (!GATED && p.bias) z += to_f32(p.bias[n], BF16);
+      if (p.pre) p.pre[r * p.ldp + n] = to_16(z, BF16);
+      float v = 0;
+      with_act(p.act, [&](auto a) { v = act<decltype(a)::value>(z); });
+      if (GATED) {
+        if (p.pre2) p.pre2[r * p.ldp2 + n] = to_16(u, BF16);
+        v *= u;
+      } else if (p.residual) {
+        v += to_f32(p.residual[r * p.ldr + n], BF16);
+      }
+      p.y[r * p.ldy + n] = to_16(v, BF16);
+    }
+    if (S > 1) tc::cluster_sync_all();  // nobody overwrites its sums, or leaves, while they are being read
+  }
+}
+
+bool aligned16(const void* p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld & 7) == 0; }
+
+// CTAs that split K: two where each block's share of the rows would fill less than half a tile and
+// K is long (1024 x 8192, one row: 7.9 us whole, 6.9 in two, 10.2 in four; 512 x 4096: 5.1, 5.1, 7.6).
+int choose_split(const DenseProduct& p, int blocks, int warps) {
+  const int tile = p.gated ? 8 : 16;
+  return (int64_t)p.N < (int64_t)blocks * tile / 2 && p.K >= 8 * kPiece * warps ? 2 : 1;
+}
+
+template <int W, bool GATED, bool BF16>
+int launch_rows(const DenseProduct& p, RowsParams& q, bool vec, int dev, cudaStream_t s, const char* who) {
+  static bool ready[64] = {false};
+  const void* fast = reinterpret_cast<const void*>(&dense_rows_kernel<W, GATED, true, BF16>);
+  const void* slow = reinterpret_cast<const void*>(&dense_rows_kernel<8, GATED, false, BF16>);
+  if (!ready[dev & 63]) {
+    int rc = eas_cuda_check(cudaFuncSetAttribute(fast, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 Shape<W>::kQueue + Shape<W>::kMostX),
+                            who, EAS_ERR_LAUNCH);
+    if (rc) return rc;
+    ready[dev & 63] = true;
+  }
+  const int warps = vec ? W : 8;
+  const int resident = 16 / warps * dense_sms(dev);
+  q.split = choose_split(p, resident, warps);
+  // no block without rows; four rows a block or more, where there are few
+  int groups = resident / q.split;
+  if (groups > (p.N + 3) / 4) groups = (p.N + 3) / 4;
+  return dense_launch(vec ? fast : slow, groups * q.split, q.split > 1 ? q.split : 0, warps * 32,
+                      vec ? Shape<W>::kQueue + q.M * (int)x_pitch(q.K) : 0, s, &q, who);
+}
+
+template <int W>
+int launch_rows(const DenseProduct& p, RowsParams& q, bool vec, int dev, cudaStream_t s, const char* who) {
+  if (p.bf16)
+    return p.gated ? launch_rows<W, true, true>(p, q, vec, dev, s, who)
+                   : launch_rows<W, false, true>(p, q, vec, dev, s, who);
+  return p.gated ? launch_rows<W, true, false>(p, q, vec, dev, s, who)
+                 : launch_rows<W, false, false>(p, q, vec, dev, s, who);
+}
+
+}  // namespace
+
+bool dense_rows_fit(int M, int K) { return M <= kDenseRows && M * x_pitch(K) <= Shape<16>::kMostX; }
+
+int dense_rows(const DenseProduct& p, cudaStream_t stream, const char* who) {
+  int dev = 0;
+  int rc = eas_cuda_check(cudaGetDevice(&dev), who, EAS_ERR_UNAVAILABLE);
+  if (rc) return rc;
+  RowsParams q = {};
+  q.x = p.a[0], q.w[0] = p.b[0], q.w[1] = p.b[1];
+  q.bias = p.bias, q.residual = p.residual, q.y = p.y[0], q.pre = p.pre, q.pre2 = p.pre2;
+  q.ldx = (int64_t)p.lda[0], q.ldw[0] = (int64_t)p.ldb[0], q.ldw[1] = (int64_t)p.ldb[1];
+  q.ldr = (int64_t)p.ldr, q.ldy = (int64_t)p.ldy[0], q.ldp = (int64_t)p.ldp, q.ldp2 = (int64_t)p.ldp2;
+  q.M = p.M, q.N = p.N, q.K = p.K, q.act = p.act;
+  const bool vec = aligned16(p.a[0], p.M > 1 ? p.lda[0] : 0) && aligned16(p.b[0], p.N > 1 ? p.ldb[0] : 0) &&
+                   (!p.gated || aligned16(p.b[1], p.N > 1 ? p.ldb[1] : 0));
+  return p.M * x_pitch(p.K) <= Shape<8>::kMostX ? launch_rows<8>(p, q, vec, dev, stream, who)
+                                                : launch_rows<16>(p, q, vec, dev, stream, who);
+}

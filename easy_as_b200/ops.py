@@ -26,6 +26,7 @@ summed from the unrounded values.  All results are the same bits on every run.
 from __future__ import annotations
 
 import ctypes
+import struct
 import sys
 from typing import Any
 
@@ -42,6 +43,96 @@ _LINEAR, _GATED, _LINEAR_BACKWARD, _GATED_BACKWARD = range(4)
 _DX, _DW, _DB = 1, 2, 4
 
 
+class _Entry:
+    """A C entry point: its argument struct is pointers (inputs, outputs, scratch), row pitches, scratch
+    bytes, M, N, K, device, dtype, activation."""
+
+    def __init__(self, op: int, name: str, buffers: int, pitches: int):
+        self.op, self.name = op, name
+        self.pointers = struct.Struct(f"={buffers + 1}Q")
+        self.rest = struct.Struct(f"={pitches + 1}Q3I3i")
+
+
+_E_LINEAR = _Entry(_LINEAR, "eas_linear", 6, 5)
+_E_GATED = _Entry(_GATED, "eas_gated", 6, 6)
+_E_LINEAR_BACKWARD = _Entry(_LINEAR_BACKWARD, "eas_linear_backward", 7, 6)
+_E_GATED_BACKWARD = _Entry(_GATED_BACKWARD, "eas_gated_backward", 9, 9)
+
+
+class _Plan:
+    """What calls with the same operator, activation and shapes, strides, dtypes and devices of every
+    buffer have in common once one of them has passed all checks: the argument struct but for its
+    pointers, the scratch it needs (buffers on 16-byte boundaries), and the address ranges to keep apart."""
+
+    __slots__ = ("entry", "rest", "device", "nbytes", "apart")
+
+
+_plans: dict[Any, _Plan] = {}
+_torch_types: tuple[Any, ...] = ()
+_streams: dict[tuple[int, int], Any] = {}
+
+
+def _quick(entry: _Entry, act: str, bufs: tuple[Any, ...], sync: bool) -> Any:
+    """Make the call from a plan of an earlier one (True), or return the key under which
+    :meth:`_Call.launch` may leave a plan (None when there can be none)."""
+    global _torch_types
+    torch = sys.modules.get("torch")
+    if torch is None:
+        return None
+    if not _torch_types:
+        _torch_types = (torch.Tensor, torch.nn.Parameter)
+    types = _torch_types
+    key: list[Any] = [entry, act]
+    for b in bufs:
+        if b is None:
+            key.append(None)
+        elif type(b) in types:
+            key += (b.shape, b.stride(), b.dtype, b.get_device())
+        else:
+            return None
+    k = tuple(key)
+    plan = _plans.get(k)
+    if plan is None or sync.__class__ is not bool:
+        return k
+    ptrs = [0 if b is None else b.data_ptr() for b in bufs]
+    any_ptr = 0
+    for q in ptrs:
+        any_ptr |= q
+    if any_ptr & 15:
+        return None
+    for a, na, b, nb, may_be_one in plan.apart:
+        pa, pb = ptrs[a], ptrs[b]
+        if pa < pb + nb and pb < pa + na and not (may_be_one and pa == pb):
+            return None   # perhaps an overlap: the full checks tell
+    device = plan.device
+    if torch._C._cuda_getDevice() != device:
+        return None
+    rt = get_runtime()
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    capturing = rt.check_capture(stream, sync) if stream else False
+    if plan.nbytes:
+        ptrs.append(torch.empty(plan.nbytes, dtype=torch.uint8, device=bufs[0].device).data_ptr())
+    else:
+        ptrs.append(0)
+    rc = getattr(rt.lib(), entry.name)(entry.pointers.pack(*ptrs) + plan.rest, stream)
+    if rc:
+        cuda_ext.check(rc, entry.name)
+    if not (sync or capturing):
+        _record(torch, device, stream, bufs)
+    rt.finish_native(device, stream, None, sync, capturing)
+    return True
+
+
+def _record(torch: Any, device: int, stream: int, bufs: Any) -> None:
+    """Buffers must outlive an asynchronous launch: torch's allocator learns which stream uses them."""
+    on = _streams.get((device, stream))
+    if on is None:
+        on = _streams[(device, stream)] = torch.cuda.current_stream(device)
+    for b in bufs:
+        if b is not None and type(b) is not Tensor:
+            b.record_stream(on)
+
+
 class _Rows:
     """A buffer as rows: pointer, rows, columns, row pitch in elements, leading shape."""
 
@@ -54,7 +145,7 @@ class _Rows:
 class _Call:
     """The buffers of one call: checked one by one, then launched together."""
 
-    __slots__ = ("what", "dtype", "device", "torch", "ins", "outs")
+    __slots__ = ("what", "dtype", "device", "torch", "ins", "outs", "copied", "in_place")
 
     def __init__(self, what: str):
         self.what = what
@@ -63,6 +154,8 @@ class _Call:
         self.torch: Any = None   # the torch module once a torch tensor was seen
         self.ins: list[_Rows] = []
         self.outs: list[tuple[str, _Rows]] = []
+        self.copied = False      # some input was copied into plain rows first
+        self.in_place: tuple[_Rows, _Rows] | None = None   # an output that may be that input
 
     def _common(self, name: str, dtype: int, device: int) -> None:
         if self.dtype is None:
@@ -89,7 +182,7 @@ class _Call:
             rows = 1
             for d in lead:
                 rows *= d
-            return _Rows(v._cuda_ptr(), rows, cols, cols, lead, v)
+            return _Rows(v._cuda_ptr(), rows, cols, cols if rows > 1 else (cols + 7) // 8 * 8, lead, v)
         torch = sys.modules.get("torch")
         if torch is None or not isinstance(v, torch.Tensor):
             raise TypeError(f"{self.what}: expected a torch CUDA tensor or an eas.Tensor on cuda for {name!r}, "
@@ -123,17 +216,19 @@ class _Call:
                     raise ValueError(f"{self.what}: the leading dimensions of {name!r} are written as one and "
                                      "must be contiguous among themselves") from None
                 flat = v.detach().reshape(-1, shape[-1])
+                self.copied = True
             rows, cols = flat.shape
             ld, unit = flat.stride()
             v = flat
         if rows <= 1:
-            ld = cols
+            ld = (cols + 7) // 8 * 8   # no second row: any pitch, and this one suits the kernels
         if (unit != 1 and cols > 1) or ld < cols:
             if written:
                 raise ValueError(f"{self.what}: {name!r} is written and needs unit stride along its last dimension "
                                  "and rows that do not overlap")
             v = v.detach().contiguous()
             ld = cols
+            self.copied = True
         return _Rows(v.data_ptr(), rows, cols, ld, shape[:-1], v)
 
     def read(self, name: str, v: Any) -> _Rows:
@@ -160,8 +255,9 @@ class _Call:
         if max(rows, n, k) > 0x7fffff00:
             raise ValueError(f"{self.what}: a dimension exceeds 2^31 - 256")
 
-    def no_overlap(self, in_place: tuple[_Rows, _Rows] | None = None) -> None:
-        """No output shares an element with an input or another output (``in_place``: a pair that may be one)."""
+    def no_overlap(self) -> None:
+        """No output shares an element with an input or another output (but for ``in_place``)."""
+        in_place = self.in_place
         for i, (name, o) in enumerate(self.outs):
             lo, hi = o.ptr, o.ptr + 2 * ((o.rows - 1) * o.ld + o.cols)
             for r in self.ins:
@@ -172,8 +268,8 @@ class _Call:
                 if r.ptr < hi and lo < r.ptr + 2 * ((r.rows - 1) * r.ld + r.cols) and _share(o, r):
                     raise ValueError(f"{self.what}: {name!r} overlaps another output")
 
-    def launch(self, entry: Any, head: tuple[Any, ...], tail: tuple[Any, ...], scratch: tuple[int, ...] | None,
-               sync: bool) -> None:
+    def launch(self, entry: _Entry, bufs: tuple[_Rows | None, ...], pitched: tuple[_Rows | None, ...],
+               sizes: tuple[int, int, int], act: int, outputs: int, off: int, sync: bool, key: Any) -> None:
         rt = get_runtime()
         device = self.device
         torch = self.torch
@@ -181,32 +277,49 @@ class _Call:
             stream = int(torch._C._cuda_getCurrentRawStream(device)) if torch is not None else 0
             capturing = rt.check_capture(stream, sync)
             lib = rt.lib()
-            ptr, nbytes, owner = None, 0, None
-            if scratch is not None:
-                need = ctypes.c_uint64()
-                cuda_ext.check(lib.eas_dense_scratch(*scratch, ctypes.byref(need)), self.what)
-                nbytes = need.value
-                if nbytes:
-                    if torch is not None:   # on the launch stream: the current one of this device
-                        owner = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{device}")
-                        ptr = owner.data_ptr()
-                    else:
-                        ptr, owner = rt.scratch(device, stream, self.what, nbytes)
-            cuda_ext.check(getattr(lib, entry)(device, *head, *tail, ptr, nbytes, stream), self.what)
+            need = ctypes.c_uint64()
+            cuda_ext.check(lib.eas_dense_scratch(entry.op, *sizes, act, outputs, off, ctypes.byref(need)), self.what)
+            ptr, nbytes, owner = 0, need.value, None
+            if nbytes:
+                if torch is not None:   # on the launch stream: the current one of this device
+                    owner = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{device}")
+                    ptr = owner.data_ptr()
+                else:
+                    ptr, owner = rt.scratch(device, stream, self.what, nbytes)
+            rest = entry.rest.pack(*(r.ld if r else 0 for r in pitched), nbytes, *sizes, device, self.dtype, act)
+            args = entry.pointers.pack(*(r.ptr if r else 0 for r in bufs), ptr) + rest
+            cuda_ext.check(getattr(lib, entry.name)(args, stream), self.what)
             keep = None
             if not (sync or capturing):
-                # buffers must outlive the launch: torch's allocator learns which stream uses them (its
-                # scratch is that stream's already), the others are kept until it is done
-                bufs = [r.keep for r in self.ins] + [r.keep for _n, r in self.outs]
+                held = [r.keep for r in bufs if r is not None]
                 if torch is not None:
-                    on = torch.cuda.current_stream(device)
-                    for b in bufs:
-                        if type(b) is not Tensor:
-                            b.record_stream(on)
-                keep = [b for b in bufs if type(b) is Tensor]
+                    _record(torch, device, stream, held)
+                keep = [b for b in held if type(b) is Tensor]
                 if torch is None and owner is not None:
                     keep.append(owner)
             rt.finish_native(device, stream, keep, sync, capturing)
+        if key is not None and not self.copied:
+            self._leave_plan(entry, bufs, rest, nbytes, key)
+
+    def _leave_plan(self, entry: _Entry, bufs: tuple[_Rows | None, ...], rest: bytes, nbytes: int, key: Any) -> None:
+        def span(r: _Rows) -> int:
+            return 2 * ((r.rows - 1) * r.ld + r.cols) if r.rows and r.cols else 0
+
+        outs = [o for _n, o in self.outs]
+        apart = []
+        for i, o in enumerate(bufs):
+            if o is None or all(o is not v for v in outs):
+                continue
+            for j, r in enumerate(bufs):
+                if r is None or r is o or (j > i and any(r is v for v in outs)):
+                    continue
+                one = self.in_place is not None and o is self.in_place[0] and r is self.in_place[1]
+                apart.append((i, span(o), j, span(r), one and (o.ld == r.ld or o.rows <= 1)))
+        p = _Plan()
+        p.entry, p.rest, p.device, p.nbytes, p.apart = entry, rest, self.device, nbytes, tuple(apart)
+        if len(_plans) >= 1024:
+            _plans.clear()
+        _plans[key] = p
 
 
 def _share(a: _Rows, b: _Rows) -> bool:
@@ -249,6 +362,9 @@ def linear(x: Any, w: Any, y: Any, *, bias: Any = None, residual: Any = None, ac
     ``pre [..., N]``, if given, receives ``x W^T + bias``, which :func:`linear_backward` needs when
     there is an activation.  ``y`` may be ``residual`` itself.
     """
+    key = _quick(_E_LINEAR, act, (x, w, bias, residual, y, pre), _sync)
+    if key is True:
+        return
     what = "linear"
     code, sync = _activation(what, act), _flag(_sync)
     c = _Call(what)
@@ -270,12 +386,10 @@ def linear(x: Any, w: Any, y: Any, *, bias: Any = None, residual: Any = None, ac
     c.sizes(X.rows, n, k)
     if X.rows == 0:
         return
-    c.no_overlap((Y, R) if R is not None else None)
-    off = _off(X, 1) | _off(W, 2)
-    c.launch("eas_linear",
-             (X.ptr, W.ptr, B.ptr if B else None, R.ptr if R else None, Y.ptr, P.ptr if P else None, X.rows, n, k),
-             (X.ld, W.ld, R.ld if R else 0, Y.ld, P.ld if P else 0, c.dtype, code),
-             (_LINEAR, X.rows, n, k, code, 0, off) if off else None, sync)
+    if R is not None:
+        c.in_place = (Y, R)
+    c.no_overlap()
+    c.launch(_E_LINEAR, (X, W, B, R, Y, P), (X, W, R, Y, P), (X.rows, n, k), code, 0, _off(X, 1) | _off(W, 2), sync, key)
 
 
 def gated(x: Any, w_gate: Any, w_up: Any, h: Any, *, act: str = "silu", gate: Any = None, up: Any = None,
@@ -285,6 +399,9 @@ def gated(x: Any, w_gate: Any, w_up: Any, h: Any, *, act: str = "silu", gate: An
     ``gate`` and ``up [..., N]``, if given (both or neither), receive the two products, which
     :func:`gated_backward` needs.
     """
+    key = _quick(_E_GATED, act, (x, w_gate, w_up, h, gate, up), _sync)
+    if key is True:
+        return
     what = "gated"
     code, sync = _activation(what, act), _flag(_sync)
     c = _Call(what)
@@ -305,11 +422,8 @@ def gated(x: Any, w_gate: Any, w_up: Any, h: Any, *, act: str = "silu", gate: An
     if X.rows == 0:
         return
     c.no_overlap()
-    off = _off(X, 1) | _off(G, 2) | _off(U, 4)
-    c.launch("eas_gated",
-             (X.ptr, G.ptr, U.ptr, H.ptr, SG.ptr if SG else None, SU.ptr if SU else None, X.rows, n, k),
-             (X.ld, G.ld, U.ld, H.ld, SG.ld if SG else 0, SU.ld if SU else 0, c.dtype, code),
-             (_GATED, X.rows, n, k, code, 0, off) if off else None, sync)
+    c.launch(_E_GATED, (X, G, U, H, SG, SU), (X, G, U, H, SG, SU), (X.rows, n, k), code, 0,
+             _off(X, 1) | _off(G, 2) | _off(U, 4), sync, key)
 
 
 def linear_backward(dy: Any, x: Any, w: Any, *, dx: Any = None, dw: Any = None, dbias: Any = None, act: str = "none",
@@ -320,6 +434,9 @@ def linear_backward(dy: Any, x: Any, w: Any, *, dx: Any = None, dw: Any = None, 
     ``pre`` is what :func:`linear` stored there (not needed for ``act="none"``).  The gradient of
     the residual is ``dy`` itself.
     """
+    key = _quick(_E_LINEAR_BACKWARD, act, (dy, pre, x, w, dx, dw, dbias), _sync)
+    if key is True:
+        return
     what = "linear_backward"
     code, sync = _activation(what, act), _flag(_sync)
     c = _Call(what)
@@ -351,12 +468,8 @@ def linear_backward(dy: Any, x: Any, w: Any, *, dx: Any = None, dw: Any = None, 
     if not outputs:
         return
     c.no_overlap()
-    off = _off(X, 1) | _off(W, 2) | _off(DY, 8)
-    c.launch("eas_linear_backward",
-             (DY.ptr, P.ptr if P else None, X.ptr, W.ptr, DX.ptr if DX else None, DW.ptr if DW else None,
-              DB.ptr if DB else None, X.rows, n, k),
-             (DY.ld, P.ld if P else 0, X.ld, W.ld, DX.ld if DX else 0, DW.ld if DW else 0, c.dtype, code),
-             (_LINEAR_BACKWARD, X.rows, n, k, code, outputs, off), sync)
+    c.launch(_E_LINEAR_BACKWARD, (DY, P, X, W, DX, DW, DB), (DY, P, X, W, DX, DW), (X.rows, n, k), code, outputs,
+             _off(X, 1) | _off(W, 2) | _off(DY, 8), sync, key)
 
 
 def gated_backward(dh: Any, x: Any, w_gate: Any, w_up: Any, gate: Any, up: Any, *, dx: Any = None,
@@ -366,6 +479,9 @@ def gated_backward(dh: Any, x: Any, w_gate: Any, w_up: Any, gate: Any, up: Any, 
 
     ``gate`` and ``up`` are what :func:`gated` stored there.
     """
+    key = _quick(_E_GATED_BACKWARD, act, (dh, gate, up, x, w_gate, w_up, dx, dw_gate, dw_up), _sync)
+    if key is True:
+        return
     what = "gated_backward"
     code, sync = _activation(what, act), _flag(_sync)
     c = _Call(what)
@@ -395,10 +511,5 @@ def gated_backward(dh: Any, x: Any, w_gate: Any, w_up: Any, gate: Any, up: Any, 
     if not outputs:
         return
     c.no_overlap()
-    off = _off(X, 1) | _off(G, 2) | _off(U, 4) | _off(DH, 8)
-    c.launch("eas_gated_backward",
-             (DH.ptr, SG.ptr, SU.ptr, X.ptr, G.ptr, U.ptr, DX.ptr if DX else None, DG.ptr if DG else None,
-              DU.ptr if DU else None, X.rows, n, k),
-             (DH.ld, SG.ld, SU.ld, X.ld, G.ld, U.ld, DX.ld if DX else 0, DG.ld if DG else 0, DU.ld if DU else 0,
-              c.dtype, code),
-             (_GATED_BACKWARD, X.rows, n, k, code, outputs, off), sync)
+    c.launch(_E_GATED_BACKWARD, (DH, SG, SU, X, G, U, DX, DG, DU), (DH, SG, SU, X, G, U, DX, DG, DU), (X.rows, n, k), code,
+             outputs, _off(X, 1) | _off(G, 2) | _off(U, 4) | _off(DH, 8), sync, key)

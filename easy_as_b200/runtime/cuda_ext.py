@@ -102,10 +102,10 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "eas_gemm_f16_noalloc": (_int, [_vp, _vp, _vp, _u32, _u32, _u32, _u32, ctypes.c_uint64, ctypes.c_uint64,
                                     ctypes.c_uint64, ctypes.c_uint64, _int, ctypes.c_uint64, ctypes.c_uint64, _int,
                                     _vp, _PINT]),
-    "eas_linear": (_int, [_int, *[_vp] * 6, *[_u32] * 3, *[_u64] * 5, _int, _int, _vp, _u64, _vp]),
-    "eas_gated": (_int, [_int, *[_vp] * 6, *[_u32] * 3, *[_u64] * 6, _int, _int, _vp, _u64, _vp]),
-    "eas_linear_backward": (_int, [_int, *[_vp] * 7, *[_u32] * 3, *[_u64] * 6, _int, _int, _vp, _u64, _vp]),
-    "eas_gated_backward": (_int, [_int, *[_vp] * 9, *[_u32] * 3, *[_u64] * 9, _int, _int, _vp, _u64, _vp]),
+    "eas_linear": (_int, [_vp, _vp]),
+    "eas_gated": (_int, [_vp, _vp]),
+    "eas_linear_backward": (_int, [_vp, _vp]),
+    "eas_gated_backward": (_int, [_vp, _vp]),
     "eas_dense_scratch": (_int, [_int, *[_u32] * 3, _int, _int, _int, ctypes.POINTER(_u64)]),
 }
 

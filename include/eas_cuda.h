@@ -354,33 +354,50 @@ int eas_gemm_f16_noalloc(const void* a, const void* b, float* c, uint32_t M, uin
  * eas_dense_scratch returns (NULL when that is 0); it is free again when the
  * call's work on `stream` is done, and calls that may overlap need one each. */
 
-/* y = act(x W^T + bias) + residual; bias, residual and pre may be NULL.  pre
- * (if given) receives x W^T + bias, which eas_linear_backward needs. */
-int eas_linear(int dev, const void* x, const void* w, const void* bias, const void* residual, void* y, void* pre,
-               uint32_t M, uint32_t N, uint32_t K, uint64_t ldx, uint64_t ldw, uint64_t ldr, uint64_t ldy,
-               uint64_t ldp, int dtype, int act, void* scratch, uint64_t scratch_bytes, void* stream);
+/* y = act(x w^T + bias) + residual; bias, residual and pre may be NULL.  pre
+ * (if given) receives x w^T + bias, which eas_linear_backward needs. */
+typedef struct {
+  const void *x, *w, *bias, *residual;
+  void *y, *pre, *scratch;
+  uint64_t ldx, ldw, ldr, ldy, ldp, scratch_bytes;
+  uint32_t M, N, K;
+  int32_t dev, dtype, act;
+} eas_linear_args;
+int eas_linear(const eas_linear_args* args, void* stream);
 
-/* h = act(x Wg^T) * (x Wu^T); gate and up (both or neither) receive the two
+/* h = act(x w_gate^T) * (x w_up^T); gate and up (both or neither) receive the two
  * products, which eas_gated_backward needs. */
-int eas_gated(int dev, const void* x, const void* w_gate, const void* w_up, void* h, void* gate, void* up,
-              uint32_t M, uint32_t N, uint32_t K, uint64_t ldx, uint64_t ldwg, uint64_t ldwu, uint64_t ldh,
-              uint64_t ldg, uint64_t ldu, int dtype, int act, void* scratch, uint64_t scratch_bytes, void* stream);
+typedef struct {
+  const void *x, *w_gate, *w_up;
+  void *h, *gate, *up, *scratch;
+  uint64_t ldx, ldwg, ldwu, ldh, ldg, ldu, scratch_bytes;
+  uint32_t M, N, K;
+  int32_t dev, dtype, act;
+} eas_gated_args;
+int eas_gated(const eas_gated_args* args, void* stream);
 
-/* dz = dy act'(pre); dx = dz W, dw = dz^T x, db = the sum of dz's rows (each may
+/* dz = dy act'(pre); dx = dz w, dw = dz^T x, db = the sum of dz's rows (each may
  * be NULL; the residual's gradient is dy itself).  pre may be NULL for act 0.
  * dz is rounded to the operands' type; db is summed from the unrounded dz. */
-int eas_linear_backward(int dev, const void* dy, const void* pre, const void* x, const void* w, void* dx, void* dw,
-                        void* db, uint32_t M, uint32_t N, uint32_t K, uint64_t lddy, uint64_t ldp, uint64_t ldx,
-                        uint64_t ldw, uint64_t lddx, uint64_t lddw, int dtype, int act, void* scratch,
-                        uint64_t scratch_bytes, void* stream);
+typedef struct {
+  const void *dy, *pre, *x, *w;
+  void *dx, *dw, *db, *scratch;
+  uint64_t lddy, ldp, ldx, ldw, lddx, lddw, scratch_bytes;
+  uint32_t M, N, K;
+  int32_t dev, dtype, act;
+} eas_linear_backward_args;
+int eas_linear_backward(const eas_linear_backward_args* args, void* stream);
 
-/* dg = dh up act'(gate), du = dh act(gate); dx = dg Wg + du Wu, dw_gate = dg^T x,
- * dw_up = du^T x (each may be NULL). */
-int eas_gated_backward(int dev, const void* dh, const void* gate, const void* up, const void* x, const void* w_gate,
-                       const void* w_up, void* dx, void* dw_gate, void* dw_up, uint32_t M, uint32_t N, uint32_t K,
-                       uint64_t lddh, uint64_t ldg, uint64_t ldu, uint64_t ldx, uint64_t ldwg, uint64_t ldwu,
-                       uint64_t lddx, uint64_t lddwg, uint64_t lddwu, int dtype, int act, void* scratch,
-                       uint64_t scratch_bytes, void* stream);
+/* dg = dh up act'(gate), du = dh act(gate); dx = dg w_gate + du w_up,
+ * dw_gate = dg^T x, dw_up = du^T x (each may be NULL). */
+typedef struct {
+  const void *dh, *gate, *up, *x, *w_gate, *w_up;
+  void *dx, *dw_gate, *dw_up, *scratch;
+  uint64_t lddh, ldg, ldu, ldx, ldwg, ldwu, lddx, lddwg, lddwu, scratch_bytes;
+  uint32_t M, N, K;
+  int32_t dev, dtype, act;
+} eas_gated_backward_args;
+int eas_gated_backward(const eas_gated_backward_args* args, void* stream);
 
 /* Scratch bytes of one call.  op: 0 eas_linear, 1 eas_gated, 2
  * eas_linear_backward, 3 eas_gated_backward.  outputs (2 and 3): 1 dx, 2 a

@@ -131,20 +131,64 @@ def test_backward_refusals():
     eas.ops.linear_backward(dy, x, w)   # nothing asked for: nothing to do
 
 
+_vp, _u64 = ctypes.c_void_p, ctypes.c_uint64
+_TAIL = [("scratch_bytes", _u64), ("M", ctypes.c_uint32), ("N", ctypes.c_uint32), ("K", ctypes.c_uint32),
+         ("dev", ctypes.c_int), ("dtype", ctypes.c_int), ("act", ctypes.c_int)]
+
+
+def _struct(pointers, pitches):
+    class Args(ctypes.Structure):
+        _fields_ = [(n, _vp) for n in pointers.split() + ["scratch"]] + [(n, _u64) for n in pitches.split()] + _TAIL
+
+    return Args
+
+
+#: the argument structs as include/eas_cuda.h declares them
+ARGS = {
+    "eas_linear": _struct("x w bias residual y pre", "ldx ldw ldr ldy ldp"),
+    "eas_gated": _struct("x w_gate w_up h gate up", "ldx ldwg ldwu ldh ldg ldu"),
+    "eas_linear_backward": _struct("dy pre x w dx dw db", "lddy ldp ldx ldw lddx lddw"),
+    "eas_gated_backward": _struct("dh gate up x w_gate w_up dx dw_gate dw_up",
+                                  "lddh ldg ldu ldx ldwg ldwu lddx lddwg lddwu"),
+}
+
+
 def _call(name, **change):
-    args = {"eas_linear": dict(dev=0, x=256, w=512, bias=None, residual=None, y=1024, pre=None, M=4, N=8, K=16, ldx=16,
-                               ldw=16, ldr=0, ldy=8, ldp=0, dtype=0, act=0, scratch=None, nbytes=0, stream=None),
-            "eas_gated": dict(dev=0, x=256, wg=512, wu=768, h=1024, gate=None, up=None, M=4, N=8, K=16, ldx=16, ldwg=16,
-                              ldwu=16, ldh=8, ldg=0, ldu=0, dtype=0, act=0, scratch=None, nbytes=0, stream=None),
-            "eas_linear_backward": dict(dev=0, dy=256, pre=512, x=768, w=1024, dx=2048, dw=4096, db=8192, M=4, N=8, K=16,
-                                        lddy=8, ldp=8, ldx=16, ldw=16, lddx=16, lddw=16, dtype=0, act=1, scratch=None,
-                                        nbytes=0, stream=None),
-            "eas_gated_backward": dict(dev=0, dh=256, gate=512, up=768, x=1024, wg=2048, wu=4096, dx=8192, dwg=16384,
-                                       dwu=32768, M=4, N=8, K=16, lddh=8, ldg=8, ldu=8, ldx=16, ldwg=16, ldwu=16,
-                                       lddx=16, lddwg=16, lddwu=16, dtype=0, act=1, scratch=None, nbytes=0,
-                                       stream=None)}[name]
-    assert set(change) <= set(args)
-    return getattr(cuda_ext.load(), name)(*{**args, **change}.values())
+    a = ARGS[name](M=4, N=8, K=16, act=0 if name in ("eas_linear", "eas_gated") else 1)
+    for i, (field, kind) in enumerate(a._fields_):
+        if field in ("bias", "residual", "scratch") or (name, field) in (("eas_linear", "pre"), ("eas_gated", "gate"),
+                                                                        ("eas_gated", "up")):
+            continue
+        if kind is _vp:
+            setattr(a, field, 4096 * (i + 1))
+        elif field.startswith("ld"):
+            setattr(a, field, 16)
+    for field, v in change.items():
+        assert any(field == f for f, _k in a._fields_)
+        setattr(a, field, v)
+    return getattr(cuda_ext.load(), name)(ctypes.byref(a), None)
+
+
+def test_argument_structs_match_the_header():
+    """Field order of each struct in the header, and the sizes that eas.ops packs."""
+    import re
+    from pathlib import Path
+
+    from easy_as_b200 import ops
+
+    text = (Path(__file__).resolve().parent.parent / "include" / "eas_cuda.h").read_text()
+    for name, cls in ARGS.items():
+        body = next(b for b, n in re.findall(r"typedef struct \{(.*?)\} (\w+);", text, re.S) if n == name + "_args")
+        fields = []
+        for decl in body.split(";"):
+            names = re.sub(r"const void|void|uint64_t|uint32_t|int32_t", "", decl).replace("*", "")
+            fields += [f.strip() for f in names.split(",") if f.strip()]
+        assert fields == [f for f, _k in cls._fields_], name
+        entry = next(e for e in (ops._E_LINEAR, ops._E_GATED, ops._E_LINEAR_BACKWARD, ops._E_GATED_BACKWARD)
+                     if e.name == name)
+        assert entry.pointers.size + entry.rest.size == ctypes.sizeof(cls), name
+    for name in ARGS:
+        assert getattr(cuda_ext.load(), name)(None, None) == cuda_ext.EAS_ERR_VALUE
 
 
 @pytest.mark.parametrize("name", ["eas_linear", "eas_gated", "eas_linear_backward", "eas_gated_backward"])
@@ -166,7 +210,7 @@ def test_c_entries_want_their_scratch(name):
     assert lib.eas_dense_scratch(op, 4, 8, 16, 1, 7 if op == 2 else 3, 0, ctypes.byref(need)) == 0
     assert need.value > 0 and need.value % 256 == 0
     for scratch, nbytes in ((None, need.value), (65536, need.value - 1), (65536 + 16, need.value)):
-        assert _call(name, scratch=scratch, nbytes=nbytes) == cuda_ext.EAS_ERR_VALUE
+        assert _call(name, scratch=scratch, scratch_bytes=nbytes) == cuda_ext.EAS_ERR_VALUE
         assert "scratch" in cuda_ext.last_error()
 
 

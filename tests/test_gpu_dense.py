@@ -16,7 +16,7 @@ TYPES = [torch.float16, torch.bfloat16]
 ACTS = list(eas.ops.ACTIVATIONS)
 
 # (M, N, K): single rows and columns, both sides of every tile edge, rows of one to several hundred
-SHAPES = [(1, 1, 1), (1, 8, 8), (2, 1, 40), (3, 5, 7), (1, 4096, 1024), (8, 72, 520), (9, 64, 64), (16, 200, 136),
+SHAPES = [(1, 1, 1), (1, 8, 8), (2, 1, 40), (3, 5, 7), (1, 4096, 1024), (4, 72, 520), (4, 2500, 72), (3, 40, 4160), (6, 520, 4104), (8, 300, 5000), (7, 96, 8200), (2, 1031, 96), (8, 72, 520), (9, 64, 64), (16, 200, 136),
           (17, 65, 33), (31, 8, 2088), (33, 128, 256), (64, 96, 1000), (65, 1000, 72), (128, 128, 64), (129, 257, 130),
           (200, 640, 192), (257, 255, 65), (384, 512, 128), (520, 1031, 264)]
 BIG = [(1024, 1536, 320), (2304, 2080, 136), (700, 4104, 512)]
@@ -513,6 +513,55 @@ def test_memory_does_not_pile_up(cuda_rt):
         step()
     torch.cuda.synchronize()
     assert torch.cuda.max_memory_allocated() - before <= 4 * dy.numel() * 2
+    cuda_rt.synchronize()
+
+
+def test_repeated_calls_keep_their_checks(cuda_rt):
+    """A call of shapes seen before is still checked for what its addresses and flags can make wrong."""
+    m, n, k, dtype = 40, 64, 64, torch.float16
+    g = gen(0)
+    whole = torch.empty(4 * m * n + 8, device="cuda", dtype=dtype)
+    x, w = normal(g, m, k, dtype), normal(g, n, k, dtype)
+    want = torch.empty(m, n, device="cuda", dtype=dtype)
+    eas.ops.linear(x, w, want)
+    for _ in range(2):
+        y = whole[:m * n].view(m, n)
+        eas.ops.linear(x, w, y)
+        assert torch.equal(y, want)
+        odd = whole[1:1 + m * n].view(m, n)             # the same shape on another alignment
+        eas.ops.linear(x, w, odd)
+        assert torch.equal(odd, want)
+        xo = whole[2 * m * n + 3:2 * m * n + 3 + m * k].view(m, k)
+        xo.copy_(x)
+        eas.ops.linear(xo, w, y)
+        assert torch.equal(y, want)
+        with pytest.raises(ValueError, match="overlaps"):
+            eas.ops.linear(x, w, x)
+        with pytest.raises(ValueError, match="overlaps"):
+            eas.ops.linear(y, w, odd)
+        res = want.clone()
+        eas.ops.linear(x, w, res, residual=res)
+        assert not torch.equal(res, want)
+        with pytest.raises(ValueError, match="overlaps"):
+            eas.ops.linear(x, w, whole[8:8 + m * n].view(m, n), residual=whole[:m * n].view(m, n))
+        with pytest.raises(TypeError, match="_sync"):
+            eas.ops.linear(x, w, y, _sync=None)
+        with pytest.raises(ValueError, match="activation"):
+            eas.ops.linear(x, w, y, act="tanh")
+        with pytest.raises(TypeError, match="dtype"):
+            eas.ops.linear(x, w, y.bfloat16())
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            y2 = torch.empty_like(want)
+            eas.ops.linear(x, w, y2, _sync=False)
+        side.synchronize()
+        assert torch.equal(y2, want)
+    left, right = whole[:2 * m * n].view(m, 2 * n)[:, :n], whole[:2 * m * n].view(m, 2 * n)[:, n:]
+    left.copy_(x)
+    for _ in range(2):
+        eas.ops.linear(left, w, right)                   # side by side in one matrix
+        assert torch.equal(right, want) and torch.equal(left, x)
     cuda_rt.synchronize()
 
 
