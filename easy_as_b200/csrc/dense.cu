@@ -13,6 +13,7 @@
 #include <stdint.h>
 
 #include "dense_internal.h"
+#include "dense_launch.h"
 #include "dense_math.cuh"
 #include "eas_internal.h"
 
@@ -41,35 +42,42 @@ struct ActGrad {
   int M, N, rows_per_block;
   int act;
   bool bf16;
-  bool v_dy, v_g, v_u, v_o;  // 16-byte accesses allowed
+  bool v_dy, v_g, v_u;  // 16-byte accesses allowed (dg and du lie in scratch: always)
 };
 
-__device__ __forceinline__ void load8(const uint16_t* p, int n, bool vec, bool bf16, float (&v)[8]) {
+template <bool BF16>
+__device__ __forceinline__ void widen8(const uint4& w, float (&v)[8]) {
+  unpack2<BF16>(w.x, v[0], v[1]);
+  unpack2<BF16>(w.y, v[2], v[3]);
+  unpack2<BF16>(w.z, v[4], v[5]);
+  unpack2<BF16>(w.w, v[6], v[7]);
+}
+
+template <bool BF16>
+__device__ __forceinline__ void load8(const uint16_t* p, int n, bool vec, float (&v)[8]) {
   if (vec && n >= 8) {
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
-    unpack2(w.x, v[0], v[1], bf16);
-    unpack2(w.y, v[2], v[3], bf16);
-    unpack2(w.z, v[4], v[5], bf16);
-    unpack2(w.w, v[6], v[7], bf16);
+    widen8<BF16>(__ldg(reinterpret_cast<const uint4*>(p)), v);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? to_f32(p[j], bf16) : 0.0f;
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? to_f32<BF16>(p[j]) : 0.0f;
   }
 }
 
-__device__ __forceinline__ void store8(uint16_t* p, int n, bool vec, bool bf16, const float (&v)[8]) {
+template <bool BF16>
+__device__ __forceinline__ void store8(uint16_t* p, int n, bool vec, const float (&v)[8]) {
   if (vec && n >= 8) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack2(v[0], v[1], bf16), pack2(v[2], v[3], bf16),
-                                              pack2(v[4], v[5], bf16), pack2(v[6], v[7], bf16));
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]),
+                                              pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7]));
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j < n) p[j] = to_16(v[j], bf16);
+      if (j < n) p[j] = to_16<BF16>(v[j]);
   }
 }
 
-template <bool GATED>
-__global__ void __launch_bounds__(256) act_grad_kernel(const ActGrad p) {
+// VEC: every array takes 16-byte accesses, so that only the last columns need other ones.
+template <bool GATED, bool BF16, bool VEC>
+__global__ void __launch_bounds__(256) act_grad_kernel(const __grid_constant__ ActGrad p) {
   __shared__ float sums[8][32][9];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int n0 = (blockIdx.x * 32 + tx) * 8;
@@ -77,16 +85,15 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGrad p) {
   const int64_t r0 = (int64_t)blockIdx.y * p.rows_per_block;
   const int64_t r1 = min((int64_t)p.M, r0 + p.rows_per_block);
   float sum[8] = {};
+  grid_order();
   if (cols > 0) {
     with_act(p.act, [&](auto a) {
       constexpr int ACT = decltype(a)::value;
-      for (int64_t m = r0 + ty; m < r1; m += 8) {
-        float dy[8], g[8], u[8], o[8];
-        load8(p.dy + m * p.lddy + n0, cols, p.v_dy, p.bf16, dy);
-        if (GATED || ACT != kNone) load8(p.g + m * p.ldg + n0, cols, p.v_g, p.bf16, g);
-        if (GATED) {
+      constexpr bool kG = GATED || ACT != kNone;
+      auto row = [&](int64_t m, const float (&dy)[8], const float (&g)[8], const float (&u)[8]) {
+        float o[8];
+        if constexpr (GATED) {
           float w[8];
-          load8(p.u + m * p.ldu + n0, cols, p.v_u, p.bf16, u);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             float v, d;
@@ -94,8 +101,8 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGrad p) {
             w[j] = dy[j] * u[j] * d;
             o[j] = dy[j] * v;
           }
-          store8(p.dg + m * p.ldo + n0, cols, p.v_o, p.bf16, w);
-          store8(p.du + m * p.ldo + n0, cols, p.v_o, p.bf16, o);
+          store8<BF16>(p.dg + m * p.ldo + n0, cols, true, w);
+          store8<BF16>(p.du + m * p.ldo + n0, cols, true, o);
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -104,8 +111,37 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGrad p) {
             o[j] = dy[j] * d;
             sum[j] += o[j];
           }
-          if (p.dg) store8(p.dg + m * p.ldo + n0, cols, p.v_o, p.bf16, o);
+          if (p.dg) store8<BF16>(p.dg + m * p.ldo + n0, cols, true, o);
         }
+      };
+      float dy[8], g[8], u[8];
+      int64_t m = r0 + ty;
+      if (VEC && cols >= 8) {
+        // the next row's words are under way while this one is worked on
+        const int64_t sd = 8 * p.lddy, sg = 8 * p.ldg, su = 8 * p.ldu;
+        const uint16_t *pd = p.dy + m * p.lddy + n0, *pg = kG ? p.g + m * p.ldg + n0 : nullptr,
+                       *pu = GATED ? p.u + m * p.ldu + n0 : nullptr;
+        uint4 wd, wg, wu;
+        auto fetch = [&]() {
+          wd = __ldg(reinterpret_cast<const uint4*>(pd));
+          if (kG) wg = __ldg(reinterpret_cast<const uint4*>(pg));
+          if (GATED) wu = __ldg(reinterpret_cast<const uint4*>(pu));
+          pd += sd, pg += sg, pu += su;
+        };
+        if (m < r1) fetch();
+        for (; m < r1; m += 8) {
+          widen8<BF16>(wd, dy);
+          if (kG) widen8<BF16>(wg, g);
+          if (GATED) widen8<BF16>(wu, u);
+          if (m + 8 < r1) fetch();
+          row(m, dy, g, u);
+        }
+      }
+      for (; m < r1; m += 8) {
+        load8<BF16>(p.dy + m * p.lddy + n0, cols, VEC || p.v_dy, dy);
+        if (kG) load8<BF16>(p.g + m * p.ldg + n0, cols, VEC || p.v_g, g);
+        if (GATED) load8<BF16>(p.u + m * p.ldu + n0, cols, VEC || p.v_u, u);
+        row(m, dy, g, u);
       }
     });
   }
@@ -120,18 +156,77 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGrad p) {
   if (n < p.N) p.partial[(int64_t)blockIdx.y * p.N + n] = s;
 }
 
-// db[n] = the sum of the row blocks' partial sums, in order
-__global__ void __launch_bounds__(256) colsum_kernel(const float* __restrict__ partial, uint16_t* __restrict__ db,
-                                                     int blocks, int N, bool bf16) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= N) return;
+template <bool GATED>
+int launch_act_grad(ActGrad& g, int blocks, cudaStream_t s, const char* who) {
+  const bool vec = g.v_dy && (g.v_g || (!GATED && g.act == kNone)) && (!GATED || g.v_u);
+  const void* kernel = g.bf16 ? (vec ? reinterpret_cast<const void*>(&act_grad_kernel<GATED, true, true>)
+                                     : reinterpret_cast<const void*>(&act_grad_kernel<GATED, true, false>))
+                              : (vec ? reinterpret_cast<const void*>(&act_grad_kernel<GATED, false, true>)
+                                     : reinterpret_cast<const void*>(&act_grad_kernel<GATED, false, false>));
+  return dense_launch(kernel, dim3((unsigned)((g.N + 255) / 256), (unsigned)blocks), 0, 256, 0, s, &g, who);
+}
+
+// db[n] = the sum of the row blocks' partial sums: 32 columns per block, 8 threads per column with
+// every 8th row block each, added in order.
+struct ColSum {
+  const float* partial;
+  uint16_t* db;
+  int blocks, N;
+  bool bf16;
+};
+
+__global__ void __launch_bounds__(256) colsum_kernel(const __grid_constant__ ColSum p) {
+  __shared__ float sums[8][32];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, n = blockIdx.x * 32 + tx;
+  grid_order();
   float s = 0;
-  for (int b = 0; b < blocks; ++b) s += partial[(int64_t)b * N + n];
-  db[n] = to_16(s, bf16);
+  if (n < p.N) {
+#pragma unroll 8
+    for (int b = ty; b < p.blocks; b += 8) s += p.partial[(int64_t)b * p.N + n];
+  }
+  sums[ty][tx] = s;
+  __syncthreads();
+  if (ty || n >= p.N) return;
+#pragma unroll
+  for (int r = 1; r < 8; ++r) s += sums[r][tx];
+  p.db[n] = p.bf16 ? to_16<true>(s) : to_16<false>(s);
+}
+
+// Copies of operands whose rows TMA cannot read in place, in rows of a multiple of 8 elements (zeros
+// past the end): up to three matrices in one launch, 8 elements per thread.
+struct Repitch {
+  struct Matrix {
+    const uint16_t* src;
+    uint16_t* dst;
+    int64_t ld;
+    int rows, cols, groups;  // groups of 8 per padded row
+  } m[3];
+  int count;
+};
+
+__global__ void __launch_bounds__(256) repitch_kernel(const __grid_constant__ Repitch p) {
+  grid_order();
+  for (int k = 0; k < p.count; ++k) {
+    const Repitch::Matrix& m = p.m[k];
+    const int64_t total = (int64_t)m.rows * m.groups;
+    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+      const int64_t r = i / m.groups;
+      const int c = (int)(i - r * m.groups) * 8;
+      const uint16_t* src = m.src + r * m.ld + c;
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t lo = c + 2 * j < m.cols ? __ldg(src + 2 * j) : 0;
+        const uint32_t hi = c + 2 * j + 1 < m.cols ? __ldg(src + 2 * j + 1) : 0;
+        w[j] = lo | (hi << 16);
+      }
+      *reinterpret_cast<uint4*>(m.dst + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
 }
 
 // Rows per block: enough blocks for 8 per SM, at least 8 rows (one per thread row), at most 64 row
-// blocks when sums are wanted (colsum_kernel reads them one after another).
+// blocks (colsum_kernel adds them).
 int rows_per_block(int M, int N) {
   const int64_t col_blocks = (N + 255) / 256;
   int64_t want = (8 * 148 + col_blocks - 1) / col_blocks;
@@ -237,14 +332,27 @@ struct Operand {
   uint64_t ld;
 };
 
-int operand(const void* src, uint64_t ld, uint32_t rows, uint32_t cols, bool off, void* scratch, uint64_t at,
-            uint64_t ld_pad, cudaStream_t s, Operand* out) {
-  *out = {u16(src), ld};
-  if (!off) return EAS_OK;
-  uint8_t* dst = static_cast<uint8_t*>(scratch) + at;
-  *out = {u16(dst), ld_pad};
-  return eas_pad_f16_2d(src, dst, rows, (uint32_t)ld_pad, ld, ld_pad, rows, cols, 1, 0, 0, s);
-}
+struct Copies {
+  Repitch r = {};
+
+  Operand add(const void* src, uint64_t ld, uint32_t rows, uint32_t cols, bool off, void* scratch, uint64_t at,
+              uint64_t ld_pad) {
+    if (!off) return {u16(src), ld};
+    uint16_t* dst = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(scratch) + at);
+    r.m[r.count++] = {u16(src), dst, (int64_t)ld, (int)rows, (int)cols, (int)(ld_pad / 8)};
+    return {dst, ld_pad};
+  }
+  int launch(cudaStream_t s, const char* who) {
+    if (!r.count) return EAS_OK;
+    int64_t most = 0;
+    for (int k = 0; k < r.count; ++k) {
+      const int64_t blocks = ((int64_t)r.m[k].rows * r.m[k].groups + 255) / 256;
+      if (blocks > most) most = blocks;
+    }
+    if (most > 8 * 148) most = 8 * 148;
+    return dense_launch(reinterpret_cast<const void*>(&repitch_kernel), dim3((unsigned)most), 0, 256, 0, s, &r, who);
+  }
+};
 
 // dx = sum_t dz_t W_t and dW_t = dz_t^T x
 int backward_products(const char* who, int terms, const Operand (&dz)[2], const Operand (&w)[2], const Operand& x,
@@ -308,9 +416,10 @@ extern "C" int eas_linear(const eas_linear_args* args, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   DeviceScope scope(dev);
   if (scope.rc) return scope.rc;
-  Operand X, W;
-  if ((rc = operand(x, ldx, M, K, off & kXOff, scratch, sc.x, sc.ldk, s, &X))) return rc;
-  if ((rc = operand(w, ldw, N, K, off & kWOff, scratch, sc.w, sc.ldk, s, &W))) return rc;
+  Copies copies;
+  const Operand X = copies.add(x, ldx, M, K, off & kXOff, scratch, sc.x, sc.ldk);
+  const Operand W = copies.add(w, ldw, N, K, off & kWOff, scratch, sc.w, sc.ldk);
+  if ((rc = copies.launch(s, who))) return rc;
   DenseProduct p;
   p.a[0] = X.p, p.lda[0] = X.ld, p.b[0] = W.p, p.ldb[0] = W.ld;
   p.M = (int)M, p.N = (int)N, p.K = (int)K;
@@ -340,10 +449,11 @@ extern "C" int eas_gated(const eas_gated_args* args, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   DeviceScope scope(dev);
   if (scope.rc) return scope.rc;
-  Operand X, G, U;
-  if ((rc = operand(x, ldx, M, K, off & kXOff, scratch, sc.x, sc.ldk, s, &X))) return rc;
-  if ((rc = operand(w_gate, ldwg, N, K, off & kWOff, scratch, sc.w, sc.ldk, s, &G))) return rc;
-  if ((rc = operand(w_up, ldwu, N, K, off & kUpOff, scratch, sc.up, sc.ldk, s, &U))) return rc;
+  Copies copies;
+  const Operand X = copies.add(x, ldx, M, K, off & kXOff, scratch, sc.x, sc.ldk);
+  const Operand G = copies.add(w_gate, ldwg, N, K, off & kWOff, scratch, sc.w, sc.ldk);
+  const Operand U = copies.add(w_up, ldwu, N, K, off & kUpOff, scratch, sc.up, sc.ldk);
+  if ((rc = copies.launch(s, who))) return rc;
   DenseProduct p;
   p.gated = true;
   p.a[0] = X.p, p.lda[0] = X.ld, p.b[0] = G.p, p.ldb[0] = G.ld, p.b[1] = U.p, p.ldb[1] = U.ld;
@@ -389,17 +499,19 @@ extern "C" int eas_linear_backward(const eas_linear_backward_args* args, void* s
     g.dy = u16(dy), g.g = u16(pre), g.dg = dz, g.partial = partial;
     g.lddy = lddy, g.ldg = ldp, g.ldo = sc.ldn;
     g.M = M, g.N = N, g.rows_per_block = sc.rows, g.act = act, g.bf16 = dtype == kBF16;
-    g.v_dy = vec_ok(dy, lddy), g.v_g = pre && vec_ok(pre, ldp), g.v_o = true;
-    act_grad_kernel<false><<<dim3((N + 255) / 256, sc.blocks), 256, 0, s>>>(g);
-    if ((rc = eas_cuda_check(cudaGetLastError(), who, EAS_ERR_LAUNCH))) return rc;
+    g.v_dy = vec_ok(dy, lddy), g.v_g = pre && vec_ok(pre, ldp);
+    rc = launch_act_grad<false>(g, sc.blocks, s, who);
+    if (rc) return rc;
     if (db) {
-      colsum_kernel<<<(N + 255) / 256, 256, 0, s>>>(partial, u16(db), sc.blocks, N, dtype == kBF16);
-      if ((rc = eas_cuda_check(cudaGetLastError(), who, EAS_ERR_LAUNCH))) return rc;
+      ColSum c = {partial, u16(db), sc.blocks, (int)N, dtype == kBF16};
+      rc = dense_launch(reinterpret_cast<const void*>(&colsum_kernel), dim3((N + 31) / 32), 0, 256, 0, s, &c, who);
+      if (rc) return rc;
     }
   }
-  Operand X = {}, W = {};
-  if (dw && (rc = operand(x, ldx, M, K, off & kXOff, scratch, sc.x, sc.ldk, s, &X))) return rc;
-  if (dx && (rc = operand(w, ldw, N, K, off & kWOff, scratch, sc.w, sc.ldk, s, &W))) return rc;
+  Copies copies;
+  const Operand X = dw ? copies.add(x, ldx, M, K, off & kXOff, scratch, sc.x, sc.ldk) : Operand{};
+  const Operand W = dx ? copies.add(w, ldw, N, K, off & kWOff, scratch, sc.w, sc.ldk) : Operand{};
+  if ((rc = copies.launch(s, who))) return rc;
   const Operand DZ = dz ? Operand{dz, sc.ldn} : Operand{u16(dy), lddy};
   return backward_products(who, 1, {DZ, {}}, {W, {}}, X, dx, lddx, {dw, nullptr}, {lddw, 0}, M, N, K, dtype, s);
 }
@@ -439,15 +551,15 @@ extern "C" int eas_gated_backward(const eas_gated_backward_args* args, void* str
   g.dy = u16(dh), g.g = u16(gate), g.u = u16(up), g.dg = dg, g.du = du;
   g.lddy = lddh, g.ldg = ldg, g.ldu = ldu, g.ldo = sc.ldn;
   g.M = M, g.N = N, g.rows_per_block = sc.rows, g.act = act, g.bf16 = dtype == kBF16;
-  g.v_dy = vec_ok(dh, lddh), g.v_g = vec_ok(gate, ldg), g.v_u = vec_ok(up, ldu), g.v_o = true;
-  act_grad_kernel<true><<<dim3((N + 255) / 256, sc.blocks), 256, 0, s>>>(g);
-  if ((rc = eas_cuda_check(cudaGetLastError(), who, EAS_ERR_LAUNCH))) return rc;
-  Operand X = {}, G = {}, U = {};
-  if ((outputs & kDw) && (rc = operand(x, ldx, M, K, off & kXOff, scratch, sc.x, sc.ldk, s, &X))) return rc;
-  if (dx) {
-    if ((rc = operand(w_gate, ldwg, N, K, off & kWOff, scratch, sc.w, sc.ldk, s, &G))) return rc;
-    if ((rc = operand(w_up, ldwu, N, K, off & kUpOff, scratch, sc.up, sc.ldk, s, &U))) return rc;
-  }
+  g.v_dy = vec_ok(dh, lddh), g.v_g = vec_ok(gate, ldg), g.v_u = vec_ok(up, ldu);
+  rc = launch_act_grad<true>(g, sc.blocks, s, who);
+  if (rc) return rc;
+  const bool dw = outputs & kDw;
+  Copies copies;
+  const Operand X = dw ? copies.add(x, ldx, M, K, off & kXOff, scratch, sc.x, sc.ldk) : Operand{};
+  const Operand G = dx ? copies.add(w_gate, ldwg, N, K, off & kWOff, scratch, sc.w, sc.ldk) : Operand{};
+  const Operand U = dx ? copies.add(w_up, ldwu, N, K, off & kUpOff, scratch, sc.up, sc.ldk) : Operand{};
+  if ((rc = copies.launch(s, who))) return rc;
   return backward_products(who, 2, {{dg, sc.ldn}, {du, sc.ldn}}, {G, U}, X, dx, lddx, {dw_gate, dw_up},
                            {lddwg, lddwu}, M, N, K, dtype, s);
 }

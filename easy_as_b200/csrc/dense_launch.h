@@ -16,13 +16,20 @@ inline bool dense_pdl_on() {
   return on;
 }
 
+// The grid before this one in the stream may still be running: nothing of global memory is touched
+// before it has finished.  The next grid may be set up meanwhile, and waits in the same place.
+__device__ __forceinline__ void grid_order() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // One launch with one parameter struct.  cluster: CTAs per cluster where the kernel does not say
-// itself, else 0.  The kernel begins with griddepcontrol.wait, so it may be scheduled while the
+// itself, else 0.  The kernel begins with grid_order(), so it may be scheduled while the
 // grid before it in the stream is finishing.
-inline int dense_launch(const void* kernel, int blocks, int cluster, int threads, int smem, cudaStream_t s,
+inline int dense_launch(const void* kernel, dim3 blocks, int cluster, int threads, int smem, cudaStream_t s,
                         void* params, const char* who) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+  cfg.gridDim = blocks;
   cfg.blockDim = dim3((unsigned)threads, 1, 1);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = s;

@@ -35,15 +35,32 @@ __device__ __forceinline__ void logistic(float z, float& p, float& q) {
 constexpr float kGeluC2 = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float kGeluA = 0.044715f;
 
-// Phi(z), without the cancellation of 1 + erf(z / sqrt 2) for negative z
-__device__ __forceinline__ float normal_cdf(float z) { return 0.5f * erfcf(-0.70710678118654752f * z); }
+// Phi(z) and e = exp(-z^2 / 2), which its density shares.  The tail 1 - Phi(|z|) is e times a smooth
+// function that falls like 1 / |z|: a polynomial without constant term in t = 1 / (1 + 0.3606 |z|), the
+// form of Hastings' approximations of the error function, here of degree 7 with coefficients fitted
+// to the least relative error (1.2e-6 for |z| < 13 in f32).  So the tail of a negative z is as exact
+// as its exponential, where 1 + erf(z / sqrt 2) would cancel; 14 instructions, against about 50 of
+// erfcf (the backward pass of 4096 x 8192 pre-activations took 89 us with it, where its bytes take 31).
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+  e = __expf(-0.5f * z * z);
+  const float t = __fdividef(1.0f, fmaf(0.36062446f, fabsf(z), 1.0f));
+  float p = fmaf(t, 4.724989589e-02f, -1.795671291e-01f);
+  p = fmaf(t, p, 1.792224294e-01f);
+  p = fmaf(t, p, 2.752668697e-02f);
+  p = fmaf(t, p, 1.395329766e-01f);
+  p = fmaf(t, p, 1.420761715e-01f);
+  p = fmaf(t, p, 1.439587504e-01f);
+  const float tail = e * (t * p);
+  return z < 0 ? tail : 1.0f - tail;
+}
 
 template <int ACT>
 __device__ __forceinline__ float act(float z) {
   if constexpr (ACT == kRelu) {
     return z < 0 ? 0.0f : z;  // NaN stays NaN
   } else if constexpr (ACT == kGelu) {
-    return z * normal_cdf(z);
+    float e;
+    return z * normal_cdf(z, e);
   } else if constexpr (ACT == kGeluTanh) {
     float p, q;
     logistic(kGeluC2 * z * (1.0f + kGeluA * z * z), p, q);
@@ -69,9 +86,10 @@ __device__ __forceinline__ void act_and_slope(float z, float& v, float& d) {
     v = z < 0 ? 0.0f : z;
     d = z > 0 ? 1.0f : (z <= 0 ? 0.0f : z);
   } else if constexpr (ACT == kGelu) {
-    const float cdf = normal_cdf(z);
+    float e;
+    const float cdf = normal_cdf(z, e);
     v = z * cdf;
-    d = cdf + z * (0.39894228040143268f * __expf(-0.5f * z * z));
+    d = cdf + z * (0.39894228040143268f * e);
   } else if constexpr (ACT == kGeluTanh) {
     const float z2 = fminf(z * z, 1e4f);  // past it s(z) s(-z) is 0 and the bracket must not be infinite
     logistic(kGeluC2 * z * (1.0f + kGeluA * z2), p, q);
@@ -88,26 +106,32 @@ __device__ __forceinline__ void act_and_slope(float z, float& v, float& d) {
   }
 }
 
-__device__ __forceinline__ float to_f32(uint16_t h, bool bf16) {
-  return bf16 ? __uint_as_float((uint32_t)h << 16) : __half2float(__ushort_as_half(h));
+template <bool BF16>
+__device__ __forceinline__ float to_f32(uint16_t h) {
+  if constexpr (BF16) return __uint_as_float((uint32_t)h << 16);
+  return __half2float(__ushort_as_half(h));
 }
 
-__device__ __forceinline__ uint16_t to_16(float v, bool bf16) {
-  return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+template <bool BF16>
+__device__ __forceinline__ uint16_t to_16(float v) {
+  if constexpr (BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+  return __half_as_ushort(__float2half_rn(v));
 }
 
 // two values in one word, the first in the low half
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
-  if (bf16)
+  if constexpr (BF16)
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   else
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
 
-__device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi, bool bf16) {
-  if (bf16) {
+template <bool BF16>
+__device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi) {
+  if constexpr (BF16) {
     lo = __uint_as_float(w << 16);
     hi = __uint_as_float(w & 0xffff0000u);
   } else {

@@ -110,13 +110,6 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
-// The grid before this one in the stream may still be running: nothing of global memory is touched
-// before it has finished.  The next grid may be set up meanwhile, and waits in the same place.
-__device__ __forceinline__ void grid_order() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
 // Instruction descriptor, kind::f16: D = f32 (bits 4-5 = 1), A and B formats at bits 7-9 and 10-12
 // (f16 0, bf16 1), A and B major at bits 15 and 16 (1 = MN), N >> 3 at bits 17-22, M >> 4 at 24-28.
 __device__ __forceinline__ uint32_t instr_desc(int m, int n, bool a_mn, bool b_mn, bool bf16) {
@@ -216,14 +209,15 @@ __device__ __forceinline__ uint8_t* next_box(Boxes& bx, int lane) {
   return box;
 }
 
+template <bool BF16>
 __device__ __forceinline__ void put(Boxes& bx, int lane, const CUtensorMap* map, bool tma, uint16_t* ptr, int64_t ld,
-                                    int M, int N, int m0, int n0, const float (&v)[32], bool bf16) {
+                                    int M, int N, int m0, int n0, const float (&v)[32]) {
   uint8_t* box = next_box(bx, lane);
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     *reinterpret_cast<uint4*>(box_chunk(box, lane, j)) =
-        make_uint4(pack2(v[8 * j], v[8 * j + 1], bf16), pack2(v[8 * j + 2], v[8 * j + 3], bf16),
-                   pack2(v[8 * j + 4], v[8 * j + 5], bf16), pack2(v[8 * j + 6], v[8 * j + 7], bf16));
+        make_uint4(pack2<BF16>(v[8 * j], v[8 * j + 1]), pack2<BF16>(v[8 * j + 2], v[8 * j + 3]),
+                   pack2<BF16>(v[8 * j + 4], v[8 * j + 5]), pack2<BF16>(v[8 * j + 6], v[8 * j + 7]));
   if (tma) {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
@@ -231,15 +225,17 @@ __device__ __forceinline__ void put(Boxes& bx, int lane, const CUtensorMap* map,
   } else {
     __syncwarp();
     const int rows = min(32, M - m0);
-    if (n0 + lane < N)
-      for (int r = 0; r < rows; ++r)
-        ptr[(int64_t)(m0 + r) * ld + n0 + lane] =
-            *reinterpret_cast<const uint16_t*>(box_chunk(box, r, lane >> 3) + (lane & 7) * 2);
+    uint16_t* dst = ptr + (int64_t)m0 * ld + n0 + lane;
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+      if (r < rows && n0 + lane < N)
+        dst[r * ld] = *reinterpret_cast<const uint16_t*>(box_chunk(box, r, lane >> 3) + (lane & 7) * 2);
   }
   if (lane == 0) bulk_commit();  // an empty group where nothing was stored: the boxes' turns count groups
 }
 
 // v += the residual's 32 x 32 piece
+template <bool BF16>
 __device__ __forceinline__ void add_residual(const Params& p, Boxes& bx, int lane, int m0, int n0, float (&v)[32]) {
   uint4 w[4];
   if (p.res_vec && n0 + 32 <= p.N) {
@@ -250,9 +246,16 @@ __device__ __forceinline__ void add_residual(const Params& p, Boxes& bx, int lan
   } else {
     uint8_t* box = next_box(bx, lane);
     const int rows = min(32, p.M - m0);
-    for (int r = 0; r < rows; ++r)
-      *reinterpret_cast<uint16_t*>(box_chunk(box, r, lane >> 3) + (lane & 7) * 2) =
-          n0 + lane < p.N ? p.residual[(int64_t)(m0 + r) * p.ldr + n0 + lane] : (uint16_t)0;
+    const uint16_t* src = p.residual + (int64_t)m0 * p.ldr + n0 + lane;
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += 16) {  // 16 loads under way
+      uint16_t h[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) h[r] = r0 + r < rows && n0 + lane < p.N ? src[(r0 + r) * p.ldr] : (uint16_t)0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        *reinterpret_cast<uint16_t*>(box_chunk(box, r0 + r, lane >> 3) + (lane & 7) * 2) = h[r];
+    }
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4*>(box_chunk(box, lane, j));
@@ -264,13 +267,14 @@ __device__ __forceinline__ void add_residual(const Params& p, Boxes& bx, int lan
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float lo, hi;
-      unpack2(q[i], lo, hi, p.bf16);
+      unpack2<BF16>(q[i], lo, hi);
       v[8 * j + 2 * i] += lo;
       v[8 * j + 2 * i + 1] += hi;
     }
   }
 }
 
+template <bool BF16>
 __device__ __forceinline__ void add_bias(const Params& p, int n0, float (&v)[32]) {
   if (p.bias_vec && n0 + 32 <= p.N) {
     const uint4* src = reinterpret_cast<const uint4*>(p.bias + n0);
@@ -281,7 +285,7 @@ __device__ __forceinline__ void add_bias(const Params& p, int n0, float (&v)[32]
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float lo, hi;
-        unpack2(q[i], lo, hi, p.bf16);
+        unpack2<BF16>(q[i], lo, hi);
         v[8 * j + 2 * i] += lo;
         v[8 * j + 2 * i + 1] += hi;
       }
@@ -289,18 +293,18 @@ __device__ __forceinline__ void add_bias(const Params& p, int n0, float (&v)[32]
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      if (n0 + j < p.N) v[j] += to_f32(p.bias[n0 + j], p.bf16);
+      if (n0 + j < p.N) v[j] += to_f32<BF16>(p.bias[n0 + j]);
   }
 }
 
 // Finish 32 x 32 results from their sums: v = z, or v = g and u.
-template <bool GATED>
-__device__ __forceinline__ void finish(const Params& p, Boxes& bx, int lane, int z, int m0, int n0, float (&v)[32],
-                                       const float (&u)[GATED ? 32 : 1]) {
-  if (!GATED && p.bias) add_bias(p, n0, v);
-  if (p.pre_ptr) put(bx, lane, &p.pre, p.pre_tma, p.pre_ptr, p.ldp, p.M, p.N, m0, n0, v, p.bf16);
+template <bool GATED, bool BF16>
+__device__ __forceinline__ void finish_as(const Params& p, Boxes& bx, int lane, int z, int m0, int n0, float (&v)[32],
+                                          const float (&u)[GATED ? 32 : 1]) {
+  if (!GATED && p.bias) add_bias<BF16>(p, n0, v);
+  if (p.pre_ptr) put<BF16>(bx, lane, &p.pre, p.pre_tma, p.pre_ptr, p.ldp, p.M, p.N, m0, n0, v);
   if constexpr (GATED) {
-    if (p.pre2_ptr) put(bx, lane, &p.pre2, p.pre2_tma, p.pre2_ptr, p.ldp2, p.M, p.N, m0, n0, u, p.bf16);
+    if (p.pre2_ptr) put<BF16>(bx, lane, &p.pre2, p.pre2_tma, p.pre2_ptr, p.ldp2, p.M, p.N, m0, n0, u);
   }
   with_act(p.act, [&](auto a) {
 #pragma unroll
@@ -309,8 +313,17 @@ __device__ __forceinline__ void finish(const Params& p, Boxes& bx, int lane, int
       if constexpr (GATED) v[j] *= u[j];
     }
   });
-  if (!GATED && p.residual) add_residual(p, bx, lane, m0, n0, v);
-  put(bx, lane, &p.y[z], p.y_tma, p.y_ptr[z], p.ldy[z], p.M, p.N, m0, n0, v, p.bf16);
+  if (!GATED && p.residual) add_residual<BF16>(p, bx, lane, m0, n0, v);
+  put<BF16>(bx, lane, &p.y[z], p.y_tma, p.y_ptr[z], p.ldy[z], p.M, p.N, m0, n0, v);
+}
+
+template <bool GATED>
+__device__ __forceinline__ void finish(const Params& p, Boxes& bx, int lane, int z, int m0, int n0, float (&v)[32],
+                                       const float (&u)[GATED ? 32 : 1]) {
+  if (p.bf16)
+    finish_as<GATED, true>(p, bx, lane, z, m0, n0, v, u);
+  else
+    finish_as<GATED, false>(p, bx, lane, z, m0, n0, v, u);
 }
 
 __device__ __forceinline__ void as_floats(const uint32_t (&r)[32], float (&v)[32]) {
@@ -808,7 +821,7 @@ int launch_pair(Params& q, int dev, cudaStream_t s, const char* who) {
     st.pairs[slot] = n;
   }
   const int pairs = q.tiles < st.pairs[slot] ? q.tiles : st.pairs[slot];
-  return dense_launch(kernel, 2 * pairs, 0, kPairThreads, kPairSmem, s, &q, who);
+  return dense_launch(kernel, dim3(2 * pairs), 0, kPairThreads, kPairSmem, s, &q, who);
 }
 
 template <int BN, int AR, bool DEEP, bool GATED, bool A_MN, bool B_MN>
@@ -823,7 +836,7 @@ int launch_tile(Params& q, int dev, cudaStream_t s, const char* who) {
     if (rc) return rc;
     ready[slot] = true;
   }
-  return dense_launch(kernel, q.tiles * q.split, q.split > 1 ? q.split : 0, kTileThreads, L::kSmem, s, &q, who);
+  return dense_launch(kernel, dim3(q.tiles * q.split), q.split > 1 ? q.split : 0, kTileThreads, L::kSmem, s, &q, who);
 }
 
 struct Choice {

@@ -140,8 +140,7 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
   };
   const int xrow = min(g, p.M - 1);
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  grid_order();
 
   const uint32_t mine = tc::smem_u32(queue) + warp * (kPieces * kSlot);
   const uint32_t put = mine + r8 * 128 + ((c8 ^ (4 * (r8 & 1))) << 4);  // + 512 per 4 rows
@@ -259,17 +258,17 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
           if (GATED) u += tc::ld_cluster_f32(from + 4 * 8);
         }
       }
-      if (!GATED && p.bias) z += to_f32(p.bias[n], BF16);
-      if (p.pre) p.pre[r * p.ldp + n] = to_16(z, BF16);
+      if (!GATED && p.bias) z += to_f32<BF16>(p.bias[n]);
+      if (p.pre) p.pre[r * p.ldp + n] = to_16<BF16>(z);
       float v = 0;
       with_act(p.act, [&](auto a) { v = act<decltype(a)::value>(z); });
       if (GATED) {
-        if (p.pre2) p.pre2[r * p.ldp2 + n] = to_16(u, BF16);
+        if (p.pre2) p.pre2[r * p.ldp2 + n] = to_16<BF16>(u);
         v *= u;
       } else if (p.residual) {
-        v += to_f32(p.residual[r * p.ldr + n], BF16);
+        v += to_f32<BF16>(p.residual[r * p.ldr + n]);
       }
-      p.y[r * p.ldy + n] = to_16(v, BF16);
+      p.y[r * p.ldy + n] = to_16<BF16>(v);
     }
     if (S > 1) tc::cluster_sync_all();  // nobody overwrites its sums, or leaves, while they are being read
   }
@@ -302,7 +301,7 @@ int launch_rows(const DenseProduct& p, RowsParams& q, bool vec, int dev, cudaStr
   // no block without rows; four rows a block or more, where there are few
   int groups = resident / q.split;
   if (groups > (p.N + 3) / 4) groups = (p.N + 3) / 4;
-  return dense_launch(vec ? fast : slow, groups * q.split, q.split > 1 ? q.split : 0, warps * 32,
+  return dense_launch(vec ? fast : slow, dim3(groups * q.split), q.split > 1 ? q.split : 0, warps * 32,
                       vec ? Shape<W>::kQueue + q.M * (int)x_pitch(q.K) : 0, s, &q, who);
 }
 
