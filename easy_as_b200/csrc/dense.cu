@@ -28,7 +28,7 @@ using namespace dense;
 // linear: dz = dy act'(z);  gated: dg = dh u act'(g), du = dh act(g).  One pass, 8 columns (16
 // bytes) per thread; a block covers 256 columns of kRowsPerBlock rows with 8 thread rows.  With
 // db, each thread keeps the f32 sums of its columns, the block adds its 8 thread rows in shared
-// memory and writes one row of partial sums, and colsum_kernel adds those in a fixed order: no
+// memory and writes one row of partial sums, which the products' launch adds in a fixed order: no
 // atomics, the same bits on every run.
 
 struct ActGrad {
@@ -166,32 +166,6 @@ int launch_act_grad(ActGrad& g, int blocks, cudaStream_t s, const char* who) {
   return dense_launch(kernel, dim3((unsigned)((g.N + 255) / 256), (unsigned)blocks), 0, 256, 0, s, &g, who);
 }
 
-// db[n] = the sum of the row blocks' partial sums: 32 columns per block, 8 threads per column with
-// every 8th row block each, added in order.
-struct ColSum {
-  const float* partial;
-  uint16_t* db;
-  int blocks, N;
-  bool bf16;
-};
-
-__global__ void __launch_bounds__(256) colsum_kernel(const __grid_constant__ ColSum p) {
-  __shared__ float sums[8][32];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, n = blockIdx.x * 32 + tx;
-  grid_order();
-  float s = 0;
-  if (n < p.N) {
-#pragma unroll 8
-    for (int b = ty; b < p.blocks; b += 8) s += p.partial[(int64_t)b * p.N + n];
-  }
-  sums[ty][tx] = s;
-  __syncthreads();
-  if (ty || n >= p.N) return;
-#pragma unroll
-  for (int r = 1; r < 8; ++r) s += sums[r][tx];
-  p.db[n] = p.bf16 ? to_16<true>(s) : to_16<false>(s);
-}
-
 // Copies of operands whose rows TMA cannot read in place, in rows of a multiple of 8 elements (zeros
 // past the end): up to three matrices in one launch, 8 elements per thread.
 struct Repitch {
@@ -226,7 +200,7 @@ __global__ void __launch_bounds__(256) repitch_kernel(const __grid_constant__ Re
 }
 
 // Rows per block: enough blocks for 8 per SM, at least 8 rows (one per thread row), at most 64 row
-// blocks (colsum_kernel adds them).
+// blocks (whose partial sums are added one after another).
 int rows_per_block(int M, int N) {
   const int64_t col_blocks = (N + 255) / 256;
   int64_t want = (8 * 148 + col_blocks - 1) / col_blocks;
@@ -354,31 +328,32 @@ struct Copies {
   }
 };
 
-// dx = sum_t dz_t W_t and dW_t = dz_t^T x
+// dx = sum_t dz_t W_t and dW_t = dz_t^T x, and db: independent of one another, so one launch.
 int backward_products(const char* who, int terms, const Operand (&dz)[2], const Operand (&w)[2], const Operand& x,
-                      void* dx, uint64_t lddx, void* const (&dw)[2], const uint64_t (&lddw)[2], uint32_t M, uint32_t N,
-                      uint32_t K, int dtype, cudaStream_t s) {
+                      void* dx, uint64_t lddx, void* const (&dw)[2], const uint64_t (&lddw)[2], const DenseColSum& sums,
+                      uint32_t M, uint32_t N, uint32_t K, int dtype, cudaStream_t s) {
+  DenseProduct p[2];
+  int count = 0;
   if (dx) {
-    DenseProduct p;
-    for (int t = 0; t < terms; ++t) p.a[t] = dz[t].p, p.lda[t] = dz[t].ld, p.b[t] = w[t].p, p.ldb[t] = w[t].ld;
-    p.b_mn = true;
-    p.M = (int)M, p.N = (int)K, p.K = (int)N, p.terms = terms;
-    p.y[0] = u16(dx), p.ldy[0] = lddx, p.bf16 = dtype == kBF16;
-    int rc = dense_mma(p, s, who);
-    if (rc) return rc;
+    DenseProduct& d = p[count++];
+    for (int t = 0; t < terms; ++t) d.a[t] = dz[t].p, d.lda[t] = dz[t].ld, d.b[t] = w[t].p, d.ldb[t] = w[t].ld;
+    d.M = (int)M, d.N = (int)K, d.K = (int)N, d.terms = terms;
+    d.y[0] = u16(dx), d.ldy[0] = lddx;
   }
-  DenseProduct p;
-  p.batch = 0;
-  for (int t = 0; t < terms; ++t) {
-    if (!dw[t]) continue;
-    const int z = p.batch++;
-    p.a[z] = dz[t].p, p.lda[z] = dz[t].ld, p.y[z] = u16(dw[t]), p.ldy[z] = lddw[t];
+  if (dw[0] || dw[1]) {
+    DenseProduct& d = p[count++];
+    d.batch = 0;
+    for (int t = 0; t < terms; ++t) {
+      if (!dw[t]) continue;
+      const int z = d.batch++;
+      d.a[z] = dz[t].p, d.lda[z] = dz[t].ld, d.y[z] = u16(dw[t]), d.ldy[z] = lddw[t];
+    }
+    d.b[0] = x.p, d.ldb[0] = x.ld;
+    d.a_mn = true;
+    d.M = (int)N, d.N = (int)K, d.K = (int)M;
   }
-  if (!p.batch) return EAS_OK;
-  p.b[0] = x.p, p.ldb[0] = x.ld;
-  p.a_mn = p.b_mn = true;
-  p.M = (int)N, p.N = (int)K, p.K = (int)M, p.bf16 = dtype == kBF16;
-  return dense_mma(p, s, who);
+  for (int i = 0; i < count; ++i) p[i].b_mn = true, p[i].bf16 = dtype == kBF16;
+  return dense_mma(p, count, sums, s, who);
 }
 
 }  // namespace
@@ -426,7 +401,7 @@ extern "C" int eas_linear(const eas_linear_args* args, void* stream) {
   p.bias = u16(bias), p.residual = u16(residual), p.y[0] = u16(y), p.pre = u16(pre);
   p.ldr = ldr, p.ldy[0] = ldy, p.ldp = ldp;
   p.act = act, p.bf16 = dtype == kBF16;
-  return few ? dense_rows(p, s, who) : dense_mma(p, s, who);
+  return few ? dense_rows(p, s, who) : dense_mma(&p, 1, DenseColSum(), s, who);
 }
 
 extern "C" int eas_gated(const eas_gated_args* args, void* stream) {
@@ -461,7 +436,7 @@ extern "C" int eas_gated(const eas_gated_args* args, void* stream) {
   p.y[0] = u16(h), p.pre = u16(gate), p.pre2 = u16(up);
   p.ldy[0] = ldh, p.ldp = ldg, p.ldp2 = ldu;
   p.act = act, p.bf16 = dtype == kBF16;
-  return few ? dense_rows(p, s, who) : dense_mma(p, s, who);
+  return few ? dense_rows(p, s, who) : dense_mma(&p, 1, DenseColSum(), s, who);
 }
 
 extern "C" int eas_linear_backward(const eas_linear_backward_args* args, void* stream) {
@@ -502,18 +477,16 @@ extern "C" int eas_linear_backward(const eas_linear_backward_args* args, void* s
     g.v_dy = vec_ok(dy, lddy), g.v_g = pre && vec_ok(pre, ldp);
     rc = launch_act_grad<false>(g, sc.blocks, s, who);
     if (rc) return rc;
-    if (db) {
-      ColSum c = {partial, u16(db), sc.blocks, (int)N, dtype == kBF16};
-      rc = dense_launch(reinterpret_cast<const void*>(&colsum_kernel), dim3((N + 31) / 32), 0, 256, 0, s, &c, who);
-      if (rc) return rc;
-    }
   }
   Copies copies;
   const Operand X = dw ? copies.add(x, ldx, M, K, off & kXOff, scratch, sc.x, sc.ldk) : Operand{};
   const Operand W = dx ? copies.add(w, ldw, N, K, off & kWOff, scratch, sc.w, sc.ldk) : Operand{};
   if ((rc = copies.launch(s, who))) return rc;
   const Operand DZ = dz ? Operand{dz, sc.ldn} : Operand{u16(dy), lddy};
-  return backward_products(who, 1, {DZ, {}}, {W, {}}, X, dx, lddx, {dw, nullptr}, {lddw, 0}, M, N, K, dtype, s);
+  DenseColSum sums;
+  if (db) sums.partial = partial, sums.db = u16(db), sums.blocks = sc.blocks, sums.N = (int)N, sums.bf16 = dtype == kBF16;
+  if (!dx && !dw) return dense_column_sums(sums, s, who);
+  return backward_products(who, 1, {DZ, {}}, {W, {}}, X, dx, lddx, {dw, nullptr}, {lddw, 0}, sums, M, N, K, dtype, s);
 }
 
 extern "C" int eas_gated_backward(const eas_gated_backward_args* args, void* stream) {
@@ -561,5 +534,5 @@ extern "C" int eas_gated_backward(const eas_gated_backward_args* args, void* str
   const Operand U = dx ? copies.add(w_up, ldwu, N, K, off & kUpOff, scratch, sc.up, sc.ldk) : Operand{};
   if ((rc = copies.launch(s, who))) return rc;
   return backward_products(who, 2, {{dg, sc.ldn}, {du, sc.ldn}}, {G, U}, X, dx, lddx, {dw_gate, dw_up},
-                           {lddwg, lddwu}, M, N, K, dtype, s);
+                           {lddwg, lddwu}, DenseColSum(), M, N, K, dtype, s);
 }

@@ -9,6 +9,8 @@
 //   batch 2 two products with one B: y_z = A_z B_0^T, z = 0, 1    (plain, terms = 1)
 // A_t[m][k] is at a[t] + m lda[t] + k, or at a[t] + k lda[t] + m when a_mn; B_t likewise by n.
 // Operand bases and pitches are multiples of 16 bytes; those of the other arrays are arbitrary.
+// Forward products have K-major operands (neither a_mn nor b_mn) and one term; backward ones have b_mn
+// and no epilogue.
 struct DenseProduct {
   const uint16_t* a[2] = {nullptr, nullptr};
   const uint16_t* b[2] = {nullptr, nullptr};
@@ -26,7 +28,18 @@ struct DenseProduct {
   bool bf16 = false;
 };
 
-int dense_mma(const DenseProduct& p, cudaStream_t stream, const char* who);
+// Column sums of `blocks` rows of N partial sums, rounded to the type: db (may be null: none).
+struct DenseColSum {
+  const float* partial = nullptr;
+  uint16_t* db = nullptr;
+  int blocks = 0, N = 0;
+  bool bf16 = false;
+};
+
+int dense_column_sums(const DenseColSum& sums, cudaStream_t stream, const char* who);
+
+// One forward product, or one or two backward ones (with column sums) that do not depend on one another.
+int dense_mma(const DenseProduct* p, int count, const DenseColSum& sums, cudaStream_t stream, const char* who);
 
 // The same for the forward products (K-major operands, one term, one product) of at most kDenseRows
 // rows that fit in shared memory; operands of any alignment.

@@ -27,21 +27,35 @@ using namespace dense;
 
 constexpr int kBK = 64;  // one 128-byte swizzle row
 
+enum Mode { kForward = 0, kGatedForward = 1, kBackward = 2 };
+
+// One product of a launch.
+struct alignas(64) Job {
+  CUtensorMap a[2], b[2], y[2];
+  uint16_t* y_ptr[2];
+  int64_t ldy[2];
+  int M, N;
+  int kb_term;         // k-blocks of one term
+  int kb_total;        // of all terms
+  int mt, nt, tiles;   // tiles along M and N, and in all
+  int group;           // M tiles that are walked together
+  bool batch2, y_tma, a_mn;
+};
+
 struct alignas(64) Params {
-  CUtensorMap a[2], b[2], y[2], pre, pre2;
+  Job job[2];
+  CUtensorMap pre, pre2;
   const uint16_t* bias;
   const uint16_t* residual;
-  uint16_t* y_ptr[2];
   uint16_t* pre_ptr;
   uint16_t* pre2_ptr;
-  int64_t ldr, ldy[2], ldp, ldp2;
-  int M, N;
-  int kb_term;   // k-blocks of one term
-  int kb_total;  // of all terms
-  int mt, nt, tiles;  // tiles along M and N, and of the whole launch
-  int split;          // CTAs of a cluster that share a tile's k-blocks
+  int64_t ldr, ldp, ldp2;
+  int tiles;   // of all jobs
+  int split;   // CTAs of a cluster that share a tile's k-blocks
+  int ratio;   // tiles of job 1 that take as long as one of job 0
   int act;
-  bool bf16, batch2, y_tma, pre_tma, pre2_tma, bias_vec, res_vec;
+  bool bf16, pre_tma, pre2_tma, bias_vec, res_vec;
+  DenseColSum sums;
   int* status;
 };
 
@@ -140,12 +154,12 @@ constexpr int kStep = MN ? 2048 / 16 : 32 / 16;
       "@e tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], a, b, %3, t;\n\t"                             \
       "add.s64 a, a, %5;\n\tadd.s64 b, b, %6;\n\t"                                                       \
       "@e tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], a, b, %3, t;\n\t}" ::"r"(d),                  \
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "n"(kStep<A_MN>), "n"(kStep<B_MN>)          \
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "l"(a_step), "n"(kStep<B_MN>)                   \
       : "memory")
 
-template <int CG, bool A_MN, bool B_MN>
-__device__ __forceinline__ void mma_kblock(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                           uint32_t accumulate) {
+template <int CG, bool B_MN>
+__device__ __forceinline__ void mma_kblock(uint32_t d, uint64_t a_desc, uint64_t a_step, uint64_t b_desc,
+                                           uint32_t idesc, uint32_t accumulate) {
   if constexpr (CG == 2)
     EAS_MMA_KBLOCK("2");
   else
@@ -237,21 +251,22 @@ __device__ __forceinline__ void put(Boxes& bx, int lane, const CUtensorMap* map,
 // v += the residual's 32 x 32 piece
 template <bool BF16>
 __device__ __forceinline__ void add_residual(const Params& p, Boxes& bx, int lane, int m0, int n0, float (&v)[32]) {
+  const int M = p.job[0].M, N = p.job[0].N;
   uint4 w[4];
-  if (p.res_vec && n0 + 32 <= p.N) {
-    const int m = min(m0 + lane, p.M - 1);  // rows past the last are not stored
+  if (p.res_vec && n0 + 32 <= N) {
+    const int m = min(m0 + lane, M - 1);  // rows past the last are not stored
     const uint4* src = reinterpret_cast<const uint4*>(p.residual + (int64_t)m * p.ldr + n0);
 #pragma unroll
     for (int j = 0; j < 4; ++j) w[j] = src[j];
   } else {
     uint8_t* box = next_box(bx, lane);
-    const int rows = min(32, p.M - m0);
+    const int rows = min(32, M - m0);
     const uint16_t* src = p.residual + (int64_t)m0 * p.ldr + n0 + lane;
 #pragma unroll
     for (int r0 = 0; r0 < 32; r0 += 16) {  // 16 loads under way
       uint16_t h[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) h[r] = r0 + r < rows && n0 + lane < p.N ? src[(r0 + r) * p.ldr] : (uint16_t)0;
+      for (int r = 0; r < 16; ++r) h[r] = r0 + r < rows && n0 + lane < N ? src[(r0 + r) * p.ldr] : (uint16_t)0;
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         *reinterpret_cast<uint16_t*>(box_chunk(box, r0 + r, lane >> 3) + (lane & 7) * 2) = h[r];
@@ -276,7 +291,8 @@ __device__ __forceinline__ void add_residual(const Params& p, Boxes& bx, int lan
 
 template <bool BF16>
 __device__ __forceinline__ void add_bias(const Params& p, int n0, float (&v)[32]) {
-  if (p.bias_vec && n0 + 32 <= p.N) {
+  const int N = p.job[0].N;
+  if (p.bias_vec && n0 + 32 <= N) {
     const uint4* src = reinterpret_cast<const uint4*>(p.bias + n0);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -293,37 +309,40 @@ __device__ __forceinline__ void add_bias(const Params& p, int n0, float (&v)[32]
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      if (n0 + j < p.N) v[j] += to_f32<BF16>(p.bias[n0 + j]);
+      if (n0 + j < N) v[j] += to_f32<BF16>(p.bias[n0 + j]);
   }
 }
 
-// Finish 32 x 32 results from their sums: v = z, or v = g and u.
-template <bool GATED, bool BF16>
-__device__ __forceinline__ void finish_as(const Params& p, Boxes& bx, int lane, int z, int m0, int n0, float (&v)[32],
-                                          const float (&u)[GATED ? 32 : 1]) {
-  if (!GATED && p.bias) add_bias<BF16>(p, n0, v);
-  if (p.pre_ptr) put<BF16>(bx, lane, &p.pre, p.pre_tma, p.pre_ptr, p.ldp, p.M, p.N, m0, n0, v);
-  if constexpr (GATED) {
-    if (p.pre2_ptr) put<BF16>(bx, lane, &p.pre2, p.pre2_tma, p.pre2_ptr, p.ldp2, p.M, p.N, m0, n0, u);
-  }
-  with_act(p.act, [&](auto a) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      v[j] = act<decltype(a)::value>(v[j]);
-      if constexpr (GATED) v[j] *= u[j];
+// Finish 32 x 32 results of a job from their sums: v = z, or v = g and u.
+template <int MODE, bool BF16>
+__device__ __forceinline__ void finish_as(const Params& p, const Job& jb, Boxes& bx, int lane, int z, int m0, int n0,
+                                          float (&v)[32], const float (&u)[MODE == kGatedForward ? 32 : 1]) {
+  constexpr bool GATED = MODE == kGatedForward;
+  if constexpr (MODE != kBackward) {
+    if (!GATED && p.bias) add_bias<BF16>(p, n0, v);
+    if (p.pre_ptr) put<BF16>(bx, lane, &p.pre, p.pre_tma, p.pre_ptr, p.ldp, jb.M, jb.N, m0, n0, v);
+    if constexpr (GATED) {
+      if (p.pre2_ptr) put<BF16>(bx, lane, &p.pre2, p.pre2_tma, p.pre2_ptr, p.ldp2, jb.M, jb.N, m0, n0, u);
     }
-  });
-  if (!GATED && p.residual) add_residual<BF16>(p, bx, lane, m0, n0, v);
-  put<BF16>(bx, lane, &p.y[z], p.y_tma, p.y_ptr[z], p.ldy[z], p.M, p.N, m0, n0, v);
+    with_act(p.act, [&](auto a) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        v[j] = act<decltype(a)::value>(v[j]);
+        if constexpr (GATED) v[j] *= u[j];
+      }
+    });
+    if (!GATED && p.residual) add_residual<BF16>(p, bx, lane, m0, n0, v);
+  }
+  put<BF16>(bx, lane, &jb.y[z], jb.y_tma, jb.y_ptr[z], jb.ldy[z], jb.M, jb.N, m0, n0, v);
 }
 
-template <bool GATED>
-__device__ __forceinline__ void finish(const Params& p, Boxes& bx, int lane, int z, int m0, int n0, float (&v)[32],
-                                       const float (&u)[GATED ? 32 : 1]) {
+template <int MODE>
+__device__ __forceinline__ void finish(const Params& p, const Job& jb, Boxes& bx, int lane, int z, int m0, int n0,
+                                       float (&v)[32], const float (&u)[MODE == kGatedForward ? 32 : 1]) {
   if (p.bf16)
-    finish_as<GATED, true>(p, bx, lane, z, m0, n0, v, u);
+    finish_as<MODE, true>(p, jb, bx, lane, z, m0, n0, v, u);
   else
-    finish_as<GATED, false>(p, bx, lane, z, m0, n0, v, u);
+    finish_as<MODE, false>(p, jb, bx, lane, z, m0, n0, v, u);
 }
 
 __device__ __forceinline__ void as_floats(const uint32_t (&r)[32], float (&v)[32]) {
@@ -332,23 +351,53 @@ __device__ __forceinline__ void as_floats(const uint32_t (&r)[32], float (&v)[32
 }
 
 struct Tile {
-  int z, m, n;
+  int j, z, m, n;
 };
 
-// Tiles in groups of 16 along M, so that the tiles in flight share operands in L2.
+// Tile t of all jobs' tiles.  Within a job they go in groups along M, so that the tiles in flight share
+// operands in L2.
+template <int MODE>
 __device__ __forceinline__ Tile tile_at(const Params& p, int t) {
-  constexpr int kGroup = 16;
   Tile c;
-  const int per_z = p.mt * p.nt;
+  c.j = MODE == kBackward && t >= p.job[0].tiles ? 1 : 0;
+  if (c.j) t -= p.job[0].tiles;
+  const Job& jb = p.job[c.j];
+  const int per_z = jb.mt * jb.nt;
   c.z = t / per_z;
   const int r = t - c.z * per_z;
-  const int g = r / (kGroup * p.nt);
-  const int first = g * kGroup;
-  const int size = min(kGroup, p.mt - first);
-  const int rr = r - g * kGroup * p.nt;
+  const int g = r / (jb.group * jb.nt);
+  const int first = g * jb.group;
+  const int size = min(jb.group, jb.mt - first);
+  const int rr = r - g * jb.group * jb.nt;
   c.m = first + rr % size;
   c.n = rr / size;
   return c;
+}
+
+// The i-th tile of pair `cid` of `pairs` (past the last: -1).  One job: every pair in turn.  Two jobs: job 0
+// is done in turn, and where its last round does not reach all pairs, the others take `ratio` tiles of
+// job 1 meanwhile; then job 1 goes in turn.  (dx of 4096 x 8192 x 4096 has 256 tiles for 74 pairs: alone
+// its fourth round leaves 40 of them idle.)
+template <int MODE>
+__device__ __forceinline__ int pair_tile(const Params& p, int i, int cid, int pairs) {
+  if (MODE != kBackward || p.tiles == p.job[0].tiles) {
+    const int64_t t = (int64_t)i * pairs + cid;
+    return t < p.tiles ? (int)t : -1;
+  }
+  const int t0 = p.job[0].tiles, t1 = p.job[1].tiles;
+  const int full = t0 / pairs, rest = t0 - full * pairs;
+  const int mine = full + (cid < rest ? 1 : 0);
+  if (i < mine) return i * pairs + cid;
+  i -= mine;
+  int64_t t;
+  const int extra = rest ? p.ratio : 0;
+  if (cid >= rest && i < extra) {
+    t = (int64_t)i * (pairs - rest) + (cid - rest);
+  } else {
+    if (cid >= rest) i -= extra;
+    t = (int64_t)extra * (pairs - rest) + (int64_t)i * pairs + cid;
+  }
+  return t < t1 ? t0 + (int)t : -1;
 }
 
 // ---------------------------------------------------------------------------
@@ -369,9 +418,10 @@ constexpr int kPairBars = kPairBoxes + 8 * 2 * kBoxBytes;
 constexpr int kPairSmem = kPairBars + (2 * kPairStages + 4) * 8 + 16 + 1024;
 static_assert(kPairSmem <= 232448, "shared memory over the 227 KB per-CTA limit");
 
-template <bool GATED, bool A_MN, bool B_MN>
+template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     dense_pair_kernel(const __grid_constant__ Params p) {
+  constexpr bool GATED = MODE == kGatedForward, B_MN = MODE == kBackward;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kPairBars);
@@ -397,8 +447,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    prefetch_map(&p.a[0]);
-    prefetch_map(&p.b[0]);
+    prefetch_map(&p.job[0].a[0]);
+    prefetch_map(&p.job[0].b[0]);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot))
@@ -421,20 +471,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const uint32_t leader_full = mapa_rank(full0, 0);
     int s = 0;
     uint32_t ph = 0;
-    for (int t = cid; t < p.tiles && going(abort_flag); t += ncl) {
-      const Tile c = tile_at(p, t);
+    for (int i = 0; going(abort_flag); ++i) {
+      const int t = pair_tile<MODE>(p, i, cid, ncl);
+      if (t < 0) break;
+      const Tile c = tile_at<MODE>(p, t);
+      const Job& jb = p.job[c.j];
+      const bool a_mn = MODE == kBackward && jb.a_mn;
       const int m0 = c.m * 256 + 128 * (int)rank;
       const int n0 = c.n * kTileN + (GATED ? 0 : 128 * (int)rank);
       int term = 0, k0 = 0;
-      for (int kb = 0; kb < p.kb_total; ++kb) {
+      for (int kb = 0; kb < jb.kb_total; ++kb) {
         if (!warp_wait(&empty[s], ph ^ 1, abort_flag)) break;
-        if (kb == p.kb_term) term = 1, k0 = 0;
-        const CUtensorMap* ma = &p.a[p.batch2 ? c.z : term];
-        const CUtensorMap* mb = &p.b[GATED ? (int)rank : term];
+        if (kb == jb.kb_term) term = 1, k0 = 0;
+        const CUtensorMap* ma = &jb.a[jb.batch2 ? c.z : term];
+        const CUtensorMap* mb = &jb.b[GATED ? (int)rank : term];
         const uint32_t fl = leader_full + s * 8;
         if (rank == 0) expect_tx(full0 + s * 8, 2 * kPairStageBytes);
         const uint32_t sa = ring + s * kPairStageBytes, sb = sa + 128 * kBK * 2;
-        if (A_MN) {
+        if (a_mn) {
           tma_load_2d_pair(sa, ma, fl, m0, k0);
           tma_load_2d_pair(sa + kBK * 128, ma, fl, m0 + 64, k0);
         } else {
@@ -455,23 +509,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     }
   } else if (warp == 1) {
     if (rank == 0) {
-      const uint32_t idesc = instr_desc(256, 256, A_MN, B_MN, p.bf16);
-      const uint64_t a0 = operand_desc<A_MN>(ring), b0 = operand_desc<B_MN>(ring + 128 * kBK * 2);
-      int s = 0, local = 0;
+      const uint64_t b0 = operand_desc<B_MN>(ring + 128 * kBK * 2);
+      int s = 0;
       uint32_t ph = 0;
-      for (int t = cid; t < p.tiles && going(abort_flag); t += ncl, ++local) {
-        const int buf = local & 1;
-        if (!warp_wait<true>(&acc_empty[buf], ((local >> 1) & 1) ^ 1, abort_flag)) break;
+      for (int i = 0; going(abort_flag); ++i) {
+        const int t = pair_tile<MODE>(p, i, cid, ncl);
+        if (t < 0) break;
+        const Job& jb = p.job[MODE == kBackward && t >= p.job[0].tiles ? 1 : 0];
+        const bool a_mn = MODE == kBackward && jb.a_mn;
+        const uint32_t idesc = instr_desc(256, 256, a_mn, B_MN, p.bf16);
+        const uint64_t a0 = a_mn ? operand_desc<true>(ring) : operand_desc<false>(ring);
+        const uint64_t a_step = a_mn ? kStep<true> : kStep<false>;
+        const int buf = i & 1;
+        if (!warp_wait<true>(&acc_empty[buf], ((i >> 1) & 1) ^ 1, abort_flag)) break;
         tc_fence_after();
         const uint32_t d = tmem + buf * 256;
         bool ok = true;
-        for (int kb = 0; kb < p.kb_total; ++kb) {
+        for (int kb = 0; kb < jb.kb_total; ++kb) {
           if (!warp_wait(&full[s], ph, abort_flag)) {
             ok = false;
             break;
           }
           const uint64_t at = (uint64_t)(s * (kPairStageBytes / 16));
-          mma_kblock<2, A_MN, B_MN>(d, a0 + at, b0 + at, idesc, kb);
+          mma_kblock<2, B_MN>(d, a0 + at, a_step, b0 + at, idesc, kb);
           commit<2>(empty0 + s * 8);
           if (++s == kPairStages) {
             s = 0;
@@ -486,20 +546,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const int q = warp & 3, half = (warp - 2) >> 2;
     Boxes bx = {smem + kPairBoxes + (warp - 2) * 2 * kBoxBytes, 0};
     const uint32_t leader[2] = {mapa_rank(smem_u32(&acc_empty[0]), 0), mapa_rank(smem_u32(&acc_empty[1]), 0)};
-    int local = 0;
-    for (int t = cid; t < p.tiles && going(abort_flag); t += ncl, ++local) {
-      const int buf = local & 1;
-      if (!warp_wait(&acc_full[buf], (local >> 1) & 1, abort_flag)) break;
+    for (int i = 0; going(abort_flag); ++i) {
+      const int t = pair_tile<MODE>(p, i, cid, ncl);
+      if (t < 0) break;
+      const int buf = i & 1;
+      if (!warp_wait(&acc_full[buf], (i >> 1) & 1, abort_flag)) break;
       tc_fence_after();
-      const Tile c = tile_at(p, t);
+      const Tile c = tile_at<MODE>(p, t);
+      const Job& jb = p.job[c.j];
       const int m0 = c.m * 256 + 128 * (int)rank + q * 32;
       const uint32_t acc = tmem + buf * 256 + ((uint32_t)(q * 32) << 16);
       constexpr int kCols = GATED ? 64 : 128;  // of this warp
-      if (m0 < p.M) {
+      if (m0 < jb.M) {
 #pragma unroll 1
         for (int cc = 0; cc < kCols; cc += 32) {
           const int col = half * kCols + cc, n0 = c.n * kTileN + col;
-          if (n0 >= p.N) break;
+          if (n0 >= jb.N) break;
           uint32_t r[32];
           float v[32], u[GATED ? 32 : 1];
           tmem_ld32(acc + col, r);
@@ -508,7 +570,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             tmem_ld32(acc + 128 + col, r);
             as_floats(r, u);
           }
-          finish<GATED>(p, bx, lane, c.z, m0, n0, v, u);
+          finish<MODE>(p, jb, bx, lane, c.z, m0, n0, v, u);
         }
       }
       tc_fence_before();
@@ -561,9 +623,32 @@ struct TileShape {
   static_assert(kSmem <= (DEEP ? 232448 : 115000), "shared memory");
 };
 
-template <int BN, int AR, bool DEEP, bool GATED, bool A_MN, bool B_MN>
+// db of 32 columns from n0 on: each row of threads adds every 6th row block, then the rows are added in order.
+__device__ __forceinline__ void column_sums(const DenseColSum& c, int n0, float* sums) {
+  constexpr int kRows = kTileThreads / 32;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, n = n0 + tx;
+  float s = 0;
+  if (n < c.N) {
+#pragma unroll 8
+    for (int b = ty; b < c.blocks; b += kRows) s += c.partial[(int64_t)b * c.N + n];
+  }
+  sums[ty * 32 + tx] = s;
+  __syncthreads();
+  if (ty || n >= c.N) return;
+#pragma unroll
+  for (int r = 1; r < kRows; ++r) s += sums[r * 32 + tx];
+  c.db[n] = c.bf16 ? to_16<true>(s) : to_16<false>(s);
+}
+
+__global__ void __launch_bounds__(kTileThreads) column_sums_kernel(const __grid_constant__ DenseColSum c) {
+  __shared__ float sums[kTileThreads];
+  grid_order();
+  column_sums(c, blockIdx.x * 32, sums);
+}
+
+template <int BN, int AR, bool DEEP, int MODE>
 __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(const __grid_constant__ Params p) {
-  static_assert(AR == 128 || !A_MN, "MN-major A comes in 64-wide pieces of all 128 rows");
+  constexpr bool GATED = MODE == kGatedForward, B_MN = MODE == kBackward;
   using L = TileShape<BN, AR, DEEP>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -575,6 +660,11 @@ __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);  // uniform
   const int lane = threadIdx.x & 31;
   const int S = p.split;
+  if (MODE == kBackward && (int)blockIdx.x >= p.tiles * S) {  // CTAs behind the tiles': column sums
+    grid_order();
+    column_sums(p.sums, ((int)blockIdx.x - p.tiles * S) * 32, reinterpret_cast<float*>(smem));
+    return;
+  }
   const int rank = (int)blockIdx.x % S;  // consecutive blocks form a cluster
 
   if (threadIdx.x == 0) {
@@ -586,8 +676,6 @@ __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    prefetch_map(&p.a[0]);
-    prefetch_map(&p.b[0]);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(BN)
@@ -601,9 +689,11 @@ __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(
   grid_order();
 
   constexpr int kTileN = GATED ? BN / 2 : BN;
-  const Tile c = tile_at(p, (int)blockIdx.x / S);
+  const Tile c = tile_at<MODE>(p, (int)blockIdx.x / S);
+  const Job& jb = p.job[c.j];
+  const bool a_mn = MODE == kBackward && jb.a_mn;  // (only with AR = 128: it comes in 64-wide pieces of all rows)
   const int m0 = c.m * 128, n0 = c.n * kTileN;
-  const int kb_lo = (int)((int64_t)rank * p.kb_total / S), kb_hi = (int)((int64_t)(rank + 1) * p.kb_total / S);
+  const int kb_lo = (int)((int64_t)rank * jb.kb_total / S), kb_hi = (int)((int64_t)(rank + 1) * jb.kb_total / S);
 
   const uint32_t ring = smem_u32(smem), full0 = smem_u32(full), empty0 = smem_u32(empty);
 
@@ -614,24 +704,24 @@ __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(
       if (!warp_wait(&empty[s], ph ^ 1, abort_flag)) break;
       const uint32_t fl = full0 + s * 8;
       expect_tx(fl, L::kStageBytes);
-      const int term = kb >= p.kb_term ? 1 : 0;
-      const int k0 = (kb - term * p.kb_term) * kBK;
-      const CUtensorMap* ma = &p.a[p.batch2 ? c.z : term];
+      const int term = kb >= jb.kb_term ? 1 : 0;
+      const int k0 = (kb - term * jb.kb_term) * kBK;
+      const CUtensorMap* ma = &jb.a[jb.batch2 ? c.z : term];
       const uint32_t sa = ring + s * L::kStageBytes, sb = sa + L::kABytes;
-      if (A_MN) {
+      if (a_mn) {
         tma_load_2d(sa, ma, fl, m0, k0);
         tma_load_2d(sa + kBK * 128, ma, fl, m0 + 64, k0);
       } else {
         tma_load_2d(sa, ma, fl, k0, m0);
       }
       if (GATED) {
-        tma_load_2d(sb, &p.b[0], fl, k0, n0);
-        tma_load_2d(sb + kTileN * 128, &p.b[1], fl, k0, n0);
+        tma_load_2d(sb, &jb.b[0], fl, k0, n0);
+        tma_load_2d(sb + kTileN * 128, &jb.b[1], fl, k0, n0);
       } else if (B_MN) {
 #pragma unroll
-        for (int j = 0; j < BN / 64; ++j) tma_load_2d(sb + j * kBK * 128, &p.b[term], fl, n0 + 64 * j, k0);
+        for (int j = 0; j < BN / 64; ++j) tma_load_2d(sb + j * kBK * 128, &jb.b[term], fl, n0 + 64 * j, k0);
       } else {
-        tma_load_2d(sb, &p.b[term], fl, k0, n0);
+        tma_load_2d(sb, &jb.b[term], fl, k0, n0);
       }
       if (++s == L::kStages) {
         s = 0;
@@ -639,8 +729,10 @@ __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(
       }
     }
   } else if (warp == 1) {
-    const uint32_t idesc = instr_desc(128, BN, A_MN, B_MN, p.bf16);
-    const uint64_t a0 = operand_desc<A_MN>(ring), b0 = operand_desc<B_MN>(ring + L::kABytes);
+    const uint32_t idesc = instr_desc(128, BN, a_mn, B_MN, p.bf16);
+    const uint64_t a0 = a_mn ? operand_desc<true>(ring) : operand_desc<false>(ring);
+    const uint64_t a_step = a_mn ? kStep<true> : kStep<false>;
+    const uint64_t b0 = operand_desc<B_MN>(ring + L::kABytes);
     int s = 0;
     uint32_t ph = 0;
     bool ok = true;
@@ -650,7 +742,7 @@ __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(
         break;
       }
       const uint64_t at = (uint64_t)(s * (L::kStageBytes / 16));
-      mma_kblock<1, A_MN, B_MN>(tmem, a0 + at, b0 + at, idesc, kb - kb_lo);
+      mma_kblock<1, B_MN>(tmem, a0 + at, a_step, b0 + at, idesc, kb - kb_lo);
       commit<1>(empty0 + s * 8);
       if (++s == L::kStages) {
         s = 0;
@@ -665,9 +757,9 @@ __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(
     const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16);
     if (S == 1) {
       Boxes bx = {smem + L::kBoxes + q * 2 * kBoxBytes, 0};
-      if (m0 + q * 32 < p.M) {
+      if (m0 + q * 32 < jb.M) {
 #pragma unroll 1
-        for (int cc = 0; cc < kTileN && n0 + cc < p.N; cc += 32) {
+        for (int cc = 0; cc < kTileN && n0 + cc < jb.N; cc += 32) {
           uint32_t r[32];
           float v[32], u[GATED ? 32 : 1];
           tmem_ld32(acc + cc, r);
@@ -676,11 +768,11 @@ __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(
             tmem_ld32(acc + kTileN + cc, r);
             as_floats(r, u);
           }
-          finish<GATED>(p, bx, lane, c.z, m0 + q * 32, n0 + cc, v, u);
+          finish<MODE>(p, jb, bx, lane, c.z, m0 + q * 32, n0 + cc, v, u);
         }
       }
       if (lane == 0) bulk_wait_all0();
-    } else if (m0 + q * 32 < p.M) {
+    } else if (m0 + q * 32 < jb.M) {
       float* part = reinterpret_cast<float*>(smem) + q * 32 + lane;
 #pragma unroll 1
       for (int cc = 0; cc < BN; cc += 32) {
@@ -699,8 +791,8 @@ __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(
     if (warp >= 2) {
       const int e = warp - 2;
       Boxes bx = {smem + L::kBoxes + e * 2 * kBoxBytes, 0};
-      const int quarters = min(4, (p.M - m0 + 31) / 32);
-      const int pieces = min(kTileN, p.N - n0 + 31) / 32 * quarters;
+      const int quarters = min(4, (jb.M - m0 + 31) / 32);
+      const int pieces = min(kTileN, jb.N - n0 + 31) / 32 * quarters;
       for (int i = rank + e * S; i < pieces; i += 4 * S) {
         const int q = i % quarters, cc = i / quarters * 32;
         const uint32_t at = smem_u32(smem) + (uint32_t)(cc * 128 + q * 32 + lane) * 4;
@@ -720,7 +812,7 @@ __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(
             for (int j = 0; j < 32; ++j) u[j] += ld_cluster_f32(from + (kTileN + j) * 512);
           }
         }
-        finish<GATED>(p, bx, lane, c.z, m0 + q * 32, n0 + cc, v, u);
+        finish<MODE>(p, jb, bx, lane, c.z, m0 + q * 32, n0 + cc, v, u);
       }
       if (lane == 0) bulk_wait_all0();
     }
@@ -757,8 +849,8 @@ int encode(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uin
 
 bool aligned16(const void* p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld & 7) == 0; }
 
-// Operand maps (a_rows, b_rows: rows of a K-major operand per box), epilogue arrays, and the tile grid of tile_m x tile_n outputs.
-int fill(Params& q, const DenseProduct& p, int a_rows, int b_rows, int tile_m, int tile_n, const char* who) {
+// One job: operand maps (a_rows, b_rows: rows of a K-major operand per box), results, tiles of tile_m x tile_n.
+int fill_job(Job& q, const DenseProduct& p, int a_rows, int b_rows, int tile_m, int tile_n, const char* who) {
   int rc = EAS_OK;
   const int na = p.terms > 1 || p.batch > 1 ? 2 : 1;
   const int nb = p.terms > 1 || p.gated ? 2 : 1;
@@ -768,11 +860,29 @@ int fill(Params& q, const DenseProduct& p, int a_rows, int b_rows, int tile_m, i
   for (int t = 0; t < nb && !rc; ++t)
     rc = p.b_mn ? encode(&q.b[t], p.b[t], p.K, p.N, p.ldb[t], kBK, 64, CU_TENSOR_MAP_SWIZZLE_128B, who)
                 : encode(&q.b[t], p.b[t], p.N, p.K, p.ldb[t], b_rows, kBK, CU_TENSOR_MAP_SWIZZLE_128B, who);
-  if (rc) return rc;
   q.y_tma = aligned16(p.y[0], p.ldy[0]) && (p.batch < 2 || aligned16(p.y[1], p.ldy[1]));
   for (int z = 0; z < p.batch && q.y_tma && !rc; ++z)
     rc = encode(&q.y[z], p.y[z], p.M, p.N, p.ldy[z], 32, 32, CU_TENSOR_MAP_SWIZZLE_64B, who);
-  if (!rc && p.pre && (q.pre_tma = aligned16(p.pre, p.ldp)))
+  if (rc) return rc;
+  for (int z = 0; z < 2; ++z) q.y_ptr[z] = p.y[z], q.ldy[z] = (int64_t)p.ldy[z];
+  q.M = p.M, q.N = p.N;
+  q.kb_term = (p.K + kBK - 1) / kBK;
+  q.kb_total = q.kb_term * p.terms;
+  const int64_t mt = ((int64_t)p.M + tile_m - 1) / tile_m, nt = ((int64_t)p.N + tile_n - 1) / tile_n;
+  if (mt * nt * p.batch > 0x1fffffff) return eas_fail(EAS_ERR_VALUE, "%s: too many output tiles", who);
+  q.mt = (int)mt, q.nt = (int)nt, q.tiles = (int)(mt * nt * p.batch);
+  // As many M tiles as keep their rows of A in half of L2 from one column of tiles to the next: 16 of
+  // 256 rows up to K of 4882, else 8 (8192^3: 838 us by 8, 855 by 16; 8192 x 2 8192 x 4096: 773, 761).
+  q.group = (int64_t)16 * tile_m * p.K * 2 <= 40000000 ? 16 : 8;
+  q.batch2 = p.batch > 1;
+  q.a_mn = p.a_mn;
+  return EAS_OK;
+}
+
+// What the epilogue of a forward product takes.
+int fill_epilogue(Params& q, const DenseProduct& p, const char* who) {
+  int rc = EAS_OK;
+  if (p.pre && (q.pre_tma = aligned16(p.pre, p.ldp)))
     rc = encode(&q.pre, p.pre, p.M, p.N, p.ldp, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B, who);
   if (!rc && p.pre2 && (q.pre2_tma = aligned16(p.pre2, p.ldp2)))
     rc = encode(&q.pre2, p.pre2, p.M, p.N, p.ldp2, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B, who);
@@ -780,18 +890,9 @@ int fill(Params& q, const DenseProduct& p, int a_rows, int b_rows, int tile_m, i
   q.bias = p.bias, q.residual = p.residual;
   q.bias_vec = (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0;
   q.res_vec = aligned16(p.residual, p.ldr);
-  for (int z = 0; z < 2; ++z) q.y_ptr[z] = p.y[z], q.ldy[z] = (int64_t)p.ldy[z];
   q.pre_ptr = p.pre, q.pre2_ptr = p.pre2;
   q.ldr = (int64_t)p.ldr, q.ldp = (int64_t)p.ldp, q.ldp2 = (int64_t)p.ldp2;
-  q.M = p.M, q.N = p.N;
-  q.kb_term = (p.K + kBK - 1) / kBK;
-  if ((int64_t)q.kb_term * p.terms > 0x7fffffff) return eas_fail(EAS_ERR_VALUE, "%s: too many products in a sum", who);
-  q.kb_total = q.kb_term * p.terms;
-  const int64_t mt = ((int64_t)p.M + tile_m - 1) / tile_m, nt = ((int64_t)p.N + tile_n - 1) / tile_n;
-  if (mt * nt * p.batch > 0x3fffffff) return eas_fail(EAS_ERR_VALUE, "%s: too many output tiles", who);
-  q.mt = (int)mt, q.nt = (int)nt, q.tiles = (int)(mt * nt * p.batch);
-  q.batch2 = p.batch > 1;
-  q.act = p.act, q.bf16 = p.bf16;
+  q.act = p.act;
   return EAS_OK;
 }
 
@@ -800,10 +901,10 @@ struct KernelState {
   int pairs[64] = {0};
 };
 
-template <bool GATED, bool A_MN, bool B_MN>
+template <int MODE>
 int launch_pair(Params& q, int dev, cudaStream_t s, const char* who) {
   static KernelState st;
-  const void* kernel = reinterpret_cast<const void*>(&dense_pair_kernel<GATED, A_MN, B_MN>);
+  const void* kernel = reinterpret_cast<const void*>(&dense_pair_kernel<MODE>);
   const int slot = dev >= 0 && dev < 64 ? dev : 0;
   if (!st.pairs[slot]) {
     int rc = eas_cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem), who,
@@ -824,11 +925,13 @@ int launch_pair(Params& q, int dev, cudaStream_t s, const char* who) {
   return dense_launch(kernel, dim3(2 * pairs), 0, kPairThreads, kPairSmem, s, &q, who);
 }
 
-template <int BN, int AR, bool DEEP, bool GATED, bool A_MN, bool B_MN>
+template <int BN, int AR, bool DEEP, int MODE>
 int launch_tile(Params& q, int dev, cudaStream_t s, const char* who) {
+  // whole clusters of column-sum CTAs
+  const int sums = q.sums.db ? ((q.sums.N + 31) / 32 + q.split - 1) / q.split * q.split : 0;
   static bool ready[64] = {false};
   using L = TileShape<BN, AR, DEEP>;
-  const void* kernel = reinterpret_cast<const void*>(&dense_tile_kernel<BN, AR, DEEP, GATED, A_MN, B_MN>);
+  const void* kernel = reinterpret_cast<const void*>(&dense_tile_kernel<BN, AR, DEEP, MODE>);
   const int slot = dev >= 0 && dev < 64 ? dev : 0;
   if (!ready[slot]) {
     int rc = eas_cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem), who,
@@ -836,7 +939,8 @@ int launch_tile(Params& q, int dev, cudaStream_t s, const char* who) {
     if (rc) return rc;
     ready[slot] = true;
   }
-  return dense_launch(kernel, dim3(q.tiles * q.split), q.split > 1 ? q.split : 0, kTileThreads, L::kSmem, s, &q, who);
+  return dense_launch(kernel, dim3((unsigned)(q.tiles * q.split + sums)), q.split > 1 ? q.split : 0, kTileThreads, L::kSmem, s, &q,
+                      who);
 }
 
 struct Choice {
@@ -847,8 +951,7 @@ struct Choice {
 };
 
 // The shape of least estimated time, in microseconds as measured on one B200 at 1.9 GHz (bf16,
-// operands from HBM; the sweep behind the constants is in the comments).  A step is one 64-deep
-// k-block of one CTA or pair.
+// operands from HBM).  A step is one 64-deep k-block of one CTA or pair.
 //   pair, 256 x 256        5.5 + rounds x k-blocks x 0.31   (4096^3: 94 us; 512 x 4096 x 4096: 25.3)
 //   one CTA per SM         4.5 + k-blocks x step, step 0.15 (BN 64) or 0.205 (128), 0.115 or 0.155 with
 //                          64 rows of A   (64 x 4096 x 4096: 12.3 BN 64, 15.0 BN 128)
@@ -856,30 +959,53 @@ struct Choice {
 //                          (2048^3: 25.1 BN 64, 17.5 BN 128)
 //   a split over 2 or 4    2 or 2.8 more for the exchange, and only while all CTAs are resident at
 //                          once (16 x 4096 x 4096, BN 64: 11.9 whole, 10.2 split in 2, 17.9 in 8)
-Choice choose(const DenseProduct& p, int sms) {
-  const int64_t kb = (int64_t)((p.K + kBK - 1) / kBK) * p.terms;
+Choice choose(const DenseProduct* p, int count, int sms) {
   const int pairs = sms / 2 > 0 ? sms / 2 : 1;
-  auto tiles_of = [&](int m, int width) {
-    const int n = p.gated ? width / 2 : width;
-    return (int64_t)((p.M + (int64_t)m - 1) / m) * ((p.N + (int64_t)n - 1) / n) * p.batch;
+  int64_t kb[2], most_kb = 0, least_kb = INT64_MAX;
+  int most_rows = 0;
+  bool a_mn = false;
+  for (int i = 0; i < count; ++i) {
+    kb[i] = (int64_t)((p[i].K + kBK - 1) / kBK) * p[i].terms;
+    most_kb = kb[i] > most_kb ? kb[i] : most_kb;
+    least_kb = kb[i] < least_kb ? kb[i] : least_kb;
+    most_rows = p[i].M > most_rows ? p[i].M : most_rows;
+    a_mn |= p[i].a_mn;
+  }
+  auto tiles_of = [&](int i, int m, int width) {
+    const int n = p[i].gated ? width / 2 : width;
+    return (int64_t)((p[i].M + (int64_t)m - 1) / m) * ((p[i].N + (int64_t)n - 1) / n) * p[i].batch;
   };
   Choice best = {0, 1, 128, false};
-  double best_us = 5.5 + (double)((tiles_of(256, 256) + pairs - 1) / pairs) * kb * 0.31;
+  double best_us;
+  if (count == 1) {
+    best_us = 5.5 + (double)((tiles_of(0, 256, 256) + pairs - 1) / pairs) * kb[0] * 0.31;
+  } else {  // the jobs fill one another's last rounds
+    double steps = 0;
+    for (int i = 0; i < count; ++i) steps += (double)tiles_of(i, 256, 256) * kb[i];
+    steps = steps / pairs + 0.5 * least_kb;
+    best_us = 5.5 + (steps > most_kb ? steps : most_kb) * 0.31;
+  }
   for (int bn = 64; bn <= 128; bn += 64) {
-    const int64_t tiles = tiles_of(128, bn);
+    int64_t tiles = 0;
+    double work = 0;  // steps of all tiles, with what a tile costs beside its steps
+    const double shared = bn == 64 ? 0.2 : 0.26, tile_us = bn == 64 ? 0.6 : 0.9;
+    for (int i = 0; i < count; ++i) {
+      const int64_t n = tiles_of(i, 128, bn);
+      tiles += n;
+      work += (double)n * (kb[i] * shared + tile_us);
+    }
     for (int split = 1; split <= 4; split *= 2) {
       const int64_t ctas = tiles * split;
-      if (split > 1 && (ctas > sms * 7 / 8 || kb < 2 * split)) break;
+      if (split > 1 && (ctas > sms * 7 / 8 || least_kb < 2 * split)) break;
       Choice c = {bn, split, 128, ctas <= sms};
       double us;
       if (c.deep) {
-        if (p.M <= 64 && !p.a_mn) c.ar = 64;
+        if (most_rows <= 64 && !a_mn) c.ar = 64;
         const double step = bn == 64 ? (c.ar == 64 ? 0.115 : 0.15) : (c.ar == 64 ? 0.155 : 0.205);
-        us = 4.5 + (double)((kb + split - 1) / split) * step + (split == 1 ? 0 : split == 2 ? 2 : 2.8);
+        us = 4.5 + (double)((most_kb + split - 1) / split) * step + (split == 1 ? 0 : split == 2 ? 2 : 2.8);
       } else {
-        double per_sm = (double)ctas / sms;
-        if (per_sm < 1.8) per_sm = 1.8;  // some SM has two
-        us = 4.0 + per_sm * (kb * (bn == 64 ? 0.2 : 0.26) + (bn == 64 ? 0.6 : 0.9));
+        const double two = 1.8 * (most_kb * shared + tile_us);  // some SM has two tiles
+        us = 4.0 + (work / sms > two ? work / sms : two);
       }
       if (us < best_us) best = c, best_us = us;
     }
@@ -887,37 +1013,59 @@ Choice choose(const DenseProduct& p, int sms) {
   return best;
 }
 
-template <bool GATED, bool A_MN, bool B_MN>
+template <int MODE>
 int launch_choice(const Choice& c, Params& q, int dev, cudaStream_t s, const char* who) {
-  if (c.bn == 0) return launch_pair<GATED, A_MN, B_MN>(q, dev, s, who);
-  if constexpr (!A_MN) {
-    if (c.ar == 64)
-      return c.bn == 64 ? launch_tile<64, 64, true, GATED, A_MN, B_MN>(q, dev, s, who)
-                        : launch_tile<128, 64, true, GATED, A_MN, B_MN>(q, dev, s, who);
+  if (c.bn == 0) {
+    if (q.sums.db) {
+      int rc = dense_column_sums(q.sums, s, who);
+      if (rc) return rc;
+    }
+    return launch_pair<MODE>(q, dev, s, who);
   }
+  if (c.ar == 64)
+    return c.bn == 64 ? launch_tile<64, 64, true, MODE>(q, dev, s, who) : launch_tile<128, 64, true, MODE>(q, dev, s, who);
   if (c.bn == 64)
-    return c.deep ? launch_tile<64, 128, true, GATED, A_MN, B_MN>(q, dev, s, who)
-                  : launch_tile<64, 128, false, GATED, A_MN, B_MN>(q, dev, s, who);
-  return c.deep ? launch_tile<128, 128, true, GATED, A_MN, B_MN>(q, dev, s, who)
-                : launch_tile<128, 128, false, GATED, A_MN, B_MN>(q, dev, s, who);
+    return c.deep ? launch_tile<64, 128, true, MODE>(q, dev, s, who) : launch_tile<64, 128, false, MODE>(q, dev, s, who);
+  return c.deep ? launch_tile<128, 128, true, MODE>(q, dev, s, who) : launch_tile<128, 128, false, MODE>(q, dev, s, who);
 }
 
 }  // namespace
 
-int dense_mma(const DenseProduct& p, cudaStream_t stream, const char* who) {
+int dense_column_sums(const DenseColSum& sums, cudaStream_t stream, const char* who) {
+  DenseColSum c = sums;
+  return dense_launch(reinterpret_cast<const void*>(&column_sums_kernel), dim3((unsigned)((c.N + 31) / 32)), 0,
+                      kTileThreads, 0, stream, &c, who);
+}
+
+int dense_mma(const DenseProduct* p, int count, const DenseColSum& sums, cudaStream_t stream, const char* who) {
   int dev = 0;
   int rc = eas_cuda_check(cudaGetDevice(&dev), who, EAS_ERR_UNAVAILABLE);
   if (rc) return rc;
-  const Choice c = choose(p, dense_sms(dev));
-  Params q = {};
-  q.status = eas_native_status_dev(dev);
-  q.split = c.split;
+  DenseProduct order[2] = {p[0], count > 1 ? p[1] : p[0]};
+  auto steps = [](const DenseProduct& v) { return (int64_t)((v.K + kBK - 1) / kBK) * v.terms; };
+  if (count > 1 && steps(order[0]) < steps(order[1])) {  // the longer tiles first
+    order[0] = p[1];
+    order[1] = p[0];
+  }
+  for (int i = 0; i < count; ++i)
+    if (steps(order[i]) > 0x7fffffff) return eas_fail(EAS_ERR_VALUE, "%s: too many products in a sum", who);
+  const Choice c = choose(order, count, dense_sms(dev));
+  const bool gated = p[0].gated;
   const int width = c.bn ? c.bn : 256;  // of the accumulator: a gated tile has half as many outputs
-  const int b_rows = !c.bn ? 128 : (p.gated ? c.bn / 2 : c.bn);
-  rc = fill(q, p, c.ar, b_rows, c.bn ? 128 : 256, p.gated ? width / 2 : width, who);
+  const int b_rows = !c.bn ? 128 : (gated ? c.bn / 2 : c.bn);
+  Params q = {};
+  for (int i = 0; i < count; ++i) {
+    rc = fill_job(q.job[i], order[i], c.ar, b_rows, c.bn ? 128 : 256, gated ? width / 2 : width, who);
+    if (rc) return rc;
+    q.tiles += q.job[i].tiles;
+  }
+  if (count > 1) q.ratio = (q.job[0].kb_total + q.job[1].kb_total / 2) / q.job[1].kb_total;
+  q.split = c.split;
+  q.bf16 = p[0].bf16;
+  q.sums = sums;
+  q.status = eas_native_status_dev(dev);
+  if (p[0].b_mn) return launch_choice<kBackward>(c, q, dev, stream, who);
+  rc = fill_epilogue(q, p[0], who);
   if (rc) return rc;
-  if (p.gated) return launch_choice<true, false, false>(c, q, dev, stream, who);
-  if (p.a_mn) return launch_choice<false, true, true>(c, q, dev, stream, who);
-  if (p.b_mn) return launch_choice<false, false, true>(c, q, dev, stream, who);
-  return launch_choice<false, false, false>(c, q, dev, stream, who);
+  return gated ? launch_choice<kGatedForward>(c, q, dev, stream, who) : launch_choice<kForward>(c, q, dev, stream, who);
 }
