@@ -215,6 +215,18 @@ __device__ __forceinline__ uint8_t* box_chunk(uint8_t* box, int row, int chunk) 
   return box + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
 }
 
+// A lane's column of a box: its place in a row takes four values, by row.
+struct ColumnInBox {
+  uint8_t* base[4];
+  __device__ __forceinline__ ColumnInBox(uint8_t* box, int lane) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) base[k] = box + (((lane >> 3) ^ k) << 4) + (lane & 7) * 2;
+  }
+  __device__ __forceinline__ uint16_t* at(int row) const {  // row known at compile time
+    return reinterpret_cast<uint16_t*>(base[(row >> 1) & 3] + row * 64);
+  }
+};
+
 __device__ __forceinline__ uint8_t* next_box(Boxes& bx, int lane) {
   uint8_t* box = bx.base + (bx.n & 1) * kBoxBytes;
   ++bx.n;
@@ -239,11 +251,18 @@ __device__ __forceinline__ void put(Boxes& bx, int lane, const CUtensorMap* map,
   } else {
     __syncwarp();
     const int rows = min(32, M - m0);
-    uint16_t* dst = ptr + (int64_t)m0 * ld + n0 + lane;
-#pragma unroll 8
-    for (int r = 0; r < 32; ++r)
-      if (r < rows && n0 + lane < N)
-        dst[r * ld] = *reinterpret_cast<const uint16_t*>(box_chunk(box, r, lane >> 3) + (lane & 7) * 2);
+    if (n0 + lane < N) {
+      uint16_t* dst = ptr + (int64_t)m0 * ld + n0 + lane;
+      const ColumnInBox col(box, lane);
+      if (rows == 32) {
+#pragma unroll
+        for (int r = 0; r < 32; ++r, dst += ld) *dst = *col.at(r);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 32; ++r, dst += ld)
+          if (r < rows) *dst = *col.at(r);
+      }
+    }
   }
   if (lane == 0) bulk_commit();  // an empty group where nothing was stored: the boxes' turns count groups
 }
@@ -260,16 +279,16 @@ __device__ __forceinline__ void add_residual(const Params& p, Boxes& bx, int lan
     for (int j = 0; j < 4; ++j) w[j] = src[j];
   } else {
     uint8_t* box = next_box(bx, lane);
-    const int rows = min(32, M - m0);
+    const int rows = n0 + lane < N ? min(32, M - m0) : 0;
     const uint16_t* src = p.residual + (int64_t)m0 * p.ldr + n0 + lane;
+    const ColumnInBox col(box, lane);
 #pragma unroll
     for (int r0 = 0; r0 < 32; r0 += 16) {  // 16 loads under way
       uint16_t h[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) h[r] = r0 + r < rows && n0 + lane < N ? src[(r0 + r) * p.ldr] : (uint16_t)0;
+      for (int r = 0; r < 16; ++r, src += p.ldr) h[r] = r0 + r < rows ? *src : (uint16_t)0;
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        *reinterpret_cast<uint16_t*>(box_chunk(box, r0 + r, lane >> 3) + (lane & 7) * 2) = h[r];
+      for (int r = 0; r < 16; ++r) *col.at(r0 + r) = h[r];
     }
     __syncwarp();
 #pragma unroll
