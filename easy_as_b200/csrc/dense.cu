@@ -167,7 +167,7 @@ int launch_act_grad(ActGrad& g, int blocks, cudaStream_t s, const char* who) {
 }
 
 // Copies of operands whose rows TMA cannot read in place, in rows of a multiple of 8 elements (zeros
-// past the end): up to three matrices in one launch, 8 elements per thread.
+// past the end): up to three matrices in one launch (one per row of blocks), 8 elements per thread.
 struct Repitch {
   struct Matrix {
     const uint16_t* src;
@@ -180,22 +180,20 @@ struct Repitch {
 
 __global__ void __launch_bounds__(256) repitch_kernel(const __grid_constant__ Repitch p) {
   grid_order();
-  for (int k = 0; k < p.count; ++k) {
-    const Repitch::Matrix& m = p.m[k];
-    const int64_t total = (int64_t)m.rows * m.groups;
-    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-      const int64_t r = i / m.groups;
-      const int c = (int)(i - r * m.groups) * 8;
-      const uint16_t* src = m.src + r * m.ld + c;
-      uint32_t w[4];
+  const Repitch::Matrix& m = p.m[blockIdx.y];
+  const int64_t total = (int64_t)m.rows * m.groups;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / m.groups;
+    const int c = (int)(i - r * m.groups) * 8;
+    const uint16_t* src = m.src + r * m.ld + c;
+    uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t lo = c + 2 * j < m.cols ? __ldg(src + 2 * j) : 0;
-        const uint32_t hi = c + 2 * j + 1 < m.cols ? __ldg(src + 2 * j + 1) : 0;
-        w[j] = lo | (hi << 16);
-      }
-      *reinterpret_cast<uint4*>(m.dst + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t lo = c + 2 * j < m.cols ? __ldg(src + 2 * j) : 0;
+      const uint32_t hi = c + 2 * j + 1 < m.cols ? __ldg(src + 2 * j + 1) : 0;
+      w[j] = lo | (hi << 16);
     }
+    *reinterpret_cast<uint4*>(m.dst + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -324,7 +322,8 @@ struct Copies {
       if (blocks > most) most = blocks;
     }
     if (most > 8 * 148) most = 8 * 148;
-    return dense_launch(reinterpret_cast<const void*>(&repitch_kernel), dim3((unsigned)most), 0, 256, 0, s, &r, who);
+    return dense_launch(reinterpret_cast<const void*>(&repitch_kernel), dim3((unsigned)most, (unsigned)r.count), 0, 256, 0, s,
+                        &r, who);
   }
 };
 

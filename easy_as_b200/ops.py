@@ -64,7 +64,7 @@ class _Plan:
     buffer have in common once one of them has passed all checks: the argument struct but for its
     pointers, the scratch it needs (buffers on 16-byte boundaries), and the address ranges to keep apart."""
 
-    __slots__ = ("entry", "rest", "device", "nbytes", "apart")
+    __slots__ = ("rest", "device", "nbytes", "apart", "large", "small", "lib", "call", "torch_c")
 
 
 _plans: dict[Any, _Plan] = {}
@@ -76,12 +76,12 @@ def _quick(entry: _Entry, act: str, bufs: tuple[Any, ...], sync: bool) -> Any:
     """Make the call from a plan of an earlier one (True), or return the key under which
     :meth:`_Call.launch` may leave a plan (None when there can be none)."""
     global _torch_types
-    torch = sys.modules.get("torch")
-    if torch is None:
-        return None
-    if not _torch_types:
-        _torch_types = (torch.Tensor, torch.nn.Parameter)
     types = _torch_types
+    if not types:
+        torch = sys.modules.get("torch")
+        if torch is None:
+            return None
+        types = _torch_types = (torch.Tensor, torch.nn.Parameter)
     key: list[Any] = [entry, act]
     for b in bufs:
         if b is None:
@@ -105,32 +105,42 @@ def _quick(entry: _Entry, act: str, bufs: tuple[Any, ...], sync: bool) -> Any:
         if pa < pb + nb and pb < pa + na and not (may_be_one and pa == pb):
             return None   # perhaps an overlap: the full checks tell
     device = plan.device
-    if torch._C._cuda_getDevice() != device:
+    torch_c = plan.torch_c
+    if torch_c._cuda_getDevice() != device or plan.lib is not cuda_ext._lib:
         return None
     rt = get_runtime()
-    stream = torch._C._cuda_getCurrentRawStream(device)
+    stream = torch_c._cuda_getCurrentRawStream(device)
     capturing = rt.check_capture(stream, sync) if stream else False
     if plan.nbytes:
+        torch = sys.modules["torch"]
         ptrs.append(torch.empty(plan.nbytes, dtype=torch.uint8, device=bufs[0].device).data_ptr())
     else:
         ptrs.append(0)
-    rc = getattr(rt.lib(), entry.name)(entry.pointers.pack(*ptrs) + plan.rest, stream)
+    rc = plan.call(entry.pointers.pack(*ptrs) + plan.rest, stream)
     if rc:
         cuda_ext.check(rc, entry.name)
-    if not (sync or capturing):
-        _record(torch, device, stream, bufs)
-    rt.finish_native(device, stream, None, sync, capturing)
+    if sync or capturing:
+        rt.finish_native(device, stream, None, sync, capturing)
+    else:
+        if plan.large:
+            _record(device, stream, [bufs[i] for i in plan.large])
+        rt.finish_native(device, stream, bufs if not plan.large else [bufs[i] for i in plan.small], False)
     return True
 
 
-def _record(torch: Any, device: int, stream: int, bufs: Any) -> None:
-    """Buffers must outlive an asynchronous launch: torch's allocator learns which stream uses them."""
+#: buffers up to this many bytes are kept alive by reference while a call on them is in flight; of larger
+#: ones torch's allocator is told the stream instead (a microsecond each), so that memory its owner has
+#: let go is not held by calls in the queue
+_SMALL = 1 << 18
+
+
+def _record(device: int, stream: int, bufs: Any) -> None:
+    """Tell torch's allocator that ``stream`` uses these tensors."""
     on = _streams.get((device, stream))
     if on is None:
-        on = _streams[(device, stream)] = torch.cuda.current_stream(device)
+        on = _streams[(device, stream)] = sys.modules["torch"].cuda.current_stream(device)
     for b in bufs:
-        if b is not None and type(b) is not Tensor:
-            b.record_stream(on)
+        b.record_stream(on)
 
 
 class _Rows:
@@ -140,6 +150,10 @@ class _Rows:
 
     def __init__(self, ptr: int, rows: int, cols: int, ld: int, lead: tuple[int, ...], keep: Any):
         self.ptr, self.rows, self.cols, self.ld, self.lead, self.keep = ptr, rows, cols, ld, lead, keep
+
+    def span(self) -> int:
+        """Bytes from the first element to the last."""
+        return 2 * ((self.rows - 1) * self.ld + self.cols) if self.rows and self.cols else 0
 
 
 class _Call:
@@ -291,10 +305,12 @@ class _Call:
             cuda_ext.check(getattr(lib, entry.name)(args, stream), self.what)
             keep = None
             if not (sync or capturing):
-                held = [r.keep for r in bufs if r is not None]
-                if torch is not None:
-                    _record(torch, device, stream, held)
-                keep = [b for b in held if type(b) is Tensor]
+                # buffers must outlive an asynchronous launch
+                held = [r for r in bufs if r is not None]
+                large = [r for r in held if type(r.keep) is not Tensor and r.span() > _SMALL]
+                if large:
+                    _record(device, stream, [r.keep for r in large])
+                keep = [r.keep for r in held if all(r is not v for v in large)]
                 if torch is None and owner is not None:
                     keep.append(owner)
             rt.finish_native(device, stream, keep, sync, capturing)
@@ -302,9 +318,6 @@ class _Call:
             self._leave_plan(entry, bufs, rest, nbytes, key)
 
     def _leave_plan(self, entry: _Entry, bufs: tuple[_Rows | None, ...], rest: bytes, nbytes: int, key: Any) -> None:
-        def span(r: _Rows) -> int:
-            return 2 * ((r.rows - 1) * r.ld + r.cols) if r.rows and r.cols else 0
-
         outs = [o for _n, o in self.outs]
         apart = []
         for i, o in enumerate(bufs):
@@ -314,9 +327,13 @@ class _Call:
                 if r is None or r is o or (j > i and any(r is v for v in outs)):
                     continue
                 one = self.in_place is not None and o is self.in_place[0] and r is self.in_place[1]
-                apart.append((i, span(o), j, span(r), one and (o.ld == r.ld or o.rows <= 1)))
+                apart.append((i, o.span(), j, r.span(), one and (o.ld == r.ld or o.rows <= 1)))
         p = _Plan()
-        p.entry, p.rest, p.device, p.nbytes, p.apart = entry, rest, self.device, nbytes, tuple(apart)
+        p.rest, p.device, p.nbytes, p.apart = rest, self.device, nbytes, tuple(apart)
+        p.large = tuple(i for i, r in enumerate(bufs) if r is not None and r.span() > _SMALL)
+        p.small = tuple(i for i, r in enumerate(bufs) if r is not None and r.span() <= _SMALL)
+        p.lib = cuda_ext.load()
+        p.call, p.torch_c = getattr(p.lib, entry.name), self.torch._C
         if len(_plans) >= 1024:
             _plans.clear()
         _plans[key] = p
