@@ -197,16 +197,20 @@ __global__ void __launch_bounds__(256) repitch_kernel(const __grid_constant__ Re
   }
 }
 
-// Rows per block: enough blocks for 8 per SM, at least 8 rows (one per thread row), at most 64 row
-// blocks (whose partial sums are added one after another).
-int rows_per_block(int M, int N) {
-  const int64_t col_blocks = (N + 255) / 256;
+// Rows per block: enough blocks for 8 per SM, at least 8 rows (one per thread row); with sums at most
+// 128 row blocks (whose partial sums are added one after another).
+int rows_per_block(int M, int N, bool sums) {
+  const int64_t col_blocks = ((int64_t)N + 255) / 256;
   int64_t want = (8 * 148 + col_blocks - 1) / col_blocks;
-  if (want > 64) want = 64;
+  if (sums && want > 128) want = 128;
   int64_t rows = ((int64_t)M + want - 1) / want;
   rows = (rows + 7) / 8 * 8;
   return (int)(rows < 8 ? 8 : rows);
 }
+
+// Up to so many rows the products' launch sums the columns of dy itself where dz is dy (32 columns per
+// CTA, beside the tiles); beyond, act_grad_kernel makes partial sums first.
+constexpr uint32_t kDirectRows = 2048;
 
 bool vec_ok(const void* p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld & 7) == 0; }
 
@@ -257,6 +261,7 @@ struct Scratch {
   uint64_t ldk = 0, ldn = 0;  // padded pitches of rows of K and of N elements
   int rows = 0, blocks = 0;
   bool need_dz = false;
+  bool direct = false;  // db straight from dy
 
   Scratch(uint32_t N, uint32_t K) : ldk(((uint64_t)K + 7) / 8 * 8), ldn(((uint64_t)N + 7) / 8 * 8) {}
   uint64_t take(uint64_t bytes) {
@@ -280,12 +285,13 @@ Scratch backward_scratch(bool gated, uint32_t M, uint32_t N, uint32_t K, int act
   if ((outputs & kDw) && (off & kXOff)) s.x = s.take(2 * (uint64_t)M * s.ldk);
   if ((outputs & kDx) && (off & kWOff)) s.w = s.take(2 * (uint64_t)N * s.ldk);
   if (gated && (outputs & kDx) && (off & kUpOff)) s.up = s.take(2 * (uint64_t)N * s.ldk);
-  s.rows = rows_per_block((int)M, (int)N);
+  s.rows = rows_per_block((int)M, (int)N, outputs & kDb);
   s.blocks = (int)(((uint64_t)M + s.rows - 1) / s.rows);
   s.need_dz = (outputs & (kDx | kDw)) && (gated || act != kNone || (off & kDyOff));
   if (s.need_dz) s.dz = s.take(2 * (uint64_t)M * s.ldn);
   if (s.need_dz && gated) s.dz2 = s.take(2 * (uint64_t)M * s.ldn);
-  if (outputs & kDb) s.partial = s.take((uint64_t)s.blocks * N * 4);
+  s.direct = (outputs & kDb) && act == kNone && !s.need_dz && M <= kDirectRows;
+  if ((outputs & kDb) && !s.direct) s.partial = s.take((uint64_t)s.blocks * N * 4);
   return s;
 }
 
@@ -467,8 +473,8 @@ extern "C" int eas_linear_backward(const eas_linear_backward_args* args, void* s
   }
   uint8_t* base = static_cast<uint8_t*>(scratch);
   uint16_t* dz = sc.need_dz ? reinterpret_cast<uint16_t*>(base + sc.dz) : nullptr;
-  float* partial = db ? reinterpret_cast<float*>(base + sc.partial) : nullptr;
-  if (dz || db) {
+  float* partial = db && !sc.direct ? reinterpret_cast<float*>(base + sc.partial) : nullptr;
+  if (dz || partial) {
     ActGrad g = {};
     g.dy = u16(dy), g.g = u16(pre), g.dg = dz, g.partial = partial;
     g.lddy = lddy, g.ldg = ldp, g.ldo = sc.ldn;
@@ -483,7 +489,13 @@ extern "C" int eas_linear_backward(const eas_linear_backward_args* args, void* s
   if ((rc = copies.launch(s, who))) return rc;
   const Operand DZ = dz ? Operand{dz, sc.ldn} : Operand{u16(dy), lddy};
   DenseColSum sums;
-  if (db) sums.partial = partial, sums.db = u16(db), sums.blocks = sc.blocks, sums.N = (int)N, sums.bf16 = dtype == kBF16;
+  if (db) {
+    sums.db = u16(db), sums.N = (int)N, sums.bf16 = dtype == kBF16;
+    if (sc.direct)
+      sums.matrix = u16(dy), sums.ld = (int64_t)lddy, sums.rows = (int)M, sums.vec = vec_ok(dy, lddy);
+    else
+      sums.partial = partial, sums.rows = sc.blocks;
+  }
   if (!dx && !dw) return dense_column_sums(sums, s, who);
   return backward_products(who, 1, {DZ, {}}, {W, {}}, X, dx, lddx, {dw, nullptr}, {lddw, 0}, sums, M, N, K, dtype, s);
 }

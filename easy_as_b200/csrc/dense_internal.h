@@ -28,12 +28,15 @@ struct DenseProduct {
   bool bf16 = false;
 };
 
-// Column sums of `blocks` rows of N partial sums, rounded to the type: db (may be null: none).
+// db[n] = the column sums of `rows` rows of N values, rounded to the type (db null: none wanted): of
+// f32 partial sums, or of a matrix of the type itself.
 struct DenseColSum {
   const float* partial = nullptr;
+  const uint16_t* matrix = nullptr;
+  int64_t ld = 0;  // of the matrix
   uint16_t* db = nullptr;
-  int blocks = 0, N = 0;
-  bool bf16 = false;
+  int rows = 0, N = 0;
+  bool bf16 = false, vec = false;  // vec: rows of the matrix start on 16 bytes
 };
 
 int dense_column_sums(const DenseColSum& sums, cudaStream_t stream, const char* who);

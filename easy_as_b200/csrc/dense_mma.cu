@@ -39,6 +39,7 @@ struct alignas(64) Job {
   int kb_total;        // of all terms
   int mt, nt, tiles;   // tiles along M and N, and in all
   int group;           // M tiles that are walked together
+  int split;           // CTAs of a cluster that share a tile's k-blocks
   bool batch2, y_tma, a_mn;
 };
 
@@ -51,7 +52,9 @@ struct alignas(64) Params {
   uint16_t* pre2_ptr;
   int64_t ldr, ldp, ldp2;
   int tiles;   // of all jobs
-  int split;   // CTAs of a cluster that share a tile's k-blocks
+  int cluster; // CTAs per cluster: the largest split
+  int ctas0;   // CTAs of job 0's tiles, and of all tiles (whole clusters each)
+  int ctas;
   int ratio;   // tiles of job 1 that take as long as one of job 0
   int act;
   bool bf16, pre_tma, pre2_tma, bias_vec, res_vec;
@@ -642,14 +645,57 @@ struct TileShape {
   static_assert(kSmem <= (DEEP ? 232448 : 115000), "shared memory");
 };
 
-// db of 32 columns from n0 on: each row of threads adds every 6th row block, then the rows are added in order.
+// db of 32 columns from n0 on: each row of threads adds every so-manieth row, then the rows of threads
+// are added in order.  `sums`: 48 x 33 floats.
+template <bool BF16>
+__device__ __forceinline__ void column_sums_of_matrix(const DenseColSum& c, int n0, float* sums) {
+  constexpr int kRows = kTileThreads / 4;  // 4 threads of 8 columns per row
+  const int tx = threadIdx.x & 3, ty = threadIdx.x >> 2, n = n0 + 8 * tx;
+  float s[8] = {};
+  if (n < c.N) {
+    const bool whole = c.vec && n + 8 <= c.N;
+#pragma unroll 4
+    for (int r = ty; r < c.rows; r += kRows) {
+      const uint16_t* src = c.matrix + (int64_t)r * c.ld + n;
+      float v[8];
+      if (whole) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(src));
+        unpack2<BF16>(w.x, v[0], v[1]);
+        unpack2<BF16>(w.y, v[2], v[3]);
+        unpack2<BF16>(w.z, v[4], v[5]);
+        unpack2<BF16>(w.w, v[6], v[7]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = n + j < c.N ? to_f32<BF16>(src[j]) : 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += v[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sums[ty * 33 + 8 * tx + j] = s[j];
+  __syncthreads();
+  const int col = threadIdx.x;
+  if (col >= 32 || n0 + col >= c.N) return;
+  float total = 0;
+  for (int r = 0; r < kRows; ++r) total += sums[r * 33 + col];
+  c.db[n0 + col] = to_16<BF16>(total);
+}
+
 __device__ __forceinline__ void column_sums(const DenseColSum& c, int n0, float* sums) {
+  if (c.matrix) {
+    if (c.bf16)
+      column_sums_of_matrix<true>(c, n0, sums);
+    else
+      column_sums_of_matrix<false>(c, n0, sums);
+    return;
+  }
   constexpr int kRows = kTileThreads / 32;
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, n = n0 + tx;
   float s = 0;
   if (n < c.N) {
 #pragma unroll 8
-    for (int b = ty; b < c.blocks; b += kRows) s += c.partial[(int64_t)b * c.N + n];
+    for (int b = ty; b < c.rows; b += kRows) s += c.partial[(int64_t)b * c.N + n];
   }
   sums[ty * 32 + tx] = s;
   __syncthreads();
@@ -660,7 +706,7 @@ __device__ __forceinline__ void column_sums(const DenseColSum& c, int n0, float*
 }
 
 __global__ void __launch_bounds__(kTileThreads) column_sums_kernel(const __grid_constant__ DenseColSum c) {
-  __shared__ float sums[kTileThreads];
+  __shared__ float sums[48 * 33];
   grid_order();
   column_sums(c, blockIdx.x * 32, sums);
 }
@@ -678,14 +724,30 @@ __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);  // uniform
   const int lane = threadIdx.x & 31;
-  const int S = p.split;
-  if (MODE == kBackward && (int)blockIdx.x >= p.tiles * S) {  // CTAs behind the tiles': column sums
+  if (MODE == kBackward && (int)blockIdx.x >= p.ctas) {  // CTAs behind the tiles': column sums
     grid_order();
-    column_sums(p.sums, ((int)blockIdx.x - p.tiles * S) * 32, reinterpret_cast<float*>(smem));
+    column_sums(p.sums, ((int)blockIdx.x - p.ctas) * 32, reinterpret_cast<float*>(smem));
     return;
   }
-  const int rank = (int)blockIdx.x % S;  // consecutive blocks form a cluster
+  const int second = MODE == kBackward && (int)blockIdx.x >= p.ctas0 ? 1 : 0;
+  const int block = (int)blockIdx.x - second * p.ctas0;
+  const int S = p.job[second].split;
+  const int rank = block % S;  // consecutive blocks form a cluster, and share tiles by S
+  if (MODE == kBackward && block / S >= p.job[second].tiles) {  // fills up the job's last cluster (S = 1)
+    grid_order();
+    return;
+  }
 
+  constexpr int kTileN = GATED ? BN / 2 : BN;
+  const Tile c = tile_at<MODE>(p, second * p.job[0].tiles + block / S);
+  const Job& jb = p.job[c.j];
+  const bool a_mn = MODE == kBackward && jb.a_mn;  // (only with AR = 128: it comes in 64-wide pieces of all rows)
+
+  if (threadIdx.x == 32) {
+    prefetch_map(&jb.a[jb.batch2 ? c.z : 0]);
+    prefetch_map(&jb.b[0]);
+    if (GATED) prefetch_map(&jb.b[1]);
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::kStages; ++s) {
       mbar_init(&full[s], 1);
@@ -707,10 +769,6 @@ __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   grid_order();
 
-  constexpr int kTileN = GATED ? BN / 2 : BN;
-  const Tile c = tile_at<MODE>(p, (int)blockIdx.x / S);
-  const Job& jb = p.job[c.j];
-  const bool a_mn = MODE == kBackward && jb.a_mn;  // (only with AR = 128: it comes in 64-wide pieces of all rows)
   const int m0 = c.m * 128, n0 = c.n * kTileN;
   const int kb_lo = (int)((int64_t)rank * jb.kb_total / S), kb_hi = (int)((int64_t)(rank + 1) * jb.kb_total / S);
 
@@ -946,8 +1004,10 @@ int launch_pair(Params& q, int dev, cudaStream_t s, const char* who) {
 
 template <int BN, int AR, bool DEEP, int MODE>
 int launch_tile(Params& q, int dev, cudaStream_t s, const char* who) {
-  // whole clusters of column-sum CTAs
-  const int sums = q.sums.db ? ((q.sums.N + 31) / 32 + q.split - 1) / q.split * q.split : 0;
+  auto whole = [&](int ctas) { return (ctas + q.cluster - 1) / q.cluster * q.cluster; };
+  q.ctas0 = whole(q.job[0].tiles * q.job[0].split);
+  q.ctas = q.ctas0 + whole(q.job[1].tiles * q.job[1].split);
+  const int sums = q.sums.db ? whole((q.sums.N + 31) / 32) : 0;
   static bool ready[64] = {false};
   using L = TileShape<BN, AR, DEEP>;
   const void* kernel = reinterpret_cast<const void*>(&dense_tile_kernel<BN, AR, DEEP, MODE>);
@@ -958,13 +1018,13 @@ int launch_tile(Params& q, int dev, cudaStream_t s, const char* who) {
     if (rc) return rc;
     ready[slot] = true;
   }
-  return dense_launch(kernel, dim3((unsigned)(q.tiles * q.split + sums)), q.split > 1 ? q.split : 0, kTileThreads, L::kSmem, s, &q,
+  return dense_launch(kernel, dim3((unsigned)(q.ctas + sums)), q.cluster > 1 ? q.cluster : 0, kTileThreads, L::kSmem, s, &q,
                       who);
 }
 
 struct Choice {
-  int bn;     // 0: the pair kernel, else the single-CTA kernel's tile width
-  int split;  // CTAs that share a tile's k-blocks
+  int bn;        // 0: the pair kernel, else the single-CTA kernel's tile width
+  int split[2];  // CTAs that share a tile's k-blocks, by job
   int ar;     // rows of A staged
   bool deep;  // one CTA per SM
 };
@@ -978,14 +1038,14 @@ struct Choice {
 //                          (2048^3: 25.1 BN 64, 17.5 BN 128)
 //   a split over 2 or 4    2 or 2.8 more for the exchange, and only while all CTAs are resident at
 //                          once (16 x 4096 x 4096, BN 64: 11.9 whole, 10.2 split in 2, 17.9 in 8)
-Choice choose(const DenseProduct* p, int count, int sms) {
+//   column sums            3 more with the pair kernel, which leaves them to a launch of their own
+Choice choose(const DenseProduct* p, int count, bool sums, int sms) {
   const int pairs = sms / 2 > 0 ? sms / 2 : 1;
-  int64_t kb[2], most_kb = 0, least_kb = INT64_MAX;
+  int64_t kb[2] = {0, 0}, least_kb = INT64_MAX;
   int most_rows = 0;
   bool a_mn = false;
   for (int i = 0; i < count; ++i) {
     kb[i] = (int64_t)((p[i].K + kBK - 1) / kBK) * p[i].terms;
-    most_kb = kb[i] > most_kb ? kb[i] : most_kb;
     least_kb = kb[i] < least_kb ? kb[i] : least_kb;
     most_rows = p[i].M > most_rows ? p[i].M : most_rows;
     a_mn |= p[i].a_mn;
@@ -994,39 +1054,49 @@ Choice choose(const DenseProduct* p, int count, int sms) {
     const int n = p[i].gated ? width / 2 : width;
     return (int64_t)((p[i].M + (int64_t)m - 1) / m) * ((p[i].N + (int64_t)n - 1) / n) * p[i].batch;
   };
-  Choice best = {0, 1, 128, false};
+  Choice best = {0, {1, 1}, 128, false};
   double best_us;
   if (count == 1) {
     best_us = 5.5 + (double)((tiles_of(0, 256, 256) + pairs - 1) / pairs) * kb[0] * 0.31;
-  } else {  // the jobs fill one another's last rounds
+  } else {  // the jobs (the longer tiles first) fill one another's last rounds
     double steps = 0;
-    for (int i = 0; i < count; ++i) steps += (double)tiles_of(i, 256, 256) * kb[i];
-    steps = steps / pairs + 0.5 * least_kb;
-    best_us = 5.5 + (steps > most_kb ? steps : most_kb) * 0.31;
-  }
-  for (int bn = 64; bn <= 128; bn += 64) {
     int64_t tiles = 0;
+    for (int i = 0; i < count; ++i) {
+      tiles += tiles_of(i, 256, 256);
+      steps += (double)tiles_of(i, 256, 256) * kb[i];
+    }
+    steps = tiles <= pairs ? kb[0] : steps / pairs + 0.5 * least_kb;
+    best_us = 5.5 + (steps > kb[0] ? steps : kb[0]) * 0.31;
+  }
+  if (sums) best_us += 3;
+  const int64_t most_split = (int64_t)sms * 7 / 8;
+  for (int bn = 64; bn <= 128; bn += 64) {
+    int64_t tiles[2] = {0, 0};
     double work = 0;  // steps of all tiles, with what a tile costs beside its steps
     const double shared = bn == 64 ? 0.2 : 0.26, tile_us = bn == 64 ? 0.6 : 0.9;
     for (int i = 0; i < count; ++i) {
-      const int64_t n = tiles_of(i, 128, bn);
-      tiles += n;
-      work += (double)n * (kb[i] * shared + tile_us);
+      tiles[i] = tiles_of(i, 128, bn);
+      work += (double)tiles[i] * (kb[i] * shared + tile_us);
     }
-    for (int split = 1; split <= 4; split *= 2) {
-      const int64_t ctas = tiles * split;
-      if (split > 1 && (ctas > sms * 7 / 8 || least_kb < 2 * split)) break;
-      Choice c = {bn, split, 128, ctas <= sms};
-      double us;
-      if (c.deep) {
-        if (most_rows <= 64 && !a_mn) c.ar = 64;
-        const double step = bn == 64 ? (c.ar == 64 ? 0.115 : 0.15) : (c.ar == 64 ? 0.155 : 0.205);
-        us = 4.5 + (double)((most_kb + split - 1) / split) * step + (split == 1 ? 0 : split == 2 ? 2 : 2.8);
-      } else {
-        const double two = 1.8 * (most_kb * shared + tile_us);  // some SM has two tiles
-        us = 4.0 + (work / sms > two ? work / sms : two);
+    const bool few = most_rows <= 64 && !a_mn;
+    const double step = bn == 64 ? (few ? 0.115 : 0.15) : (few ? 0.155 : 0.205);
+    for (int s0 = 1; s0 <= 4; s0 *= 2) {
+      for (int s1 = 1; s1 <= (count > 1 ? s0 : 1); s1 *= 2) {
+        const int64_t ctas = tiles[0] * s0 + tiles[1] * s1;
+        if (s0 > 1 && (ctas > most_split || kb[0] < 2 * s0 || (s1 > 1 && kb[1] < 2 * s1))) continue;
+        Choice c = {bn, {s0, s1}, 128, ctas <= sms};
+        double us;
+        if (c.deep) {
+          if (few) c.ar = 64;
+          const double t0 = (double)((kb[0] + s0 - 1) / s0) * step + (s0 == 1 ? 0 : s0 == 2 ? 2 : 2.8);
+          const double t1 = (double)((kb[1] + s1 - 1) / s1) * step + (s1 == 1 ? 0 : s1 == 2 ? 2 : 2.8);
+          us = 4.5 + (t0 > t1 ? t0 : t1);
+        } else {
+          const double two = 1.8 * (kb[0] * shared + tile_us);  // some SM has two tiles
+          us = 4.0 + (work / sms > two ? work / sms : two);
+        }
+        if (us < best_us) best = c, best_us = us;
       }
-      if (us < best_us) best = c, best_us = us;
     }
   }
   return best;
@@ -1068,7 +1138,7 @@ int dense_mma(const DenseProduct* p, int count, const DenseColSum& sums, cudaStr
   }
   for (int i = 0; i < count; ++i)
     if (steps(order[i]) > 0x7fffffff) return eas_fail(EAS_ERR_VALUE, "%s: too many products in a sum", who);
-  const Choice c = choose(order, count, dense_sms(dev));
+  const Choice c = choose(order, count, sums.db != nullptr, dense_sms(dev));
   const bool gated = p[0].gated;
   const int width = c.bn ? c.bn : 256;  // of the accumulator: a gated tile has half as many outputs
   const int b_rows = !c.bn ? 128 : (gated ? c.bn / 2 : c.bn);
@@ -1076,10 +1146,12 @@ int dense_mma(const DenseProduct* p, int count, const DenseColSum& sums, cudaStr
   for (int i = 0; i < count; ++i) {
     rc = fill_job(q.job[i], order[i], c.ar, b_rows, c.bn ? 128 : 256, gated ? width / 2 : width, who);
     if (rc) return rc;
+    q.job[i].split = c.split[i];
     q.tiles += q.job[i].tiles;
   }
   if (count > 1) q.ratio = (q.job[0].kb_total + q.job[1].kb_total / 2) / q.job[1].kb_total;
-  q.split = c.split;
+  q.cluster = c.split[0] > c.split[1] ? c.split[0] : c.split[1];
+  if (count == 1) q.job[1].split = 1;
   q.bf16 = p[0].bf16;
   q.sums = sums;
   q.status = eas_native_status_dev(dev);
