@@ -376,6 +376,43 @@ extern "C" int eas_dense_scratch(int op, uint32_t M, uint32_t N, uint32_t K, int
   return EAS_OK;
 }
 
+extern "C" int eas_dense_plan(int op, uint32_t M, uint32_t N, uint32_t K, int outputs, int num_sms, int* kernel,
+                              int* width, int* split0, int* split1, int* a_rows, int* ctas_per_sm) {
+  if (!kernel || !width || !split0 || !split1 || !a_rows || !ctas_per_sm)
+    return eas_fail(EAS_ERR_VALUE, "eas_dense_plan: null pointer");
+  if (op < 0 || op > 3) return eas_fail(EAS_ERR_VALUE, "eas_dense_plan: op must be 0..3");
+  int rc = check_sizes("eas_dense_plan", M, N, K, kF16, kNone);
+  if (rc) return rc;
+  if (M == 0 || num_sms <= 0 || (op >= 2 && !(outputs & (kDx | kDw))))
+    return eas_fail(EAS_ERR_VALUE, "eas_dense_plan: no product");
+  const bool gated = op & 1;
+  DenseProduct p[2];
+  int count = 1;
+  if (op < 2) {
+    p[0].gated = gated;
+    p[0].M = (int)M, p[0].N = (int)N, p[0].K = (int)K;
+    if (dense_rows_fit((int)M, (int)K)) {
+      *kernel = 0, *width = gated ? 8 : 16, *split0 = dense_rows_split(p[0], num_sms), *split1 = 1;
+      *a_rows = kDenseRows, *ctas_per_sm = 2;
+      return EAS_OK;
+    }
+  } else {
+    count = 0;
+    if (outputs & kDx) {
+      DenseProduct& d = p[count++];
+      d.M = (int)M, d.N = (int)K, d.K = (int)N, d.terms = gated ? 2 : 1, d.b_mn = true;
+    }
+    if (outputs & kDw) {
+      DenseProduct& d = p[count++];
+      d.M = (int)N, d.N = (int)K, d.K = (int)M, d.batch = gated ? 2 : 1, d.a_mn = d.b_mn = true;
+    }
+  }
+  const DenseShape s = dense_shape(p, count, outputs & kDb, num_sms);
+  *kernel = s.bn ? 1 : 2, *width = s.bn ? s.bn : 256, *split0 = s.split[0], *split1 = s.split[1];
+  *a_rows = s.ar, *ctas_per_sm = s.bn && !s.deep ? 2 : 1;
+  return EAS_OK;
+}
+
 extern "C" int eas_linear(const eas_linear_args* args, void* stream) {
   const char* who = "eas_linear";
   if (!args) return eas_fail(EAS_ERR_VALUE, "%s: null arguments", who);

@@ -44,8 +44,18 @@ int dense_column_sums(const DenseColSum& sums, cudaStream_t stream, const char* 
 // One forward product, or one or two backward ones (with column sums) that do not depend on one another.
 int dense_mma(const DenseProduct* p, int count, const DenseColSum& sums, cudaStream_t stream, const char* who);
 
+// The shape of kernel that dense_mma runs such products on.
+struct DenseShape {
+  int bn;        // 0: the pair kernel, else the single-CTA kernel's tile width
+  int split[2];  // CTAs that share a tile's k-blocks, by product (the one of the longer sums first)
+  int ar;        // rows of A staged
+  bool deep;     // one CTA per SM
+};
+DenseShape dense_shape(const DenseProduct* p, int count, bool sums, int sms);
+
 // The same for the forward products (K-major operands, one term, one product) of at most kDenseRows
 // rows that fit in shared memory; operands of any alignment.
 constexpr int kDenseRows = 8;
 bool dense_rows_fit(int M, int K);
+int dense_rows_split(const DenseProduct& p, int sms);
 int dense_rows(const DenseProduct& p, cudaStream_t stream, const char* who);

@@ -733,8 +733,12 @@ __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(
   const int block = (int)blockIdx.x - second * p.ctas0;
   const int S = p.job[second].split;
   const int rank = block % S;  // consecutive blocks form a cluster, and share tiles by S
-  if (MODE == kBackward && block / S >= p.job[second].tiles) {  // fills up the job's last cluster (S = 1)
+  if (MODE == kBackward && block / S >= p.job[second].tiles) {  // fills up the job's last cluster
     grid_order();
+    if (S > 1) {  // the barriers of the CTAs that work
+      cluster_sync_all();
+      cluster_sync_all();
+    }
     return;
   }
 
@@ -868,6 +872,10 @@ __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(
     if (warp >= 2) {
       const int e = warp - 2;
       Boxes bx = {smem + L::kBoxes + e * 2 * kBoxBytes, 0};
+      // the S CTAs of this tile are neighbours in the cluster, which may hold several tiles
+      uint32_t first;
+      asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(first));
+      first -= (uint32_t)rank;
       const int quarters = min(4, (jb.M - m0 + 31) / 32);
       const int pieces = min(kTileN, jb.N - n0 + 31) / 32 * quarters;
       for (int i = rank + e * S; i < pieces; i += 4 * S) {
@@ -881,7 +889,7 @@ __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(
           for (int j = 0; j < 32; ++j) u[j] = 0;
         }
         for (int s = 0; s < S; ++s) {
-          const uint32_t from = mapa_rank(at, (uint32_t)s);
+          const uint32_t from = mapa_rank(at, first + (uint32_t)s);
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] += ld_cluster_f32(from + j * 512);
           if constexpr (GATED) {
@@ -1022,12 +1030,7 @@ int launch_tile(Params& q, int dev, cudaStream_t s, const char* who) {
                       who);
 }
 
-struct Choice {
-  int bn;        // 0: the pair kernel, else the single-CTA kernel's tile width
-  int split[2];  // CTAs that share a tile's k-blocks, by job
-  int ar;     // rows of A staged
-  bool deep;  // one CTA per SM
-};
+using Choice = DenseShape;
 
 // The shape of least estimated time, in microseconds as measured on one B200 at 1.9 GHz (bf16,
 // operands from HBM).  A step is one 64-deep k-block of one CTA or pair.
@@ -1118,7 +1121,21 @@ int launch_choice(const Choice& c, Params& q, int dev, cudaStream_t s, const cha
   return c.deep ? launch_tile<128, 128, true, MODE>(q, dev, s, who) : launch_tile<128, 128, false, MODE>(q, dev, s, who);
 }
 
+int64_t steps_of(const DenseProduct& p) { return (int64_t)((p.K + kBK - 1) / kBK) * p.terms; }
+
+void longer_first(const DenseProduct* p, int count, DenseProduct (&order)[2]) {
+  const bool swap = count > 1 && steps_of(p[0]) < steps_of(p[1]);
+  order[0] = p[swap ? 1 : 0];
+  order[1] = p[count > 1 && !swap ? 1 : 0];
+}
+
 }  // namespace
+
+DenseShape dense_shape(const DenseProduct* p, int count, bool sums, int sms) {
+  DenseProduct order[2];
+  longer_first(p, count, order);
+  return choose(order, count, sums, sms);
+}
 
 int dense_column_sums(const DenseColSum& sums, cudaStream_t stream, const char* who) {
   DenseColSum c = sums;
@@ -1130,14 +1147,10 @@ int dense_mma(const DenseProduct* p, int count, const DenseColSum& sums, cudaStr
   int dev = 0;
   int rc = eas_cuda_check(cudaGetDevice(&dev), who, EAS_ERR_UNAVAILABLE);
   if (rc) return rc;
-  DenseProduct order[2] = {p[0], count > 1 ? p[1] : p[0]};
-  auto steps = [](const DenseProduct& v) { return (int64_t)((v.K + kBK - 1) / kBK) * v.terms; };
-  if (count > 1 && steps(order[0]) < steps(order[1])) {  // the longer tiles first
-    order[0] = p[1];
-    order[1] = p[0];
-  }
+  DenseProduct order[2];
+  longer_first(p, count, order);
   for (int i = 0; i < count; ++i)
-    if (steps(order[i]) > 0x7fffffff) return eas_fail(EAS_ERR_VALUE, "%s: too many products in a sum", who);
+    if (steps_of(order[i]) > 0x7fffffff) return eas_fail(EAS_ERR_VALUE, "%s: too many products in a sum", who);
   const Choice c = choose(order, count, sums.db != nullptr, dense_sms(dev));
   const bool gated = p[0].gated;
   const int width = c.bn ? c.bn : 256;  // of the accumulator: a gated tile has half as many outputs

@@ -316,6 +316,11 @@ int launch_rows(const DenseProduct& p, RowsParams& q, bool vec, int dev, cudaStr
 
 }  // namespace
 
+int dense_rows_split(const DenseProduct& p, int sms) {
+  const int warps = p.M * x_pitch(p.K) <= Shape<8>::kMostX ? 8 : 16;
+  return choose_split(p, 16 / warps * sms, warps);
+}
+
 bool dense_rows_fit(int M, int K) { return M <= kDenseRows && M * x_pitch(K) <= Shape<16>::kMostX; }
 
 int dense_rows(const DenseProduct& p, cudaStream_t stream, const char* who) {

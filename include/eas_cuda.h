@@ -406,6 +406,14 @@ int eas_gated_backward(const eas_gated_backward_args* args, void* stream);
 int eas_dense_scratch(int op, uint32_t M, uint32_t N, uint32_t K, int act, int outputs, int unaligned,
                       uint64_t* bytes);
 
+/* The kernel that a call's products run on, without a device (reporting and
+ * tests): *kernel 0 is the one for few rows, 1 the single-CTA tiles of 128 x
+ * *width sums, 2 the CTA pairs (*width 256); *split0 and *split1 CTAs share the
+ * sum of one tile (of the first and second product), *a_rows rows of the first
+ * operand are staged, *ctas_per_sm is 1 or 2.  op and outputs as above. */
+int eas_dense_plan(int op, uint32_t M, uint32_t N, uint32_t K, int outputs, int num_sms, int* kernel, int* width,
+                   int* split0, int* split1, int* a_rows, int* ctas_per_sm);
+
 /* ---- host-side fault injection (tests; no device fault is ever made; no
  *      counterpart in the reference) ---------------------------------------- */
 

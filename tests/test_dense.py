@@ -214,6 +214,31 @@ def test_c_entries_want_their_scratch(name):
         assert "scratch" in cuda_ext.last_error()
 
 
+def test_gpu_tests_reach_every_kernel():
+    """The sizes of the exact GPU tests run every kernel that any call can reach (each is instantiated for some)."""
+    import random
+
+    import dense_shapes as ds
+
+    covered = set().union(*(ds.kernels(s) for s in ds.SHAPES + ds.BIG + ds.VARIANTS))
+    rng = random.Random(0)
+    for _ in range(6000):
+        shape = tuple(int(2 ** rng.uniform(0, 13.5)) for _ in range(3))
+        missing = ds.kernels(shape) - covered
+        assert not missing, (shape, missing)
+    assert {k[1] for k in covered} == {0, 1, 2}
+
+
+def test_plan_checks_its_arguments():
+    import dense_shapes as ds
+
+    assert ds.plan(ds.LINEAR, 1, 4096, 4096)[0] == 0
+    assert ds.plan(ds.LINEAR, 8192, 8192, 8192)[0] == 2
+    for bad in ((4, 1, 1, 1, 0), (2, 1, 1, 1, 0), (2, 1, 1, 1, 4), (0, 0, 1, 1, 0), (0, 1, 0, 1, 0)):
+        with pytest.raises(ValueError):
+            ds.plan(*bad)
+
+
 def test_scratch_query_checks_its_arguments():
     lib = cuda_ext.load()
     need = ctypes.c_uint64(5)
