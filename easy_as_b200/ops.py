@@ -59,88 +59,49 @@ _E_LINEAR_BACKWARD = _Entry(_LINEAR_BACKWARD, "eas_linear_backward", 7, 6)
 _E_GATED_BACKWARD = _Entry(_GATED_BACKWARD, "eas_gated_backward", 9, 9)
 
 
-class _Plan:
-    """What calls with the same operator, activation and shapes, strides, dtypes and devices of every
-    buffer have in common once one of them has passed all checks: the argument struct but for its
-    pointers, the scratch it needs (buffers on 16-byte boundaries), and the address ranges to keep apart."""
-
-    __slots__ = ("rest", "device", "nbytes", "apart", "large", "small", "lib", "call", "torch_c")
+# The extension that repeats a checked call (csrc/ops_torch.cpp), loaded with the first torch tensor:
+# None before, False where it is not built for this torch (every call then takes the full path).
+_ext: Any = None
+_ext_lib: Any = None
 
 
-_plans: dict[Any, _Plan] = {}
-_torch_types: tuple[Any, ...] = ()
-_streams: dict[tuple[int, int], Any] = {}
+def _load_ext() -> Any:
+    global _ext, _ext_lib
+    import importlib.machinery
+    import importlib.util
+
+    from . import build
+
+    _ext = False
+    try:
+        if build.OPS_STAMP.read_text().strip() == build.ops_hash():
+            loader = importlib.machinery.ExtensionFileLoader("eas_ops", str(build.OPS))
+            mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("eas_ops", loader))
+            loader.exec_module(mod)
+            lib = cuda_ext.load()
+            mod.init(sys.modules["torch"].nn.Parameter, _address(lib.eas_stream_is_capturing))
+            _ext, _ext_lib = mod, lib
+    except (OSError, ImportError):
+        pass
+    return _ext
 
 
-def _quick(entry: _Entry, act: str, bufs: tuple[Any, ...], sync: bool) -> Any:
-    """Make the call from a plan of an earlier one (True), or return the key under which
-    :meth:`_Call.launch` may leave a plan (None when there can be none)."""
-    global _torch_types
-    types = _torch_types
-    if not types:
-        torch = sys.modules.get("torch")
-        if torch is None:
-            return None
-        types = _torch_types = (torch.Tensor, torch.nn.Parameter)
-    key: list[Any] = [entry, act]
-    for b in bufs:
-        if b is None:
-            key.append(None)
-        elif type(b) in types:
-            key += (b.shape, b.stride(), b.dtype, b.get_device())
-        else:
-            return None
-    k = tuple(key)
-    plan = _plans.get(k)
-    if plan is None or sync.__class__ is not bool:
-        return k
-    ptrs = [0 if b is None else b.data_ptr() for b in bufs]
-    any_ptr = 0
-    for q in ptrs:
-        any_ptr |= q
-    if any_ptr & 15:
-        return None
-    for a, na, b, nb, may_be_one in plan.apart:
-        pa, pb = ptrs[a], ptrs[b]
-        if pa < pb + nb and pb < pa + na and not (may_be_one and pa == pb):
-            return None   # perhaps an overlap: the full checks tell
-    device = plan.device
-    torch_c = plan.torch_c
-    if torch_c._cuda_getDevice() != device or plan.lib is not cuda_ext._lib:
-        return None
-    rt = get_runtime()
-    stream = torch_c._cuda_getCurrentRawStream(device)
-    capturing = rt.check_capture(stream, sync) if stream else False
-    if plan.nbytes:
-        torch = sys.modules["torch"]
-        ptrs.append(torch.empty(plan.nbytes, dtype=torch.uint8, device=bufs[0].device).data_ptr())
-    else:
-        ptrs.append(0)
-    rc = plan.call(entry.pointers.pack(*ptrs) + plan.rest, stream)
+def _address(fn: Any) -> int:
+    return int(ctypes.cast(fn, ctypes.c_void_p).value or 0)
+
+
+def _quick(entry: _Entry, act: str, bufs: tuple[Any, ...], sync: bool) -> bool:
+    """Make the call from the plan of an earlier one, if there is one for these buffers."""
+    if not _ext or _ext_lib is not cuda_ext._lib:
+        return False
+    r = _ext.quick(entry.op, _ACT.get(act, -1), bufs, sync)
+    if r is None:
+        return False
+    rc, device, stream, capturing = r
     if rc:
         cuda_ext.check(rc, entry.name)
-    if sync or capturing:
-        rt.finish_native(device, stream, None, sync, capturing)
-    else:
-        if plan.large:
-            _record(device, stream, [bufs[i] for i in plan.large])
-        rt.finish_native(device, stream, bufs if not plan.large else [bufs[i] for i in plan.small], False)
+    get_runtime().finish_native(device, stream, None, sync, capturing)
     return True
-
-
-#: buffers up to this many bytes are kept alive by reference while a call on them is in flight; of larger
-#: ones torch's allocator is told the stream instead (a microsecond each), so that memory its owner has
-#: let go is not held by calls in the queue
-_SMALL = 1 << 18
-
-
-def _record(device: int, stream: int, bufs: Any) -> None:
-    """Tell torch's allocator that ``stream`` uses these tensors."""
-    on = _streams.get((device, stream))
-    if on is None:
-        on = _streams[(device, stream)] = sys.modules["torch"].cuda.current_stream(device)
-    for b in bufs:
-        b.record_stream(on)
 
 
 class _Rows:
@@ -283,7 +244,7 @@ class _Call:
                     raise ValueError(f"{self.what}: {name!r} overlaps another output")
 
     def launch(self, entry: _Entry, bufs: tuple[_Rows | None, ...], pitched: tuple[_Rows | None, ...],
-               sizes: tuple[int, int, int], act: int, outputs: int, off: int, sync: bool, key: Any) -> None:
+               sizes: tuple[int, int, int], act: int, outputs: int, off: int, sync: bool, given: tuple[Any, ...]) -> None:
         rt = get_runtime()
         device = self.device
         torch = self.torch
@@ -305,19 +266,24 @@ class _Call:
             cuda_ext.check(getattr(lib, entry.name)(args, stream), self.what)
             keep = None
             if not (sync or capturing):
-                # buffers must outlive an asynchronous launch
-                held = [r for r in bufs if r is not None]
-                large = [r for r in held if type(r.keep) is not Tensor and r.span() > _SMALL]
-                if large:
-                    _record(device, stream, [r.keep for r in large])
-                keep = [r.keep for r in held if all(r is not v for v in large)]
-                if torch is None and owner is not None:
+                # buffers must outlive an asynchronous launch: torch's allocator learns which stream uses
+                # them (its scratch is that stream's already), the others are kept until it is done
+                held = [r.keep for r in bufs if r is not None]
+                keep = [b for b in held if type(b) is Tensor]
+                if torch is not None:
+                    on = torch.cuda.current_stream(device)
+                    for b in held:
+                        if type(b) is not Tensor:
+                            b.record_stream(on)
+                elif owner is not None:
                     keep.append(owner)
             rt.finish_native(device, stream, keep, sync, capturing)
-        if key is not None and not self.copied:
-            self._leave_plan(entry, bufs, rest, nbytes, key)
+        if torch is not None and not self.copied and _ext is not False and (_ext or _load_ext()):
+            self._leave_plan(entry, bufs, given, act, rest, nbytes)
 
-    def _leave_plan(self, entry: _Entry, bufs: tuple[_Rows | None, ...], rest: bytes, nbytes: int, key: Any) -> None:
+    def _leave_plan(self, entry: _Entry, bufs: tuple[_Rows | None, ...], given: tuple[Any, ...], act: int, rest: bytes,
+                    nbytes: int) -> None:
+        """Let the extension repeat this call (``given``: the buffers as they came)."""
         outs = [o for _n, o in self.outs]
         apart = []
         for i, o in enumerate(bufs):
@@ -328,15 +294,7 @@ class _Call:
                     continue
                 one = self.in_place is not None and o is self.in_place[0] and r is self.in_place[1]
                 apart.append((i, o.span(), j, r.span(), one and (o.ld == r.ld or o.rows <= 1)))
-        p = _Plan()
-        p.rest, p.device, p.nbytes, p.apart = rest, self.device, nbytes, tuple(apart)
-        p.large = tuple(i for i, r in enumerate(bufs) if r is not None and r.span() > _SMALL)
-        p.small = tuple(i for i, r in enumerate(bufs) if r is not None and r.span() <= _SMALL)
-        p.lib = cuda_ext.load()
-        p.call, p.torch_c = getattr(p.lib, entry.name), self.torch._C
-        if len(_plans) >= 1024:
-            _plans.clear()
-        _plans[key] = p
+        _ext.leave(entry.op, act, given, _address(getattr(_ext_lib, entry.name)), rest, self.device, nbytes, tuple(apart))
 
 
 def _share(a: _Rows, b: _Rows) -> bool:
@@ -379,8 +337,8 @@ def linear(x: Any, w: Any, y: Any, *, bias: Any = None, residual: Any = None, ac
     ``pre [..., N]``, if given, receives ``x W^T + bias``, which :func:`linear_backward` needs when
     there is an activation.  ``y`` may be ``residual`` itself.
     """
-    key = _quick(_E_LINEAR, act, (x, w, bias, residual, y, pre), _sync)
-    if key is True:
+    given = (x, w, bias, residual, y, pre)
+    if _quick(_E_LINEAR, act, given, _sync):
         return
     what = "linear"
     code, sync = _activation(what, act), _flag(_sync)
@@ -406,7 +364,7 @@ def linear(x: Any, w: Any, y: Any, *, bias: Any = None, residual: Any = None, ac
     if R is not None:
         c.in_place = (Y, R)
     c.no_overlap()
-    c.launch(_E_LINEAR, (X, W, B, R, Y, P), (X, W, R, Y, P), (X.rows, n, k), code, 0, _off(X, 1) | _off(W, 2), sync, key)
+    c.launch(_E_LINEAR, (X, W, B, R, Y, P), (X, W, R, Y, P), (X.rows, n, k), code, 0, _off(X, 1) | _off(W, 2), sync, given)
 
 
 def gated(x: Any, w_gate: Any, w_up: Any, h: Any, *, act: str = "silu", gate: Any = None, up: Any = None,
@@ -416,8 +374,8 @@ def gated(x: Any, w_gate: Any, w_up: Any, h: Any, *, act: str = "silu", gate: An
     ``gate`` and ``up [..., N]``, if given (both or neither), receive the two products, which
     :func:`gated_backward` needs.
     """
-    key = _quick(_E_GATED, act, (x, w_gate, w_up, h, gate, up), _sync)
-    if key is True:
+    given = (x, w_gate, w_up, h, gate, up)
+    if _quick(_E_GATED, act, given, _sync):
         return
     what = "gated"
     code, sync = _activation(what, act), _flag(_sync)
@@ -440,7 +398,7 @@ def gated(x: Any, w_gate: Any, w_up: Any, h: Any, *, act: str = "silu", gate: An
         return
     c.no_overlap()
     c.launch(_E_GATED, (X, G, U, H, SG, SU), (X, G, U, H, SG, SU), (X.rows, n, k), code, 0,
-             _off(X, 1) | _off(G, 2) | _off(U, 4), sync, key)
+             _off(X, 1) | _off(G, 2) | _off(U, 4), sync, given)
 
 
 def linear_backward(dy: Any, x: Any, w: Any, *, dx: Any = None, dw: Any = None, dbias: Any = None, act: str = "none",
@@ -451,8 +409,8 @@ def linear_backward(dy: Any, x: Any, w: Any, *, dx: Any = None, dw: Any = None, 
     ``pre`` is what :func:`linear` stored there (not needed for ``act="none"``).  The gradient of
     the residual is ``dy`` itself.
     """
-    key = _quick(_E_LINEAR_BACKWARD, act, (dy, pre, x, w, dx, dw, dbias), _sync)
-    if key is True:
+    given = (dy, pre, x, w, dx, dw, dbias)
+    if _quick(_E_LINEAR_BACKWARD, act, given, _sync):
         return
     what = "linear_backward"
     code, sync = _activation(what, act), _flag(_sync)
@@ -486,7 +444,7 @@ def linear_backward(dy: Any, x: Any, w: Any, *, dx: Any = None, dw: Any = None, 
         return
     c.no_overlap()
     c.launch(_E_LINEAR_BACKWARD, (DY, P, X, W, DX, DW, DB), (DY, P, X, W, DX, DW), (X.rows, n, k), code, outputs,
-             _off(X, 1) | _off(W, 2) | _off(DY, 8), sync, key)
+             _off(X, 1) | _off(W, 2) | _off(DY, 8), sync, given)
 
 
 def gated_backward(dh: Any, x: Any, w_gate: Any, w_up: Any, gate: Any, up: Any, *, dx: Any = None,
@@ -496,8 +454,8 @@ def gated_backward(dh: Any, x: Any, w_gate: Any, w_up: Any, gate: Any, up: Any, 
 
     ``gate`` and ``up`` are what :func:`gated` stored there.
     """
-    key = _quick(_E_GATED_BACKWARD, act, (dh, gate, up, x, w_gate, w_up, dx, dw_gate, dw_up), _sync)
-    if key is True:
+    given = (dh, gate, up, x, w_gate, w_up, dx, dw_gate, dw_up)
+    if _quick(_E_GATED_BACKWARD, act, given, _sync):
         return
     what = "gated_backward"
     code, sync = _activation(what, act), _flag(_sync)
@@ -529,4 +487,4 @@ def gated_backward(dh: Any, x: Any, w_gate: Any, w_up: Any, gate: Any, up: Any, 
         return
     c.no_overlap()
     c.launch(_E_GATED_BACKWARD, (DH, SG, SU, X, G, U, DX, DG, DU), (DH, SG, SU, X, G, U, DX, DG, DU), (X.rows, n, k), code,
-             outputs, _off(X, 1) | _off(G, 2) | _off(U, 4) | _off(DH, 8), sync, key)
+             outputs, _off(X, 1) | _off(G, 2) | _off(U, 4) | _off(DH, 8), sync, given)

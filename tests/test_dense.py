@@ -214,6 +214,25 @@ def test_c_entries_want_their_scratch(name):
         assert "scratch" in cuda_ext.last_error()
 
 
+def test_extension_is_built_and_leaves_doubtful_calls_alone():
+    torch = pytest.importorskip("torch")
+    from easy_as_b200 import build, ops
+
+    assert build.OPS_STAMP.read_text().strip() == build.ops_hash()
+    ext = ops._load_ext()
+    assert ext
+    t = torch.zeros(4, 4, dtype=torch.float16)
+    for bufs in ((t, t, t), (new(4, 4),), (None, 3), [t], (None,) * 17):
+        assert ext.quick(0, 0, bufs, True) is None            # no CUDA tensors, other objects, no plan
+    assert ext.quick(0, -1, (None,), True) is None             # an unknown activation
+    assert ext.quick(0, 0, (None,), 1) is None                 # a flag that is not bool
+    assert ext.leave(0, 0, (t,), 1, b"", 0, 0, ()) is False     # nothing kept for them either
+    with pytest.raises(TypeError):
+        ext.quick(0, 0, (t,))
+    with pytest.raises(TypeError):
+        ext.quick("x", 0, (t,), True)
+
+
 def test_gpu_tests_reach_every_kernel():
     """The sizes of the exact GPU tests run every kernel that any call can reach (each is instantiated for some)."""
     import random
