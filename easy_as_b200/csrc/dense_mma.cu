@@ -1033,14 +1033,16 @@ int launch_tile(Params& q, int dev, cudaStream_t s, const char* who) {
 using Choice = DenseShape;
 
 // The shape of least estimated time, in microseconds as measured on one B200 at 1.9 GHz (bf16,
-// operands from HBM).  A step is one 64-deep k-block of one CTA or pair.
+// operands from HBM).  A step is one 64-deep k-block of one CTA or pair.  Over 65 random sizes the choice
+// was the best of all shapes within 5 %, but for eight within 21 (before the last entry's numbers).
 //   pair, 256 x 256        5.5 + rounds x k-blocks x 0.31   (4096^3: 94 us; 512 x 4096 x 4096: 25.3)
 //   one CTA per SM         4.5 + k-blocks x step, step 0.15 (BN 64) or 0.205 (128), 0.115 or 0.155 with
 //                          64 rows of A   (64 x 4096 x 4096: 12.3 BN 64, 15.0 BN 128)
 //   two CTAs per SM        4.0 + CTAs per SM x (k-blocks x step + 0.6 or 0.9), step 0.2 or 0.26
 //                          (2048^3: 25.1 BN 64, 17.5 BN 128)
-//   a split over 2 or 4    2 or 2.8 more for the exchange, and only while all CTAs are resident at
-//                          once (16 x 4096 x 4096, BN 64: 11.9 whole, 10.2 split in 2, 17.9 in 8)
+//   a split over 2 or 4    1.2 or 1.6 more for the exchange, and only while all CTAs are resident at
+//                          once (16 x 4096 x 4096, BN 64: 11.9 whole, 10.2 split in 2, 17.9 in 8;
+//                          184 x 560 x 1504: 6.9 whole, 5.9 split in 4)
 //   column sums            3 more with the pair kernel, which leaves them to a launch of their own
 Choice choose(const DenseProduct* p, int count, bool sums, int sms) {
   const int pairs = sms / 2 > 0 ? sms / 2 : 1;
@@ -1091,8 +1093,8 @@ Choice choose(const DenseProduct* p, int count, bool sums, int sms) {
         double us;
         if (c.deep) {
           if (few) c.ar = 64;
-          const double t0 = (double)((kb[0] + s0 - 1) / s0) * step + (s0 == 1 ? 0 : s0 == 2 ? 2 : 2.8);
-          const double t1 = (double)((kb[1] + s1 - 1) / s1) * step + (s1 == 1 ? 0 : s1 == 2 ? 2 : 2.8);
+          const double t0 = (double)((kb[0] + s0 - 1) / s0) * step + (s0 == 1 ? 0 : s0 == 2 ? 1.2 : 1.6);
+          const double t1 = (double)((kb[1] + s1 - 1) / s1) * step + (s1 == 1 ? 0 : s1 == 2 ? 1.2 : 1.6);
           us = 4.5 + (t0 > t1 ? t0 : t1);
         } else {
           const double two = 1.8 * (kb[0] * shared + tile_us);  // some SM has two tiles

@@ -15,7 +15,8 @@ VARIANTS = [(141, 9525, 1), (11, 2053, 2908), (5331, 1, 1863), (68, 1, 1601), (9
             (8, 4149, 5625), (72, 4488, 2854), (6, 2055, 7158), (2694, 66, 2214), (9, 1267, 2388), (9, 5295, 1),
             (275, 5248, 1), (4363, 37, 2853), (9, 1112, 2749), (2219, 36, 2229), (1, 1124, 2501), (3131, 1257, 1),
             (2182, 837, 1), (1755, 785, 1), (1, 1, 9666), (70, 1, 8776), (1, 1722, 4343), (3387, 1292, 72),
-            (1, 1355, 2095), (1720, 1511, 66), (2247, 861, 66), (1, 64, 50000)]
+            (1, 1355, 2095), (1720, 1511, 66), (2247, 861, 66), (13, 2500, 1355), (1723, 515, 1),
+            (2701, 1202, 51), (1, 64, 50000)]
 
 LINEAR, GATED, LINEAR_BACKWARD, GATED_BACKWARD = range(4)
 DX, DW, DB = 1, 2, 4
