@@ -12,6 +12,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "dense_internal.h"
 #include "dense_launch.h"
 #include "dense_math.cuh"
@@ -241,6 +243,23 @@ int check_sizes(const char* who, uint32_t M, uint32_t N, uint32_t K, int dtype, 
   return EAS_OK;
 }
 
+// A matrix of 16-bit values as it was passed; null ones are absent.
+struct Given {
+  const void* p;
+  uint64_t ld;
+  uint32_t rows, cols;
+};
+
+int check_matrices(const char* who, std::initializer_list<Given> all) {
+  for (const Given& g : all) {
+    if (!g.p) continue;
+    if (reinterpret_cast<uintptr_t>(g.p) & 1) return eas_fail(EAS_ERR_VALUE, "%s: an address is odd", who);
+    if (g.rows > 1 && g.ld < g.cols)
+      return eas_fail(EAS_ERR_VALUE, "%s: a row pitch is smaller than the row", who);
+  }
+  return EAS_OK;
+}
+
 int zero_rows(void* p, uint64_t ld, uint32_t rows, uint32_t cols, cudaStream_t s, const char* who) {
   return eas_cuda_check(cudaMemset2DAsync(p, ld * 2, 0, (size_t)cols * 2, rows, s), who, EAS_ERR_LAUNCH);
 }
@@ -426,6 +445,9 @@ extern "C" int eas_linear(const eas_linear_args* args, void* stream) {
   int rc = check_sizes(who, M, N, K, dtype, act);
   if (rc || M == 0) return rc;
   if (!x || !w || !y) return eas_fail(EAS_ERR_VALUE, "%s: null operand", who);
+  rc = check_matrices(who, {{x, ldx, M, K}, {w, ldw, N, K}, {bias, N, 1, N}, {y, ldy, M, N}, {pre, ldp, M, N},
+                            {residual, N, 1, N}});  // (the residual's rows may be one and the same)
+  if (rc) return rc;
   const bool few = dense_rows_fit((int)M, (int)K);
   const int off = few ? 0 : off_mask(x, ldx, kXOff) | off_mask(w, ldw, kWOff);
   const Scratch sc = forward_scratch(false, M, N, K, off);
@@ -459,6 +481,10 @@ extern "C" int eas_gated(const eas_gated_args* args, void* stream) {
   int rc = check_sizes(who, M, N, K, dtype, act);
   if (rc || M == 0) return rc;
   if (!x || !w_gate || !w_up || !h) return eas_fail(EAS_ERR_VALUE, "%s: null operand", who);
+  rc = check_matrices(who, {{x, ldx, M, K}, {w_gate, ldwg, N, K}, {w_up, ldwu, N, K}, {h, ldh, M, N}, {gate, ldg, M, N},
+                            {up, ldu, M, N}});
+  if (rc) return rc;
+  if (!gate != !up) return eas_fail(EAS_ERR_VALUE, "%s: gate and up go together", who);
   const bool few = dense_rows_fit((int)M, (int)K);
   const int off = few ? 0 : off_mask(x, ldx, kXOff) | off_mask(w_gate, ldwg, kWOff) | off_mask(w_up, ldwu, kUpOff);
   const Scratch sc = forward_scratch(true, M, N, K, off);
@@ -495,6 +521,9 @@ extern "C" int eas_linear_backward(const eas_linear_backward_args* args, void* s
   if (rc) return rc;
   if ((M && !dy) || (M && act != kNone && !pre) || (dx && !w) || (M && dw && !x))
     return eas_fail(EAS_ERR_VALUE, "%s: null operand", who);
+  rc = check_matrices(who, {{dy, lddy, M, N}, {pre, ldp, M, N}, {x, ldx, M, K}, {w, ldw, N, K}, {dx, lddx, M, K},
+                            {dw, lddw, N, K}, {db, N, 1, N}});
+  if (rc) return rc;
   const int outputs = (dx ? kDx : 0) | (dw ? kDw : 0) | (db ? kDb : 0);
   if (!outputs) return EAS_OK;
   const int off = off_mask(x, ldx, kXOff) | off_mask(w, ldw, kWOff) | off_mask(dy, lddy, kDyOff);
@@ -551,6 +580,9 @@ extern "C" int eas_gated_backward(const eas_gated_backward_args* args, void* str
   if (rc) return rc;
   if ((M && (!dh || !gate || !up)) || (dx && (!w_gate || !w_up)) || (M && (dw_gate || dw_up) && !x))
     return eas_fail(EAS_ERR_VALUE, "%s: null operand", who);
+  rc = check_matrices(who, {{dh, lddh, M, N}, {gate, ldg, M, N}, {up, ldu, M, N}, {x, ldx, M, K}, {w_gate, ldwg, N, K},
+                            {w_up, ldwu, N, K}, {dx, lddx, M, K}, {dw_gate, lddwg, N, K}, {dw_up, lddwu, N, K}});
+  if (rc) return rc;
   const int outputs = (dx ? kDx : 0) | (dw_gate || dw_up ? kDw : 0);
   if (!outputs) return EAS_OK;
   const int off = off_mask(x, ldx, kXOff) | off_mask(w_gate, ldwg, kWOff) | off_mask(w_up, ldwu, kUpOff) |

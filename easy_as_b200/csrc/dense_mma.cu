@@ -1123,6 +1123,9 @@ int launch_choice(const Choice& c, Params& q, int dev, cudaStream_t s, const cha
   return c.deep ? launch_tile<128, 128, true, MODE>(q, dev, s, who) : launch_tile<128, 128, false, MODE>(q, dev, s, who);
 }
 
+// The epilogue waits for a whole sum (0.31 us per k-block), with the budget of all waits, about 2 s.
+constexpr int64_t kMostSteps = 1 << 22;
+
 int64_t steps_of(const DenseProduct& p) { return (int64_t)((p.K + kBK - 1) / kBK) * p.terms; }
 
 void longer_first(const DenseProduct* p, int count, DenseProduct (&order)[2]) {
@@ -1152,7 +1155,8 @@ int dense_mma(const DenseProduct* p, int count, const DenseColSum& sums, cudaStr
   DenseProduct order[2];
   longer_first(p, count, order);
   for (int i = 0; i < count; ++i)
-    if (steps_of(order[i]) > 0x7fffffff) return eas_fail(EAS_ERR_VALUE, "%s: too many products in a sum", who);
+    if (steps_of(order[i]) > kMostSteps)
+      return eas_fail(EAS_ERR_VALUE, "%s: sums of more than %lld products are not taken", who, (long long)kMostSteps * kBK);
   const Choice c = choose(order, count, sums.db != nullptr, dense_sms(dev));
   const bool gated = p[0].gated;
   const int width = c.bn ? c.bn : 256;  // of the accumulator: a gated tile has half as many outputs

@@ -20,6 +20,9 @@ Sums are kept in f32 and every result is rounded once.  The backward passes also
 ``dg`` and ``du``, which are operands of matrix products, to the operands' dtype; ``dbias`` is
 summed from the unrounded values.  All results are the same bits on every run.
 
+The calls are plain launches: torch's autograd does not see them (nor that a buffer was written),
+and gradients come from the backward calls.
+
 ``act`` is one of ``none``, ``relu``, ``gelu`` (with erf), ``gelu_tanh``, ``silu``, ``sigmoid``.
 """
 

@@ -344,7 +344,8 @@ int eas_gemm_f16_noalloc(const void* a, const void* b, float* c, uint32_t M, uin
  * once.  M rows (tokens), K inputs, N outputs (of each projection).
  *   act: 0 none, 1 relu, 2 gelu (erf), 3 gelu_tanh, 4 silu, 5 sigmoid
  *   matrices are row-major with unit column stride; ld* are row pitches in
- *   elements, any alignment
+ *   elements, at least the columns (the residual's may be 0), any alignment
+ *   sums of at most 2^28 products
  *   dev is the device of the operands and of `stream`; it need not be current
  * M = 0 is a launch of nothing (the gradients of weights and bias, sums over no
  * rows, are set to zero); N = 0 or K = 0 is EAS_ERR_VALUE.  No output may

@@ -195,7 +195,7 @@ def test_argument_structs_match_the_header():
 @pytest.mark.parametrize("change,match", [
     ({"dtype": 2}, "dtype"), ({"dtype": -1}, "dtype"), ({"act": 6}, "activation"), ({"act": -1}, "activation"),
     ({"N": 0}, "positive"), ({"K": 0}, "positive"), ({"M": 0xffffffff}, "exceeds"), ({"K": 0x80000000}, "exceeds"),
-    ({"x": None}, "null"),
+    ({"x": None}, "null"), ({"x": 4097}, "odd"), ({"ldx": 15}, "pitch"),
 ])
 def test_c_entries_check_their_arguments(name, change, match):
     assert _call(name, **change) == cuda_ext.EAS_ERR_VALUE
