@@ -1043,6 +1043,8 @@ using Choice = DenseShape;
 //   a split over 2 or 4    1.2 or 1.6 more for the exchange, and only while all CTAs are resident at
 //                          once (16 x 4096 x 4096, BN 64: 11.9 whole, 10.2 split in 2, 17.9 in 8;
 //                          184 x 560 x 1504: 6.9 whole, 5.9 split in 4)
+//   two products           a few long sums beside many short ones are split over up to 8 CTAs (dx beside dW
+//                          of 7 x 6215 x 795: 98 k-blocks beside 637 tiles of one; whole, they took 46)
 //   column sums            3 more with the pair kernel, which leaves them to a launch of their own
 Choice choose(const DenseProduct* p, int count, bool sums, int sms) {
   const int pairs = sms / 2 > 0 ? sms / 2 : 1;
@@ -1085,20 +1087,25 @@ Choice choose(const DenseProduct* p, int count, bool sums, int sms) {
     }
     const bool few = most_rows <= 64 && !a_mn;
     const double step = bn == 64 ? (few ? 0.115 : 0.15) : (few ? 0.155 : 0.205);
-    for (int s0 = 1; s0 <= 4; s0 *= 2) {
+    auto exchange = [](int split) { return split == 1 ? 0 : split == 2 ? 1.2 : split == 4 ? 1.6 : 2.2; };
+    for (int s0 = 1; s0 <= 8; s0 *= 2) {
       for (int s1 = 1; s1 <= (count > 1 ? s0 : 1); s1 *= 2) {
         const int64_t ctas = tiles[0] * s0 + tiles[1] * s1;
-        if (s0 > 1 && (ctas > most_split || kb[0] < 2 * s0 || (s1 > 1 && kb[1] < 2 * s1))) continue;
+        if (s0 > 1 && (kb[0] < 2 * s0 || (s1 > 1 && kb[1] < 2 * s1))) continue;
         Choice c = {bn, {s0, s1}, 128, ctas <= sms};
         double us;
         if (c.deep) {
+          if (s0 > 4 || (s0 > 1 && ctas > most_split)) continue;
           if (few) c.ar = 64;
-          const double t0 = (double)((kb[0] + s0 - 1) / s0) * step + (s0 == 1 ? 0 : s0 == 2 ? 1.2 : 1.6);
-          const double t1 = (double)((kb[1] + s1 - 1) / s1) * step + (s1 == 1 ? 0 : s1 == 2 ? 1.2 : 1.6);
+          const double t0 = (double)((kb[0] + s0 - 1) / s0) * step + exchange(s0);
+          const double t1 = (double)((kb[1] + s1 - 1) / s1) * step + exchange(s1);
           us = 4.5 + (t0 > t1 ? t0 : t1);
         } else {
-          const double two = 1.8 * (kb[0] * shared + tile_us);  // some SM has two tiles
-          us = 4.0 + (work / sms > two ? work / sms : two);
+          if (s1 > 1 || (s0 > 1 && count == 1)) continue;
+          // the longer tiles beside another, and all work spread over the SMs
+          const double t0 = (double)((kb[0] + s0 - 1) / s0) * 1.8 * shared + 1.8 * tile_us + exchange(s0);
+          const double all = (work + (double)tiles[0] * s0 * exchange(s0)) / sms;
+          us = 4.0 + (all > t0 ? all : t0);
         }
         if (us < best_us) best = c, best_us = us;
       }

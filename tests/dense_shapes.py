@@ -16,7 +16,8 @@ VARIANTS = [(141, 9525, 1), (11, 2053, 2908), (5331, 1, 1863), (68, 1, 1601), (9
             (275, 5248, 1), (4363, 37, 2853), (9, 1112, 2749), (2219, 36, 2229), (1, 1124, 2501), (3131, 1257, 1),
             (2182, 837, 1), (1755, 785, 1), (1, 1, 9666), (70, 1, 8776), (1, 1722, 4343), (3387, 1292, 72),
             (1, 1355, 2095), (1720, 1511, 66), (2247, 861, 66), (13, 2500, 1355), (1723, 515, 1),
-            (2701, 1202, 51), (1, 64, 50000)]
+            (2701, 1202, 51), (7, 6215, 795), (177, 7941, 170),
+            (3503, 160, 408), (1, 64, 50000)]
 
 LINEAR, GATED, LINEAR_BACKWARD, GATED_BACKWARD = range(4)
 DX, DW, DB = 1, 2, 4
@@ -32,7 +33,12 @@ def plan(op, m, n, k, outputs=0, sms=148):
 
 
 def kernels(shape):
-    """Every kernel that the exact tests run a shape on (backward passes: all outputs, and each alone)."""
+    """Every way of a kernel that the exact tests run a shape on (backward passes: all outputs, and each alone): the
+    kernel, its width and rows, CTAs per SM, whether the sums of each product are split, and by as many CTAs."""
     calls = [(LINEAR, 0), (GATED, 0), (LINEAR_BACKWARD, DX | DW | DB), (LINEAR_BACKWARD, DX), (LINEAR_BACKWARD, DW),
              (GATED_BACKWARD, DX | DW), (GATED_BACKWARD, DX)]
-    return {(min(op, LINEAR_BACKWARD),) + plan(op, *shape, outputs) for op, outputs in calls}
+    found = set()
+    for op, outputs in calls:
+        kernel, width, s0, s1, rows, per_sm = plan(op, *shape, outputs)
+        found.add((min(op, LINEAR_BACKWARD), kernel, width, rows, per_sm, s0 > 1, s1 > 1, s0 == s1))
+    return found
