@@ -285,6 +285,38 @@ def test_special_values_stay_in_their_rows(m):
     assert db[3].isnan() and int(db.isnan().sum()) == 1
 
 
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("m", [2, 40, 300])
+def test_special_values_stay_in_their_columns(m, name):
+    """A NaN in one output's weights or bias is in that column alone, whatever the columns beside it share."""
+    n, k, dtype = 264, 72, torch.bfloat16
+    g = gen(m)
+    x, w, wu = normal(g, m, k, dtype), normal(g, n, k, dtype, 0.1), normal(g, n, k, dtype, 0.1)
+    bias = vector(normal(g, 1, n, dtype))
+    y, clean, h, hc = (torch.empty(m, n, device="cuda", dtype=dtype) for _ in range(4))
+    eas.ops.linear(x, w, clean, bias=bias, act=name)
+    eas.ops.gated(x, w, wu, hc, act=name)
+    for c in (0, 5, 130, n - 1):
+        bad = bias.clone()
+        bad[c] = float("nan")
+        eas.ops.linear(x, w, y, bias=bad, act=name)
+        wb = w.clone()
+        wb[c, 3] = float("nan")
+        eas.ops.gated(x, wb, wu, h, act=name)
+        keep = [i for i in range(n) if i != c]
+        assert y[:, c].isnan().all() and torch.equal(y[:, keep], clean[:, keep])
+        assert h[:, c].isnan().all() and torch.equal(h[:, keep], hc[:, keep])
+    for big in (3e38, 1e20, -1e20, -3e38):   # far values beside near ones
+        bad = bias.clone()
+        bad[2::4] = big
+        eas.ops.linear(x, w, y, bias=bad, act=name)
+        keep = [i for i in range(n) if i % 4 != 2]
+        assert torch.equal(y[:, keep], clean[:, keep])
+        far = oracle.act(name, bad[2::4].double())[0].nan_to_num(0.0)
+        far = torch.where(bad[2::4].double() < -1e4, torch.zeros_like(far), far) if name != "none" else far
+        assert torch.allclose(y[:, 2::4].double(), far.expand(m, -1), rtol=2.0 ** -7, atol=1e-30)
+
+
 def test_far_pre_activations():
     """Slopes and values where the exponentials under- and overflow."""
     dtype = torch.bfloat16
