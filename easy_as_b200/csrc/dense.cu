@@ -28,15 +28,21 @@ using namespace dense;
 // ---------------------------------------------------------------------------
 //
 // linear: dz = dy act'(z);  gated: dg = dh u act'(g), du = dh act(g).  One pass, 8 columns (16
-// bytes) per thread; a block covers 256 columns of kRowsPerBlock rows with 8 thread rows.  With
+// bytes) per thread; a block covers 256 columns of rows_per_block() rows with 8 thread rows.  With
 // db, each thread keeps the f32 sums of its columns, the block adds its 8 thread rows in shared
 // memory and writes one row of partial sums, which the products' launch adds in a fixed order: no
 // atomics, the same bits on every run.
+
+bool vec_ok(const void* p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld & 7) == 0; }
+
+// Past the last value of a matrix.
+const uint16_t* past_end(const uint16_t* p, int64_t ld, int64_t rows, int64_t cols) { return p + (rows - 1) * ld + cols; }
 
 struct ActGrad {
   const uint16_t* dy;
   const uint16_t* g;
   const uint16_t* u;
+  const uint16_t *dy_end, *g_end, *u_end;  // past their last values
   uint16_t* dg;     // dz, or dg; null when dz is dy itself (act none) and only db is wanted
   uint16_t* du;
   float* partial;   // [row blocks][N] sums of dz, or null
@@ -44,7 +50,6 @@ struct ActGrad {
   int M, N, rows_per_block;
   int act;
   bool bf16;
-  bool v_dy, v_g, v_u;  // 16-byte accesses allowed (dg and du lie in scratch: always)
 };
 
 template <bool BF16>
@@ -56,18 +61,8 @@ __device__ __forceinline__ void widen8(const uint4& w, float (&v)[8]) {
 }
 
 template <bool BF16>
-__device__ __forceinline__ void load8(const uint16_t* p, int n, bool vec, float (&v)[8]) {
-  if (vec && n >= 8) {
-    widen8<BF16>(__ldg(reinterpret_cast<const uint4*>(p)), v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? to_f32<BF16>(p[j]) : 0.0f;
-  }
-}
-
-template <bool BF16>
-__device__ __forceinline__ void store8(uint16_t* p, int n, bool vec, const float (&v)[8]) {
-  if (vec && n >= 8) {
+__device__ __forceinline__ void store8(uint16_t* p, int n, const float (&v)[8]) {
+  if (n >= 8) {
     *reinterpret_cast<uint4*>(p) = make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]),
                                               pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7]));
   } else {
@@ -77,7 +72,8 @@ __device__ __forceinline__ void store8(uint16_t* p, int n, bool vec, const float
   }
 }
 
-// VEC: every array takes 16-byte accesses, so that only the last columns need other ones.
+// VEC: every array takes 16-byte accesses, so that only the last columns need other ones.  (Others are
+// gathered from aligned words.)
 template <bool GATED, bool BF16, bool VEC>
 __global__ void __launch_bounds__(256) act_grad_kernel(const __grid_constant__ ActGrad p) {
   __shared__ float sums[8][32][9];
@@ -103,8 +99,8 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const __grid_constant__ A
             w[j] = dy[j] * u[j] * d;
             o[j] = dy[j] * v;
           }
-          store8<BF16>(p.dg + m * p.ldo + n0, cols, true, w);
-          store8<BF16>(p.du + m * p.ldo + n0, cols, true, o);
+          store8<BF16>(p.dg + m * p.ldo + n0, cols, w);
+          store8<BF16>(p.du + m * p.ldo + n0, cols, o);
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -113,7 +109,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const __grid_constant__ A
             o[j] = dy[j] * d;
             sum[j] += o[j];
           }
-          if (p.dg) store8<BF16>(p.dg + m * p.ldo + n0, cols, true, o);
+          if (p.dg) store8<BF16>(p.dg + m * p.ldo + n0, cols, o);
         }
       };
       float dy[8], g[8], u[8];
@@ -140,9 +136,13 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const __grid_constant__ A
         }
       }
       for (; m < r1; m += 8) {
-        load8<BF16>(p.dy + m * p.lddy + n0, cols, VEC || p.v_dy, dy);
-        if (kG) load8<BF16>(p.g + m * p.ldg + n0, cols, VEC || p.v_g, g);
-        if (GATED) load8<BF16>(p.u + m * p.ldu + n0, cols, VEC || p.v_u, u);
+        Gather8 wd, wg, wu;
+        wd.fetch(p.dy + m * p.lddy + n0, cols, p.dy, p.dy_end);
+        if (kG) wg.fetch(p.g + m * p.ldg + n0, cols, p.g, p.g_end);
+        if (GATED) wu.fetch(p.u + m * p.ldu + n0, cols, p.u, p.u_end);
+        widen8<BF16>(wd.get(), dy);
+        if (kG) widen8<BF16>(wg.get(), g);
+        if (GATED) widen8<BF16>(wu.get(), u);
         row(m, dy, g, u);
       }
     });
@@ -160,7 +160,11 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const __grid_constant__ A
 
 template <bool GATED>
 int launch_act_grad(ActGrad& g, int blocks, cudaStream_t s, const char* who) {
-  const bool vec = g.v_dy && (g.v_g || (!GATED && g.act == kNone)) && (!GATED || g.v_u);
+  const bool kG = GATED || g.act != kNone;
+  const bool vec = vec_ok(g.dy, g.lddy) && (!kG || vec_ok(g.g, g.ldg)) && (!GATED || vec_ok(g.u, g.ldu));
+  g.dy_end = past_end(g.dy, g.lddy, g.M, g.N);
+  if (kG) g.g_end = past_end(g.g, g.ldg, g.M, g.N);
+  if (GATED) g.u_end = past_end(g.u, g.ldu, g.M, g.N);
   const void* kernel = g.bf16 ? (vec ? reinterpret_cast<const void*>(&act_grad_kernel<GATED, true, true>)
                                      : reinterpret_cast<const void*>(&act_grad_kernel<GATED, true, false>))
                               : (vec ? reinterpret_cast<const void*>(&act_grad_kernel<GATED, false, true>)
@@ -169,7 +173,9 @@ int launch_act_grad(ActGrad& g, int blocks, cudaStream_t s, const char* who) {
 }
 
 // Copies of operands whose rows TMA cannot read in place, in rows of a multiple of 8 elements (zeros
-// past the end): up to three matrices in one launch (one per row of blocks), 8 elements per thread.
+// past the end): up to three matrices in one launch (one per row of blocks), 8 elements per thread.  Bound
+// by HBM: 97 MB of 3648 x 6675 weights take 39 us, 5 TB/s.  (Loading aligned words and shifting them,
+// as the other kernels do, took as long there and 2 us more on small matrices.)
 struct Repitch {
   struct Matrix {
     const uint16_t* src;
@@ -213,8 +219,6 @@ int rows_per_block(int M, int N, bool sums) {
 // Up to so many rows the products' launch sums the columns of dy itself where dz is dy (32 columns per
 // CTA, beside the tiles); beyond, act_grad_kernel makes partial sums first.
 constexpr uint32_t kDirectRows = 2048;
-
-bool vec_ok(const void* p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld & 7) == 0; }
 
 // Makes `dev` current for the scope of a call.
 struct DeviceScope {
@@ -545,7 +549,6 @@ extern "C" int eas_linear_backward(const eas_linear_backward_args* args, void* s
     g.dy = u16(dy), g.g = u16(pre), g.dg = dz, g.partial = partial;
     g.lddy = lddy, g.ldg = ldp, g.ldo = sc.ldn;
     g.M = M, g.N = N, g.rows_per_block = sc.rows, g.act = act, g.bf16 = dtype == kBF16;
-    g.v_dy = vec_ok(dy, lddy), g.v_g = pre && vec_ok(pre, ldp);
     rc = launch_act_grad<false>(g, sc.blocks, s, who);
     if (rc) return rc;
   }
@@ -558,7 +561,7 @@ extern "C" int eas_linear_backward(const eas_linear_backward_args* args, void* s
   if (db) {
     sums.db = u16(db), sums.N = (int)N, sums.bf16 = dtype == kBF16;
     if (sc.direct)
-      sums.matrix = u16(dy), sums.ld = (int64_t)lddy, sums.rows = (int)M, sums.vec = vec_ok(dy, lddy);
+      sums.matrix = u16(dy), sums.ld = (int64_t)lddy, sums.rows = (int)M;
     else
       sums.partial = partial, sums.rows = sc.blocks;
   }
@@ -604,7 +607,6 @@ extern "C" int eas_gated_backward(const eas_gated_backward_args* args, void* str
   g.dy = u16(dh), g.g = u16(gate), g.u = u16(up), g.dg = dg, g.du = du;
   g.lddy = lddh, g.ldg = ldg, g.ldu = ldu, g.ldo = sc.ldn;
   g.M = M, g.N = N, g.rows_per_block = sc.rows, g.act = act, g.bf16 = dtype == kBF16;
-  g.v_dy = vec_ok(dh, lddh), g.v_g = vec_ok(gate, ldg), g.v_u = vec_ok(up, ldu);
   rc = launch_act_grad<true>(g, sc.blocks, s, who);
   if (rc) return rc;
   const bool dw = outputs & kDw;

@@ -36,7 +36,7 @@ struct DenseColSum {
   int64_t ld = 0;  // of the matrix
   uint16_t* db = nullptr;
   int rows = 0, N = 0;
-  bool bf16 = false, vec = false;  // vec: rows of the matrix start on 16 bytes
+  bool bf16 = false;
 };
 
 int dense_column_sums(const DenseColSum& sums, cudaStream_t stream, const char* who);

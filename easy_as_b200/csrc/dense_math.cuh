@@ -154,4 +154,52 @@ __device__ __forceinline__ void with_act(int a, F&& f) {
   }
 }
 
+// 16-bit values s .. s + 7 of the 16 in two neighbouring words of 16 bytes.
+__device__ __forceinline__ uint4 shift8(const uint4& a, const uint4& b, int s) {
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int j = 0; j < 6; ++j) w[j] = s & 4 ? w[j + 2] : w[j];
+#pragma unroll
+  for (int j = 0; j < 5; ++j) w[j] = s & 2 ? w[j + 1] : w[j];
+  const int bits = (s & 1) * 16;
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                    __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+
+// v with zeros behind its first n of 8 values.
+__device__ __forceinline__ uint4 first8(const uint4& v, int n) {
+  auto mask = [&](int j) { return n >= 2 * j + 2 ? 0xffffffffu : n == 2 * j + 1 ? 0xffffu : 0u; };
+  return make_uint4(v.x & mask(0), v.y & mask(1), v.z & mask(2), v.w & mask(3));
+}
+
+// The first n of 8 values (zeros behind them) from any address: the one or two aligned words of 16 bytes
+// that hold them, shifted together.  fetch() only loads, so that several can be under way before the
+// first get().  A word that reaches out of the matrix's own memory [lo, hi) is left out, and its
+// values are read one by one.
+struct Gather8 {
+  uint4 a, b;
+  const uint16_t* p;
+  int n, s;
+  bool inside;
+
+  __device__ __forceinline__ void fetch(const uint16_t* from, int count, const uint16_t* lo, const uint16_t* hi) {
+    p = from, n = count;
+    s = (int)(reinterpret_cast<uintptr_t>(p) >> 1) & 7;
+    const uint16_t* word = p - s;
+    const bool two = s + min(n, 8) > 8;
+    inside = word >= lo && word + (two ? 16 : 8) <= hi;
+    a = b = make_uint4(0, 0, 0, 0);
+    if (inside && n > 0) a = __ldg(reinterpret_cast<const uint4*>(word));
+    if (inside && two) b = __ldg(reinterpret_cast<const uint4*>(word) + 1);
+  }
+  __device__ __forceinline__ uint4 get() const {
+    uint4 v = shift8(a, b, s);
+    if (!inside) {
+      auto one = [&](int j) { return j < n ? (uint32_t)__ldg(p + j) : 0u; };
+      v = make_uint4(one(0) | one(1) << 16, one(2) | one(3) << 16, one(4) | one(5) << 16, one(6) | one(7) << 16);
+    }
+    return first8(v, n);
+  }
+};
+
 }  // namespace dense

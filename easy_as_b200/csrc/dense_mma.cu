@@ -282,17 +282,14 @@ __device__ __forceinline__ void add_residual(const Params& p, Boxes& bx, int lan
     for (int j = 0; j < 4; ++j) w[j] = src[j];
   } else {
     uint8_t* box = next_box(bx, lane);
-    const int rows = n0 + lane < N ? min(32, M - m0) : 0;
-    const uint16_t* src = p.residual + (int64_t)m0 * p.ldr + n0 + lane;
-    const ColumnInBox col(box, lane);
+    const int c = lane & 3, cols = N - n0 - 8 * c;
+    const uint16_t* end = p.residual + (int64_t)(M - 1) * p.ldr + N;
+    Gather8 from[4];
 #pragma unroll
-    for (int r0 = 0; r0 < 32; r0 += 16) {  // 16 loads under way
-      uint16_t h[16];
+    for (int i = 0; i < 4; ++i)
+      from[i].fetch(p.residual + (int64_t)min(m0 + 8 * i + (lane >> 2), M - 1) * p.ldr + n0 + 8 * c, cols, p.residual, end);
 #pragma unroll
-      for (int r = 0; r < 16; ++r, src += p.ldr) h[r] = r0 + r < rows ? *src : (uint16_t)0;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) *col.at(r0 + r) = h[r];
-    }
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(box_chunk(box, 8 * i + (lane >> 2), c)) = from[i].get();
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4*>(box_chunk(box, lane, j));
@@ -645,7 +642,7 @@ struct TileShape {
   static_assert(kSmem <= (DEEP ? 232448 : 115000), "shared memory");
 };
 
-// db of 32 columns from n0 on: each row of threads adds every so-manieth row, then the rows of threads
+// db of 32 columns from n0 on: each row of threads adds every 48th row, then the rows of threads
 // are added in order.  `sums`: 48 x 33 floats.
 template <bool BF16>
 __device__ __forceinline__ void column_sums_of_matrix(const DenseColSum& c, int n0, float* sums) {
@@ -653,21 +650,17 @@ __device__ __forceinline__ void column_sums_of_matrix(const DenseColSum& c, int 
   const int tx = threadIdx.x & 3, ty = threadIdx.x >> 2, n = n0 + 8 * tx;
   float s[8] = {};
   if (n < c.N) {
-    const bool whole = c.vec && n + 8 <= c.N;
+    const uint16_t* end = c.matrix + (int64_t)(c.rows - 1) * c.ld + c.N;
 #pragma unroll 4
     for (int r = ty; r < c.rows; r += kRows) {
-      const uint16_t* src = c.matrix + (int64_t)r * c.ld + n;
+      Gather8 from;
+      from.fetch(c.matrix + (int64_t)r * c.ld + n, c.N - n, c.matrix, end);
+      const uint4 w = from.get();
       float v[8];
-      if (whole) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(src));
-        unpack2<BF16>(w.x, v[0], v[1]);
-        unpack2<BF16>(w.y, v[2], v[3]);
-        unpack2<BF16>(w.z, v[4], v[5]);
-        unpack2<BF16>(w.w, v[6], v[7]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = n + j < c.N ? to_f32<BF16>(src[j]) : 0.0f;
-      }
+      unpack2<BF16>(w.x, v[0], v[1]);
+      unpack2<BF16>(w.y, v[2], v[3]);
+      unpack2<BF16>(w.z, v[4], v[5]);
+      unpack2<BF16>(w.w, v[6], v[7]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[j] += v[j];
     }

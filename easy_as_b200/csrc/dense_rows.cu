@@ -5,20 +5,24 @@
 //
 // With so few rows the product reads W once and does almost nothing with it: the bound is HBM, and
 // what counts is to keep bytes under way with few instructions.  Each warp copies 16 rows x 64 values
-// at a time into a queue of its own in shared memory (cp.async), several pieces ahead, and
-// hands them to mma.sync from there.  A warp reads only what it copied itself, so the queue needs
-// no barrier between warps.  x lies in shared memory whole.  Rows of W are the instruction's 16 rows (gated: 8 of the gate, 8 of the up projection),
-// rows of x its 8 columns.  Its k order is a convention between the two operands: lane t of a quad
-// takes k = 8t .. 8t+7 of 32, as it lies in memory, and hands words 0-1 to one m16n8k16 and words
-// 2-3 to the next, on both operands alike.  Rows that do not start on 16 bytes are loaded straight
-// into registers, value by value.
+// at a time into a queue of its own in shared memory (cp.async), several pieces ahead, and hands them
+// to mma.sync from there.  A warp reads only what it copied itself, so the queue needs no barrier
+// between warps.  x lies in shared memory whole.  Rows of W are the instruction's 16 rows (gated: 8 of
+// the gate, 8 of the up projection), rows of x its 8 columns.  Its k order is a convention between the
+// two operands: lane t of a quad takes k = 8t .. 8t+7 of 32, as it lies in memory, and hands words 0-1
+// to one m16n8k16 and words 2-3 to the next, on both operands alike.
+//
+// Rows that do not start on 16 bytes are copied as the aligned words that hold them, one more per row
+// and piece, and shifted into place on their way from the queue to the instruction (4096 x 4096, one
+// row: 7.8 us; K = 4095: 11.0, and 15.2 with 8 rows; loaded value by value they took 24).
 //
 // Two blocks of 8 warps stay on each SM (or one of 16, where x needs the room), each with an equal
-// share of W's rows (N / 296 of them, give or take one, so that no SM has more to read than another), in tiles of at most 16 (gated: 8 of
-// each weight).  The warps take every 8th (16th) 64-wide piece of K, and the queue runs on over the
-// tiles' ends.  Where a share would be too few rows for a tile, the CTAs of a cluster share the
-// rows of several and split K.  The sums of the warps, then of the cluster's CTAs, are added in a
-// fixed order through (distributed) shared memory, so results are the same bits on every run.
+// share of W's rows (N / 296 of them, give or take one, so that no SM has more to read than another),
+// in tiles of at most 16 (gated: 8 of each weight).  The warps take every 8th (16th) 64-wide piece of K,
+// and the queue runs on over the tiles' ends.  Where a share would be too few rows for a tile, the CTAs
+// of a cluster share the rows of several and split K.  The sums of the warps, then of the cluster's
+// CTAs, are added in a fixed order through (distributed) shared memory, so results are the same bits
+// on every run.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -35,6 +39,7 @@ using namespace dense;
 struct RowsParams {
   const uint16_t* x;
   const uint16_t* w[2];
+  const uint16_t *x_end, *w_end[2];  // past their last values
   const uint16_t* bias;
   const uint16_t* residual;
   uint16_t* y;
@@ -58,17 +63,6 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// 8 values of a row, of which `n` are left: zeros past them.
-__device__ __forceinline__ uint4 load8(const uint16_t* p, int n) {
-  uint32_t w[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t lo = 2 * j < n ? __ldg(p + 2 * j) : 0, hi = 2 * j + 1 < n ? __ldg(p + 2 * j + 1) : 0;
-    w[j] = lo | (hi << 16);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 __device__ __forceinline__ void copy16(uint32_t dst, const uint16_t* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -86,28 +80,32 @@ __device__ __forceinline__ uint4 lds128(uint32_t at) {
 }
 
 constexpr int kPiece = 64;       // values of K per row and piece
-constexpr int kSlot = 16 * 128;  // a piece of 16 rows of W
-constexpr int kPieces = 4;       // per warp
-constexpr int kDepth = kPieces - 1;  // under way while one is consumed
 
 // W warps per block, and of x in shared memory: two blocks of 8 warps per SM, or one of 16 with twice
-// the room for x.
-template <int W>
+// the room for x.  VEC: rows of x and W start on 16 bytes.  A slot holds a piece of 16 rows of W: 8 words
+// each, and behind them (not VEC) the 16 rows' ninth ones.
+template <int W, bool VEC>
 struct Shape {
-  static constexpr int kQueue = W * kPieces * kSlot;  // 64 or 128 KB
-  static constexpr int kMostX = W == 8 ? 40960 : 81920;
+  static constexpr int kSlot = 16 * 128 + (VEC ? 0 : 16 * 16);
+  static constexpr int kPieces = VEC ? 4 : 3;      // per warp
+  static constexpr int kDepth = kPieces - 1;       // under way while one is consumed
+  static constexpr int kQueue = W * kPieces * kSlot;  // 64 or 54 KB, or twice that
 };
+
+template <int W>
+constexpr int kMostX = W == 8 ? 40960 : 81920;
 
 // x in shared memory: rows of whole pieces, 64 bytes apart modulo 128, so that the quads of a
 // quarter warp read different banks.
 __host__ __device__ constexpr int64_t x_pitch(int64_t K) { return (K + kPiece - 1) / kPiece * (2 * kPiece) + 64; }
 
-// VEC: rows of x and W start on 16 bytes.
 template <int kWarps, bool GATED, bool VEC, bool BF16>
 __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
     dense_rows_kernel(const __grid_constant__ RowsParams p) {
   constexpr int kTile = GATED ? 8 : 16;  // outputs; always 16 rows of W
   constexpr int kRows = kDenseRows, kCols = 16;
+  using Q = Shape<kWarps, VEC>;
+  constexpr int kSlot = Q::kSlot, kDepth = Q::kDepth;
   extern __shared__ __align__(128) uint8_t queue[];
   __shared__ float part[2][kWarps][kRows][kCols + 1];  // tiles take turns
   __shared__ float sums[kRows][kCols + 1];
@@ -126,41 +124,72 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
   // Chunk c of a row lies at place c ^ 4 (row & 1), so that two rows' quads read different banks.
   // Rows past the tile are not copied: whatever their place in the queue holds reaches only sums
   // that nobody looks at.
-  const int c8 = lane & 7, r8 = lane >> 3;
-  const uint16_t* w[4];
+  // (Not VEC: 9 words of each row, in the order of the lanes.)
+  constexpr int kCopies = VEC ? 4 : 5;
+  auto copy_row = [&](int i) { return VEC ? (lane >> 3) + 4 * i : (lane + 32 * i) / 9; };
+  auto copy_word = [&](int i) { return VEC ? lane & 7 : (lane + 32 * i) % 9; };
+  auto word_at = [](int r, int c) { return c == 8 ? 2048 + 16 * r : r * 128 + ((c ^ (4 * (r & 1))) << 4); };
+  auto lag = [](const uint16_t* at) { return VEC ? 0 : (int)(reinterpret_cast<uintptr_t>(at) >> 1) & 7; };
+  auto w_row = [&](int r, int n0, int n1) {  // row r of a tile's 16
+    const int n = n0 + (GATED ? r & 7 : r), h = GATED && r >= 8;
+    return p.w[h] + (int64_t)(n < n1 ? n : n0) * p.ldw[h];
+  };
+  const uint16_t* w[kCopies];
   int have = 0;
+  int left_of[kCopies];  // (not VEC) values of K behind the word's first
   auto aim = [&](int n0, int n1) {
     have = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int h = GATED ? i >> 1 : 0, n = n0 + r8 + 4 * (GATED ? i & 1 : i);
-      have |= (n < n1 ? 1 : 0) << i;
-      w[i] = p.w[h] + (int64_t)(n < n1 ? n : n0) * p.ldw[h] + 8 * c8;
+    for (int i = 0; i < kCopies; ++i) {
+      const int r = min(copy_row(i), 15), c = copy_word(i);
+      const uint16_t* at = w_row(r, n0, n1);
+      const int s = lag(at);
+      const bool use = copy_row(i) < 16 && n0 + (GATED ? r & 7 : r) < n1 && (c < 8 || s);
+      have |= (use ? 1 : 0) << i;
+      w[i] = at - s + 8 * c;
+      left_of[i] = p.K - 8 * c + s;
     }
   };
   const int xrow = min(g, p.M - 1);
 
   grid_order();
 
-  const uint32_t mine = tc::smem_u32(queue) + warp * (kPieces * kSlot);
-  const uint32_t put = mine + r8 * 128 + ((c8 ^ (4 * (r8 & 1))) << 4);  // + 512 per 4 rows
-  const uint32_t take = mine + g * 128 + ((t ^ (4 * (g & 1))) << 4);    // v = 1: ^ 64; row g + 8: + 1024
+  const uint32_t mine = tc::smem_u32(queue) + warp * (Q::kPieces * kSlot);
+  const uint32_t take = mine + word_at(g, t);  // v = 1: ^ 64; row g + 8: + 1024
+  // (not VEC) the words behind those, of rows g and g + 8
+  const uint32_t next0 = mine + word_at(g, t + 1), next1[2] = {mine + word_at(g, t + 5), mine + word_at(g + 8, t + 5)};
   const int64_t pitch = x_pitch(p.K);
-  const uint32_t xs = tc::smem_u32(queue) + Shape<kWarps>::kQueue;
+  const uint32_t xs = tc::smem_u32(queue) + Q::kQueue;
   const uint32_t xmine = xs + (uint32_t)(xrow * pitch) + 16 * t;
   int in_tile = 0, in_k = first, in_slot = 0, out_slot = 0;
   if (tiles > 0) aim(tile_row(0), tile_row(1));
   auto issue = [&]() {  // always one group, empty past the end: the waits count groups
-    if (VEC && in_tile < tiles && in_k < p.K) {
-      const uint32_t at = put + in_slot * kSlot;
-      if (in_k + kPiece <= p.K) {
+    if (in_tile < tiles && in_k < p.K) {
+      const uint32_t at = mine + in_slot * kSlot;
+      if constexpr (!VEC) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (have >> i & 1) copy16(at + i * 512, w[i] + in_k);
+        for (int i = 0; i < kCopies; ++i) {
+          const uint32_t dst = at + word_at(copy_row(i), copy_word(i));
+          const int h = GATED && copy_row(i) >= 8;
+          const uint16_t* src = w[i] + in_k;
+          if (!(have >> i & 1) || in_k >= left_of[i]) continue;
+          if (src >= p.w[h] && src + 8 <= p.w_end[h]) {
+            copy16(dst, src);
+          } else {  // reaches out of the matrix's memory
+            for (int j = 0; j < 8; ++j)
+              if (src + j >= p.w[h] && src + j < p.w_end[h])
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + 2 * j), "h"(src[j]) : "memory");
+          }
+        }
+      } else if (in_k + kPiece <= p.K) {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i)
+          if (have >> i & 1) copy16(at + word_at(copy_row(i), copy_word(i)), w[i] + in_k);
       } else {  // zeros past the end of K
-        const int left = p.K - in_k - 8 * c8;
+        const int left = p.K - in_k - 8 * copy_word(0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) copy8(at + i * 512, w[i] + (left > 0 ? in_k : 0), left);
+        for (int i = 0; i < kCopies; ++i)
+          copy8(at + word_at(copy_row(i), copy_word(i)), w[i] + (left > 0 ? in_k : 0), left);
       }
       in_slot = in_slot == kDepth ? 0 : in_slot + 1;
       in_k += stride;
@@ -171,53 +200,56 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  if constexpr (VEC) {
-    // x once per block: from every warp's piece it would be read by all SMs at the same time, and
-    // its few lines of L2 were what the kernel waited for (4 rows: 44 us where one took 34)
-    const int words = (int)((pitch - 64) / 16);
-    for (int e = threadIdx.x; e < p.M * words; e += kWarps * 32) {
-      const int r = e / words, c = e % words;
-      const int left = p.K - 8 * c;
-      copy8(xs + (uint32_t)(r * pitch) + 16 * c, p.x + (int64_t)r * p.ldx + (left > 0 ? 8 * c : 0), left);
+  // x once per block: from every warp's piece it would be read by all SMs at the same time, and
+  // its few lines of L2 were what the kernel waited for (4 rows: 44 us where one took 34)
+  const int words = (int)((pitch - 64) / 16);
+  for (int e = threadIdx.x; e < p.M * words; e += kWarps * 32) {
+    const int r = e / words, c = e % words;
+    const int left = p.K - 8 * c;
+    const uint16_t* src = p.x + (int64_t)r * p.ldx + (left > 0 ? 8 * c : 0);
+    const uint32_t dst = xs + (uint32_t)(r * pitch) + 16 * c;
+    if constexpr (VEC) {
+      copy8(dst, src, left);
+    } else {
+      Gather8 from;
+      from.fetch(src, left, p.x, p.x_end);
+      const uint4 v = from.get();
+      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                   : "memory");
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    for (int i = 0; i < kDepth; ++i) issue();
-    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth) : "memory");
-    __syncthreads();
   }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  for (int i = 0; i < kDepth; ++i) issue();
+  asm volatile("cp.async.wait_group %0;" ::"n"(kDepth) : "memory");
+  __syncthreads();
 
   for (int j = 0; j < tiles; ++j) {
     const int n0 = tile_row(j), width = tile_row(j + 1) - n0;
-    const uint16_t* row[2];  // of this lane's values of W, where they are loaded one by one
-    if (!VEC) {
+    int shift[2];  // of rows g and g + 8
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int n = n0 + min(GATED ? g : 8 * i + g, width - 1);
-        row[i] = p.w[GATED ? i : 0] + (int64_t)n * p.ldw[GATED ? i : 0] + 8 * t;
-      }
-    }
+    for (int i = 0; i < 2; ++i) shift[i] = lag(w_row(g + 8 * i, n0, n0 + width));
     float acc[4] = {};
     for (int k = first; k < p.K; k += stride) {
-      uint32_t at = 0;
-      if constexpr (VEC) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
-        __syncwarp();  // the piece is here, and everyone has read the one before it
-        issue();
-        at = take + out_slot * kSlot;
-        out_slot = out_slot == kDepth ? 0 : out_slot + 1;
-      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+      __syncwarp();  // the piece is here, and everyone has read the one before it
+      issue();
+      const uint32_t slot = out_slot * kSlot;
+      out_slot = out_slot == kDepth ? 0 : out_slot + 1;
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
-        uint4 a[2], b;
-        if constexpr (VEC) {
-          a[0] = lds128((at ^ (v * 64)));
-          a[1] = lds128((at ^ (v * 64)) + 1024);
-          b = lds128(xmine + 2 * k + v * 64);
-        } else {
-          const int left = p.K - k - 32 * v - 8 * t;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) a[i] = load8(row[i] + k + 32 * v, left);
-          b = load8(p.x + (int64_t)xrow * p.ldx + 8 * t + k + 32 * v, left);
+        uint4 a[2];
+        const uint4 b = lds128(xmine + 2 * k + v * 64);
+        a[0] = lds128((take + slot) ^ (v * 64));
+        a[1] = lds128(((take + slot) ^ (v * 64)) + 1024);
+        if constexpr (!VEC) {
+          const uint4 c0 = lds128((v ? next1[0] : next0) + slot), c1 = lds128((v ? next1[1] : next0 + 1024) + slot);
+          a[0] = shift8(a[0], c0, shift[0]);
+          a[1] = shift8(a[1], c1, shift[1]);
+          if (k + kPiece > p.K) {  // what lies behind the row's end
+            const int left = p.K - k - 32 * v - 8 * t;
+            a[0] = first8(a[0], left);
+            a[1] = first8(a[1], left);
+          }
         }
         const uint32_t a0[4] = {a[0].x, a[1].x, a[0].y, a[1].y};
         const uint32_t a1[4] = {a[0].z, a[1].z, a[0].w, a[1].w};
@@ -287,22 +319,24 @@ template <int W, bool GATED, bool BF16>
 int launch_rows(const DenseProduct& p, RowsParams& q, bool vec, int dev, cudaStream_t s, const char* who) {
   static bool ready[64] = {false};
   const void* fast = reinterpret_cast<const void*>(&dense_rows_kernel<W, GATED, true, BF16>);
-  const void* slow = reinterpret_cast<const void*>(&dense_rows_kernel<8, GATED, false, BF16>);
+  const void* slow = reinterpret_cast<const void*>(&dense_rows_kernel<W, GATED, false, BF16>);
   if (!ready[dev & 63]) {
-    int rc = eas_cuda_check(cudaFuncSetAttribute(fast, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 Shape<W>::kQueue + Shape<W>::kMostX),
-                            who, EAS_ERR_LAUNCH);
+    auto allow = [&](const void* kernel, int bytes) {
+      return eas_cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), who,
+                            EAS_ERR_LAUNCH);
+    };
+    int rc = allow(fast, Shape<W, true>::kQueue + kMostX<W>);
+    if (!rc) rc = allow(slow, Shape<W, false>::kQueue + kMostX<W>);
     if (rc) return rc;
     ready[dev & 63] = true;
   }
-  const int warps = vec ? W : 8;
-  const int resident = 16 / warps * dense_sms(dev);
-  q.split = choose_split(p, resident, warps);
+  const int resident = 16 / W * dense_sms(dev);
+  q.split = choose_split(p, resident, W);
   // no block without rows; four rows a block or more, where there are few
   int groups = resident / q.split;
   if (groups > (p.N + 3) / 4) groups = (p.N + 3) / 4;
-  return dense_launch(vec ? fast : slow, dim3(groups * q.split), q.split > 1 ? q.split : 0, warps * 32,
-                      vec ? Shape<W>::kQueue + q.M * (int)x_pitch(q.K) : 0, s, &q, who);
+  return dense_launch(vec ? fast : slow, dim3(groups * q.split), q.split > 1 ? q.split : 0, W * 32,
+                      (vec ? Shape<W, true>::kQueue : Shape<W, false>::kQueue) + q.M * (int)x_pitch(q.K), s, &q, who);
 }
 
 template <int W>
@@ -317,11 +351,11 @@ int launch_rows(const DenseProduct& p, RowsParams& q, bool vec, int dev, cudaStr
 }  // namespace
 
 int dense_rows_split(const DenseProduct& p, int sms) {
-  const int warps = p.M * x_pitch(p.K) <= Shape<8>::kMostX ? 8 : 16;
+  const int warps = p.M * x_pitch(p.K) <= kMostX<8> ? 8 : 16;
   return choose_split(p, 16 / warps * sms, warps);
 }
 
-bool dense_rows_fit(int M, int K) { return M <= kDenseRows && M * x_pitch(K) <= Shape<16>::kMostX; }
+bool dense_rows_fit(int M, int K) { return M <= kDenseRows && M * x_pitch(K) <= kMostX<16>; }
 
 int dense_rows(const DenseProduct& p, cudaStream_t stream, const char* who) {
   int dev = 0;
@@ -333,8 +367,10 @@ int dense_rows(const DenseProduct& p, cudaStream_t stream, const char* who) {
   q.ldx = (int64_t)p.lda[0], q.ldw[0] = (int64_t)p.ldb[0], q.ldw[1] = (int64_t)p.ldb[1];
   q.ldr = (int64_t)p.ldr, q.ldy = (int64_t)p.ldy[0], q.ldp = (int64_t)p.ldp, q.ldp2 = (int64_t)p.ldp2;
   q.M = p.M, q.N = p.N, q.K = p.K, q.act = p.act;
+  q.x_end = q.x + (q.M - 1) * q.ldx + q.K;
+  for (int i = 0; i < (p.gated ? 2 : 1); ++i) q.w_end[i] = q.w[i] + (q.N - 1) * q.ldw[i] + q.K;
   const bool vec = aligned16(p.a[0], p.M > 1 ? p.lda[0] : 0) && aligned16(p.b[0], p.N > 1 ? p.ldb[0] : 0) &&
                    (!p.gated || aligned16(p.b[1], p.N > 1 ? p.ldb[1] : 0));
-  return p.M * x_pitch(p.K) <= Shape<8>::kMostX ? launch_rows<8>(p, q, vec, dev, stream, who)
+  return p.M * x_pitch(p.K) <= kMostX<8> ? launch_rows<8>(p, q, vec, dev, stream, who)
                                                 : launch_rows<16>(p, q, vec, dev, stream, who);
 }

@@ -285,6 +285,44 @@ def test_special_values_stay_in_their_rows(m):
     assert db[3].isnan() and int(db.isnan().sum()) == 1
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 5, 7), (1, 300, 64), (2, 17, 65), (3, 70, 1025), (5, 4099, 130), (7, 33, 127),
+                                   (8, 600, 4095), (8, 2, 4999), (4, 21, 9001), (9, 70, 33), (40, 300, 201), (130, 72, 63)])
+def test_rows_at_any_address(m, n, k, dtype):
+    """Operands whose rows start anywhere, with NaN all around them, give the bits that aligned copies give."""
+    g = gen(m * n + k)
+
+    def placed(t, front, pitch):
+        rows, cols = t.shape
+        mem = torch.full((front + (rows - 1) * pitch + cols,), float("nan"), device="cuda", dtype=dtype)
+        view = mem.as_strided((rows, cols), (pitch, 1), front)
+        view.copy_(t)
+        return view
+
+    x, w, wu = normal(g, m, k, dtype), normal(g, n, k, dtype, 0.1), normal(g, n, k, dtype, 0.1)
+    res, dy, z = normal(g, m, n, dtype), normal(g, m, n, dtype), normal(g, m, n, dtype)
+    new = lambda *shape: torch.full(shape, 7.0, device="cuda", dtype=dtype)
+
+    def run(x, w, wu, res, dy, z):
+        y, h, dx, dw, db = new(m, n), new(m, n), new(m, k), new(n, k), new(n)
+        eas.ops.linear(x, w, y, residual=res, act="silu")
+        eas.ops.gated(x, w, wu, h)
+        eas.ops.linear_backward(dy, x, w, dx=dx, dw=dw, dbias=db, act="gelu", pre=z)
+        dx2, dg, du, db2 = new(m, k), new(n, k), new(n, k), new(n)
+        eas.ops.gated_backward(dy, x, w, wu, z, res, dx=dx2, dw_gate=dg, dw_up=du)
+        eas.ops.linear_backward(dy, x, w, dbias=db2)
+        return y, h, dx, dw, db, dx2, dg, du, db2
+
+    pitch_k, pitch_n = -(-k // 8) * 8, -(-n // 8) * 8
+    want = run(*(placed(t, 0, p) for t, p in ((x, pitch_k), (w, pitch_k), (wu, pitch_k), (res, pitch_n), (dy, pitch_n),
+                                              (z, pitch_n))))
+    assert all(t.isfinite().all() for t in want)
+    for front, extra in ((1, 0), (7, 1), (4, 3), (3, 6), (0, 1), (6, 13)):
+        odd = [placed(t, (front + 3 * i) % 8, t.shape[1] + extra + i) for i, t in enumerate((x, w, wu, res, dy, z))]
+        for a, b in zip(run(*odd), want):
+            assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("name", ACTS)
 @pytest.mark.parametrize("m", [2, 40, 300])
 def test_special_values_stay_in_their_columns(m, name):
