@@ -24,6 +24,57 @@ namespace {
 using namespace dense;
 
 // ---------------------------------------------------------------------------
+// copies of operands whose rows TMA cannot read in place
+// ---------------------------------------------------------------------------
+//
+// Up to three matrices, in rows of a multiple of 8 elements (zeros past the end), 8 elements per thread,
+// beside the elementwise half of a backward pass or in a launch of their own.  Bound by HBM: 97 MB of
+// 3648 x 6675 weights take 39 us, 5 TB/s.  (Loading aligned words and shifting them, as the other
+// kernels do, took as long there and 2 us more on small matrices.)
+
+struct Repitch {
+  struct Matrix {
+    const uint16_t* src;
+    uint16_t* dst;
+    int64_t ld, end;   // groups of this matrix and of those before it
+    int cols, groups;  // groups of 8 per padded row
+  } m[3];
+  int count;
+};
+
+__device__ __forceinline__ void repitch(const Repitch& p, int64_t block, int64_t blocks) {
+  const int64_t total = p.m[p.count - 1].end;
+  const bool small = total < (1ll << 31);  // a division of 32 bits
+  for (int64_t i = block * 256 + threadIdx.x; i < total; i += blocks * 256) {
+    const int k = i < p.m[0].end ? 0 : i < p.m[1].end ? 1 : 2;
+    const Repitch::Matrix& m = p.m[k];
+    const int64_t g = i - (k ? p.m[k - 1].end : 0);
+    const int64_t r = small ? (uint32_t)g / (uint32_t)m.groups : g / m.groups;
+    const int c = (int)(g - r * m.groups) * 8;
+    const uint16_t* src = m.src + r * m.ld + c;
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t lo = c + 2 * j < m.cols ? __ldg(src + 2 * j) : 0;
+      const uint32_t hi = c + 2 * j + 1 < m.cols ? __ldg(src + 2 * j + 1) : 0;
+      w[j] = lo | (hi << 16);
+    }
+    *reinterpret_cast<uint4*>(m.dst + g * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+int repitch_blocks(const Repitch& p) {
+  if (!p.count) return 0;
+  const int64_t blocks = (p.m[p.count - 1].end + 255) / 256;
+  return (int)(blocks < 24 * 148 ? blocks : 24 * 148);
+}
+
+__global__ void __launch_bounds__(256) repitch_kernel(const __grid_constant__ Repitch p) {
+  grid_order();
+  repitch(p, blockIdx.x, gridDim.x);
+}
+
+// ---------------------------------------------------------------------------
 // the elementwise half of the backward pass
 // ---------------------------------------------------------------------------
 //
@@ -48,6 +99,8 @@ struct ActGrad {
   float* partial;   // [row blocks][N] sums of dz, or null
   int64_t lddy, ldg, ldu, ldo;
   int M, N, rows_per_block;
+  int row_blocks;   // the blocks behind those make copies
+  Repitch copies;
   int act;
   bool bf16;
 };
@@ -77,6 +130,12 @@ __device__ __forceinline__ void store8(uint16_t* p, int n, const float (&v)[8]) 
 template <bool GATED, bool BF16, bool VEC>
 __global__ void __launch_bounds__(256) act_grad_kernel(const __grid_constant__ ActGrad p) {
   __shared__ float sums[8][32][9];
+  if ((int)blockIdx.y >= p.row_blocks) {
+    grid_order();
+    repitch(p.copies, (int64_t)(blockIdx.y - p.row_blocks) * gridDim.x + blockIdx.x,
+            (int64_t)(gridDim.y - p.row_blocks) * gridDim.x);
+    return;
+  }
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int n0 = (blockIdx.x * 32 + tx) * 8;
   const int cols = p.N - n0;
@@ -169,40 +228,10 @@ int launch_act_grad(ActGrad& g, int blocks, cudaStream_t s, const char* who) {
                                      : reinterpret_cast<const void*>(&act_grad_kernel<GATED, true, false>))
                               : (vec ? reinterpret_cast<const void*>(&act_grad_kernel<GATED, false, true>)
                                      : reinterpret_cast<const void*>(&act_grad_kernel<GATED, false, false>));
-  return dense_launch(kernel, dim3((unsigned)((g.N + 255) / 256), (unsigned)blocks), 0, 256, 0, s, &g, who);
-}
-
-// Copies of operands whose rows TMA cannot read in place, in rows of a multiple of 8 elements (zeros
-// past the end): up to three matrices in one launch (one per row of blocks), 8 elements per thread.  Bound
-// by HBM: 97 MB of 3648 x 6675 weights take 39 us, 5 TB/s.  (Loading aligned words and shifting them,
-// as the other kernels do, took as long there and 2 us more on small matrices.)
-struct Repitch {
-  struct Matrix {
-    const uint16_t* src;
-    uint16_t* dst;
-    int64_t ld;
-    int rows, cols, groups;  // groups of 8 per padded row
-  } m[3];
-  int count;
-};
-
-__global__ void __launch_bounds__(256) repitch_kernel(const __grid_constant__ Repitch p) {
-  grid_order();
-  const Repitch::Matrix& m = p.m[blockIdx.y];
-  const int64_t total = (int64_t)m.rows * m.groups;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / m.groups;
-    const int c = (int)(i - r * m.groups) * 8;
-    const uint16_t* src = m.src + r * m.ld + c;
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t lo = c + 2 * j < m.cols ? __ldg(src + 2 * j) : 0;
-      const uint32_t hi = c + 2 * j + 1 < m.cols ? __ldg(src + 2 * j + 1) : 0;
-      w[j] = lo | (hi << 16);
-    }
-    *reinterpret_cast<uint4*>(m.dst + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
+  const int width = (g.N + 255) / 256;
+  g.row_blocks = blocks;
+  blocks += (repitch_blocks(g.copies) + width - 1) / width;
+  return dense_launch(kernel, dim3((unsigned)width, (unsigned)blocks), 0, 256, 0, s, &g, who);
 }
 
 // Rows per block: enough blocks for 8 per SM, at least 8 rows (one per thread row); with sums at most
@@ -340,18 +369,14 @@ struct Copies {
               uint64_t ld_pad) {
     if (!off) return {u16(src), ld};
     uint16_t* dst = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(scratch) + at);
-    r.m[r.count++] = {u16(src), dst, (int64_t)ld, (int)rows, (int)cols, (int)(ld_pad / 8)};
+    const int groups = (int)(ld_pad / 8);
+    const int64_t before = r.count ? r.m[r.count - 1].end : 0;
+    r.m[r.count++] = {u16(src), dst, (int64_t)ld, before + (int64_t)rows * groups, (int)cols, groups};
     return {dst, ld_pad};
   }
   int launch(cudaStream_t s, const char* who) {
     if (!r.count) return EAS_OK;
-    int64_t most = 0;
-    for (int k = 0; k < r.count; ++k) {
-      const int64_t blocks = ((int64_t)r.m[k].rows * r.m[k].groups + 255) / 256;
-      if (blocks > most) most = blocks;
-    }
-    if (most > 8 * 148) most = 8 * 148;
-    return dense_launch(reinterpret_cast<const void*>(&repitch_kernel), dim3((unsigned)most, (unsigned)r.count), 0, 256, 0, s,
+    return dense_launch(reinterpret_cast<const void*>(&repitch_kernel), dim3((unsigned)repitch_blocks(r)), 0, 256, 0, s,
                         &r, who);
   }
 };
@@ -541,6 +566,9 @@ extern "C" int eas_linear_backward(const eas_linear_backward_args* args, void* s
     if (db && (rc = zero_rows(db, N, 1, N, s, who))) return rc;
     return EAS_OK;
   }
+  Copies copies;
+  const Operand X = dw ? copies.add(x, ldx, M, K, off & kXOff, scratch, sc.x, sc.ldk) : Operand{};
+  const Operand W = dx ? copies.add(w, ldw, N, K, off & kWOff, scratch, sc.w, sc.ldk) : Operand{};
   uint8_t* base = static_cast<uint8_t*>(scratch);
   uint16_t* dz = sc.need_dz ? reinterpret_cast<uint16_t*>(base + sc.dz) : nullptr;
   float* partial = db && !sc.direct ? reinterpret_cast<float*>(base + sc.partial) : nullptr;
@@ -549,13 +577,12 @@ extern "C" int eas_linear_backward(const eas_linear_backward_args* args, void* s
     g.dy = u16(dy), g.g = u16(pre), g.dg = dz, g.partial = partial;
     g.lddy = lddy, g.ldg = ldp, g.ldo = sc.ldn;
     g.M = M, g.N = N, g.rows_per_block = sc.rows, g.act = act, g.bf16 = dtype == kBF16;
+    g.copies = copies.r;
     rc = launch_act_grad<false>(g, sc.blocks, s, who);
-    if (rc) return rc;
+  } else {
+    rc = copies.launch(s, who);
   }
-  Copies copies;
-  const Operand X = dw ? copies.add(x, ldx, M, K, off & kXOff, scratch, sc.x, sc.ldk) : Operand{};
-  const Operand W = dx ? copies.add(w, ldw, N, K, off & kWOff, scratch, sc.w, sc.ldk) : Operand{};
-  if ((rc = copies.launch(s, who))) return rc;
+  if (rc) return rc;
   const Operand DZ = dz ? Operand{dz, sc.ldn} : Operand{u16(dy), lddy};
   DenseColSum sums;
   if (db) {
@@ -601,20 +628,20 @@ extern "C" int eas_gated_backward(const eas_gated_backward_args* args, void* str
     return EAS_OK;
   }
   uint8_t* base = static_cast<uint8_t*>(scratch);
+  const bool dw = outputs & kDw;
+  Copies copies;
+  const Operand X = dw ? copies.add(x, ldx, M, K, off & kXOff, scratch, sc.x, sc.ldk) : Operand{};
+  const Operand G = dx ? copies.add(w_gate, ldwg, N, K, off & kWOff, scratch, sc.w, sc.ldk) : Operand{};
+  const Operand U = dx ? copies.add(w_up, ldwu, N, K, off & kUpOff, scratch, sc.up, sc.ldk) : Operand{};
   uint16_t* dg = reinterpret_cast<uint16_t*>(base + sc.dz);  // need_dz: some output is asked for
   uint16_t* du = reinterpret_cast<uint16_t*>(base + sc.dz2);
   ActGrad g = {};
   g.dy = u16(dh), g.g = u16(gate), g.u = u16(up), g.dg = dg, g.du = du;
   g.lddy = lddh, g.ldg = ldg, g.ldu = ldu, g.ldo = sc.ldn;
   g.M = M, g.N = N, g.rows_per_block = sc.rows, g.act = act, g.bf16 = dtype == kBF16;
+  g.copies = copies.r;
   rc = launch_act_grad<true>(g, sc.blocks, s, who);
   if (rc) return rc;
-  const bool dw = outputs & kDw;
-  Copies copies;
-  const Operand X = dw ? copies.add(x, ldx, M, K, off & kXOff, scratch, sc.x, sc.ldk) : Operand{};
-  const Operand G = dx ? copies.add(w_gate, ldwg, N, K, off & kWOff, scratch, sc.w, sc.ldk) : Operand{};
-  const Operand U = dx ? copies.add(w_up, ldwu, N, K, off & kUpOff, scratch, sc.up, sc.ldk) : Operand{};
-  if ((rc = copies.launch(s, who))) return rc;
   return backward_products(who, 2, {{dg, sc.ldn}, {du, sc.ldn}}, {G, U}, X, dx, lddx, {dw_gate, dw_up},
                            {lddwg, lddwu}, DenseColSum(), M, N, K, dtype, s);
 }
