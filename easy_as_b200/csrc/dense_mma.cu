@@ -282,14 +282,17 @@ __device__ __forceinline__ void add_residual(const Params& p, Boxes& bx, int lan
     for (int j = 0; j < 4; ++j) w[j] = src[j];
   } else {
     uint8_t* box = next_box(bx, lane);
-    const int c = lane & 3, cols = N - n0 - 8 * c;
-    const uint16_t* end = p.residual + (int64_t)(M - 1) * p.ldr + N;
-    Gather8 from[4];
+    const int rows = n0 + lane < N ? min(32, M - m0) : 0;
+    const uint16_t* src = p.residual + (int64_t)m0 * p.ldr + n0 + lane;
+    const ColumnInBox col(box, lane);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      from[i].fetch(p.residual + (int64_t)min(m0 + 8 * i + (lane >> 2), M - 1) * p.ldr + n0 + 8 * c, cols, p.residual, end);
+    for (int r0 = 0; r0 < 32; r0 += 16) {  // 16 loads under way
+      uint16_t h[16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(box_chunk(box, 8 * i + (lane >> 2), c)) = from[i].get();
+      for (int r = 0; r < 16; ++r, src += p.ldr) h[r] = r0 + r < rows ? *src : (uint16_t)0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) *col.at(r0 + r) = h[r];
+    }
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4*>(box_chunk(box, lane, j));
@@ -1025,19 +1028,22 @@ int launch_tile(Params& q, int dev, cudaStream_t s, const char* who) {
 
 using Choice = DenseShape;
 
-// The shape of least estimated time, in microseconds as measured on one B200 at 1.9 GHz (bf16,
-// operands from HBM).  A step is one 64-deep k-block of one CTA or pair.  Over 65 random sizes the choice
-// was the best of all shapes within 5 %, but for eight within 21 (before the last entry's numbers).
-//   pair, 256 x 256        5.5 + rounds x k-blocks x 0.31   (4096^3: 94 us; 512 x 4096 x 4096: 25.3)
-//   one CTA per SM         4.5 + k-blocks x step, step 0.15 (BN 64) or 0.205 (128), 0.115 or 0.155 with
+// The shape of least estimated time, in microseconds on one B200 at 1.9 GHz (operands from HBM).  A step is
+// one 64-deep k-block of one CTA or pair.  The numbers are fitted to 650 random calls of all four operators, and
+// tried on 2000 more, each timed with every shape: the choice takes 1.4 % longer than the best one (two
+// products: 2.1) on geometric average.
+//   pair, 256 x 256        7 + rounds x k-blocks x 0.28   (512 x 4096 x 4096: 25.3)
+//   one CTA per SM         5.4 + k-blocks x step, step 0.125 (BN 64) or 0.215 (128), 0.11 or 0.19 with
 //                          64 rows of A   (64 x 4096 x 4096: 12.3 BN 64, 15.0 BN 128)
-//   two CTAs per SM        4.0 + CTAs per SM x (k-blocks x step + 0.6 or 0.9), step 0.2 or 0.26
-//                          (2048^3: 25.1 BN 64, 17.5 BN 128)
-//   a split over 2 or 4    1.2 or 1.6 more for the exchange, and only while all CTAs are resident at
+//   two CTAs per SM        4.6 + CTAs per SM x (k-blocks x step + 0.7), step 0.2 or 0.3 (2048^3: 25.1
+//                          BN 64, 17.5 BN 128), one product's in whole rounds (gated 736 x 3456 x 4608,
+//                          324 CTAs for 296 places: 82; as pairs 52)
+//   a split over 2 or 4    1.35 or 2.1 more for the exchange, and only while all CTAs are resident at
 //                          once (16 x 4096 x 4096, BN 64: 11.9 whole, 10.2 split in 2, 17.9 in 8;
 //                          184 x 560 x 1504: 6.9 whole, 5.9 split in 4)
 //   two products           a few long sums beside many short ones are split over up to 8 CTAs (dx beside dW
-//                          of 7 x 6215 x 795: 98 k-blocks beside 637 tiles of one; whole, they took 46)
+//                          of 7 x 6215 x 795: 98 k-blocks beside 637 tiles of one; whole, they took 46),
+//                          where each CTA also holds its place for 1.8 while it waits for the others
 //   column sums            3 more with the pair kernel, which leaves them to a launch of their own
 Choice choose(const DenseProduct* p, int count, bool sums, int sms) {
   const int pairs = sms / 2 > 0 ? sms / 2 : 1;
@@ -1057,7 +1063,7 @@ Choice choose(const DenseProduct* p, int count, bool sums, int sms) {
   Choice best = {0, {1, 1}, 128, false};
   double best_us;
   if (count == 1) {
-    best_us = 5.5 + (double)((tiles_of(0, 256, 256) + pairs - 1) / pairs) * kb[0] * 0.31;
+    best_us = 7 + (double)((tiles_of(0, 256, 256) + pairs - 1) / pairs) * kb[0] * 0.28;
   } else {  // the jobs (the longer tiles first) fill one another's last rounds
     double steps = 0;
     int64_t tiles = 0;
@@ -1066,21 +1072,21 @@ Choice choose(const DenseProduct* p, int count, bool sums, int sms) {
       steps += (double)tiles_of(i, 256, 256) * kb[i];
     }
     steps = tiles <= pairs ? kb[0] : steps / pairs + 0.5 * least_kb;
-    best_us = 5.5 + (steps > kb[0] ? steps : kb[0]) * 0.31;
+    best_us = 7 + (steps > kb[0] ? steps : kb[0]) * 0.28;
   }
   if (sums) best_us += 3;
   const int64_t most_split = (int64_t)sms * 7 / 8;
   for (int bn = 64; bn <= 128; bn += 64) {
     int64_t tiles[2] = {0, 0};
     double work = 0;  // steps of all tiles, with what a tile costs beside its steps
-    const double shared = bn == 64 ? 0.2 : 0.26, tile_us = bn == 64 ? 0.6 : 0.9;
+    const double shared = bn == 64 ? 0.2 : 0.3, tile_us = 0.7;
     for (int i = 0; i < count; ++i) {
       tiles[i] = tiles_of(i, 128, bn);
       work += (double)tiles[i] * (kb[i] * shared + tile_us);
     }
     const bool few = most_rows <= 64 && !a_mn;
-    const double step = bn == 64 ? (few ? 0.115 : 0.15) : (few ? 0.155 : 0.205);
-    auto exchange = [](int split) { return split == 1 ? 0 : split == 2 ? 1.2 : split == 4 ? 1.6 : 2.2; };
+    const double step = bn == 64 ? (few ? 0.11 : 0.125) : (few ? 0.19 : 0.215);
+    auto exchange = [](int split) { return split == 1 ? 0 : split == 2 ? 1.35 : 2.1; };
     for (int s0 = 1; s0 <= 8; s0 *= 2) {
       for (int s1 = 1; s1 <= (count > 1 ? s0 : 1); s1 *= 2) {
         const int64_t ctas = tiles[0] * s0 + tiles[1] * s1;
@@ -1092,13 +1098,18 @@ Choice choose(const DenseProduct* p, int count, bool sums, int sms) {
           if (few) c.ar = 64;
           const double t0 = (double)((kb[0] + s0 - 1) / s0) * step + exchange(s0);
           const double t1 = (double)((kb[1] + s1 - 1) / s1) * step + exchange(s1);
-          us = 4.5 + (t0 > t1 ? t0 : t1);
+          us = 5.4 + (t0 > t1 ? t0 : t1);
         } else {
           if (s1 > 1 || (s0 > 1 && count == 1)) continue;
           // the longer tiles beside another, and all work spread over the SMs
-          const double t0 = (double)((kb[0] + s0 - 1) / s0) * 1.8 * shared + 1.8 * tile_us + exchange(s0);
-          const double all = (work + (double)tiles[0] * s0 * exchange(s0)) / sms;
-          us = 4.0 + (all > t0 ? all : t0);
+          const double meet = s0 == 1 ? 0 : s0 == 2 ? 2.2 : s0 == 4 ? 3.0 : 3.3;
+          const double t0 = (double)((kb[0] + s0 - 1) / s0) * 1.1 * shared + 1.1 * tile_us + meet;
+          double all = (work + (double)tiles[0] * (s0 * meet + (s0 - 1) * 1.8)) / sms;
+          if (count == 1) {  // like tiles start and end together: whole rounds, two per SM
+            const int64_t rounds = (ctas + 2 * sms - 1) / (2 * sms);
+            if (rounds > 1) all = (double)rounds * 2 * work / ctas;
+          }
+          us = 4.6 + (all > t0 ? all : t0);
         }
         if (us < best_us) best = c, best_us = us;
       }
@@ -1123,7 +1134,7 @@ int launch_choice(const Choice& c, Params& q, int dev, cudaStream_t s, const cha
   return c.deep ? launch_tile<128, 128, true, MODE>(q, dev, s, who) : launch_tile<128, 128, false, MODE>(q, dev, s, who);
 }
 
-// The epilogue waits for a whole sum (0.31 us per k-block), with the budget of all waits, about 2 s.
+// The epilogue waits for a whole sum (0.3 us per k-block), with the budget of all waits, about 2 s.
 constexpr int64_t kMostSteps = 1 << 22;
 
 int64_t steps_of(const DenseProduct& p) { return (int64_t)((p.K + kBK - 1) / kBK) * p.terms; }

@@ -14,7 +14,9 @@
 //
 // Rows that do not start on 16 bytes are copied as the aligned words that hold them, one more per row
 // and piece, and shifted into place on their way from the queue to the instruction (4096 x 4096, one
-// row: 7.8 us; K = 4095: 11.0, and 15.2 with 8 rows; loaded value by value they took 24).
+// row: 7.8 us; K = 4095: 11.0, and 15.2 with 8 rows; loaded value by value they take 24).  Of less than
+// 4 MB of weights they are loaded value by value straight into registers: that starts 2 us sooner (576 x
+// 123 gated: 2.8 us, against 4.5; 3912 x 1000: 6.7, against 7.1; gated 3272 x 1408: 16.1, against 14.1).
 //
 // Two blocks of 8 warps stay on each SM (or one of 16, where x needs the room), each with an equal
 // share of W's rows (N / 296 of them, give or take one, so that no SM has more to read than another),
@@ -63,6 +65,17 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// 8 values of a row, of which `n` are left: zeros past them.
+__device__ __forceinline__ uint4 load8(const uint16_t* p, int n) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t lo = 2 * j < n ? __ldg(p + 2 * j) : 0, hi = 2 * j + 1 < n ? __ldg(p + 2 * j + 1) : 0;
+    w[j] = lo | (hi << 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 __device__ __forceinline__ void copy16(uint32_t dst, const uint16_t* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -81,15 +94,18 @@ __device__ __forceinline__ uint4 lds128(uint32_t at) {
 
 constexpr int kPiece = 64;       // values of K per row and piece
 
+// How W comes: by words of its rows, which start on 16 bytes; by words that are shifted; value by value.
+enum Way { kWords, kShifted, kValues };
+
 // W warps per block, and of x in shared memory: two blocks of 8 warps per SM, or one of 16 with twice
-// the room for x.  VEC: rows of x and W start on 16 bytes.  A slot holds a piece of 16 rows of W: 8 words
-// each, and behind them (not VEC) the 16 rows' ninth ones.
-template <int W, bool VEC>
+// the room for x.  A slot holds a piece of 16 rows of W: 8 words
+// each, and behind them (shifted) the 16 rows' ninth ones.
+template <int W, Way WAY>
 struct Shape {
-  static constexpr int kSlot = 16 * 128 + (VEC ? 0 : 16 * 16);
-  static constexpr int kPieces = VEC ? 4 : 3;      // per warp
+  static constexpr int kSlot = 16 * 128 + (WAY == kShifted ? 16 * 16 : 0);
+  static constexpr int kPieces = WAY == kWords ? 4 : 3;      // per warp
   static constexpr int kDepth = kPieces - 1;       // under way while one is consumed
-  static constexpr int kQueue = W * kPieces * kSlot;  // 64 or 54 KB, or twice that
+  static constexpr int kQueue = WAY == kValues ? 0 : W * kPieces * kSlot;  // 64 or 54 KB, or twice that
 };
 
 template <int W>
@@ -99,12 +115,13 @@ constexpr int kMostX = W == 8 ? 40960 : 81920;
 // quarter warp read different banks.
 __host__ __device__ constexpr int64_t x_pitch(int64_t K) { return (K + kPiece - 1) / kPiece * (2 * kPiece) + 64; }
 
-template <int kWarps, bool GATED, bool VEC, bool BF16>
+template <int kWarps, bool GATED, Way WAY, bool BF16>
 __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
     dense_rows_kernel(const __grid_constant__ RowsParams p) {
   constexpr int kTile = GATED ? 8 : 16;  // outputs; always 16 rows of W
   constexpr int kRows = kDenseRows, kCols = 16;
-  using Q = Shape<kWarps, VEC>;
+  constexpr bool VEC = WAY == kWords;
+  using Q = Shape<kWarps, WAY>;
   constexpr int kSlot = Q::kSlot, kDepth = Q::kDepth;
   extern __shared__ __align__(128) uint8_t queue[];
   __shared__ float part[2][kWarps][kRows][kCols + 1];  // tiles take turns
@@ -124,7 +141,7 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
   // Chunk c of a row lies at place c ^ 4 (row & 1), so that two rows' quads read different banks.
   // Rows past the tile are not copied: whatever their place in the queue holds reaches only sums
   // that nobody looks at.
-  // (Not VEC: 9 words of each row, in the order of the lanes.)
+  // (Shifted: 9 words of each row, in the order of the lanes.)
   constexpr int kCopies = VEC ? 4 : 5;
   auto copy_row = [&](int i) { return VEC ? (lane >> 3) + 4 * i : (lane + 32 * i) / 9; };
   auto copy_word = [&](int i) { return VEC ? lane & 7 : (lane + 32 * i) % 9; };
@@ -136,8 +153,9 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
   };
   const uint16_t* w[kCopies];
   int have = 0;
-  int left_of[kCopies];  // (not VEC) values of K behind the word's first
+  int left_of[kCopies];  // (shifted) values of K behind the word's first
   auto aim = [&](int n0, int n1) {
+    if (WAY == kValues) return;
     have = 0;
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
@@ -156,7 +174,7 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
 
   const uint32_t mine = tc::smem_u32(queue) + warp * (Q::kPieces * kSlot);
   const uint32_t take = mine + word_at(g, t);  // v = 1: ^ 64; row g + 8: + 1024
-  // (not VEC) the words behind those, of rows g and g + 8
+  // (shifted) the words behind those, of rows g and g + 8
   const uint32_t next0 = mine + word_at(g, t + 1), next1[2] = {mine + word_at(g, t + 5), mine + word_at(g + 8, t + 5)};
   const int64_t pitch = x_pitch(p.K);
   const uint32_t xs = tc::smem_u32(queue) + Q::kQueue;
@@ -164,7 +182,7 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
   int in_tile = 0, in_k = first, in_slot = 0, out_slot = 0;
   if (tiles > 0) aim(tile_row(0), tile_row(1));
   auto issue = [&]() {  // always one group, empty past the end: the waits count groups
-    if (in_tile < tiles && in_k < p.K) {
+    if (WAY != kValues && in_tile < tiles && in_k < p.K) {
       const uint32_t at = mine + in_slot * kSlot;
       if constexpr (!VEC) {
 #pragma unroll
@@ -200,53 +218,66 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  // x once per block: from every warp's piece it would be read by all SMs at the same time, and
-  // its few lines of L2 were what the kernel waited for (4 rows: 44 us where one took 34)
-  const int words = (int)((pitch - 64) / 16);
-  for (int e = threadIdx.x; e < p.M * words; e += kWarps * 32) {
-    const int r = e / words, c = e % words;
-    const int left = p.K - 8 * c;
-    const uint16_t* src = p.x + (int64_t)r * p.ldx + (left > 0 ? 8 * c : 0);
-    const uint32_t dst = xs + (uint32_t)(r * pitch) + 16 * c;
-    if constexpr (VEC) {
-      copy8(dst, src, left);
-    } else {
-      Gather8 from;
-      from.fetch(src, left, p.x, p.x_end);
-      const uint4 v = from.get();
-      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                   : "memory");
+  if constexpr (WAY != kValues) {
+    // x once per block: from every warp's piece it would be read by all SMs at the same time, and
+    // its few lines of L2 were what the kernel waited for (4 rows: 44 us where one took 34)
+    const int words = (int)((pitch - 64) / 16);
+    for (int e = threadIdx.x; e < p.M * words; e += kWarps * 32) {
+      const int r = e / words, c = e % words;
+      const int left = p.K - 8 * c;
+      const uint16_t* src = p.x + (int64_t)r * p.ldx + (left > 0 ? 8 * c : 0);
+      const uint32_t dst = xs + (uint32_t)(r * pitch) + 16 * c;
+      if constexpr (VEC) {
+        copy8(dst, src, left);
+      } else {
+        Gather8 from;
+        from.fetch(src, left, p.x, p.x_end);
+        const uint4 v = from.get();
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                     : "memory");
+      }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    for (int i = 0; i < kDepth; ++i) issue();
+    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth) : "memory");
+    __syncthreads();
   }
-  asm volatile("cp.async.commit_group;" ::: "memory");
-  for (int i = 0; i < kDepth; ++i) issue();
-  asm volatile("cp.async.wait_group %0;" ::"n"(kDepth) : "memory");
-  __syncthreads();
 
   for (int j = 0; j < tiles; ++j) {
     const int n0 = tile_row(j), width = tile_row(j + 1) - n0;
     int shift[2];  // of rows g and g + 8
 #pragma unroll
     for (int i = 0; i < 2; ++i) shift[i] = lag(w_row(g + 8 * i, n0, n0 + width));
+    const uint16_t* row[2] = {w_row(g, n0, n0 + width) + 8 * t, w_row(g + 8, n0, n0 + width) + 8 * t};
     float acc[4] = {};
     for (int k = first; k < p.K; k += stride) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
-      __syncwarp();  // the piece is here, and everyone has read the one before it
-      issue();
-      const uint32_t slot = out_slot * kSlot;
-      out_slot = out_slot == kDepth ? 0 : out_slot + 1;
+      uint32_t slot = 0;
+      if constexpr (WAY != kValues) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+        __syncwarp();  // the piece is here, and everyone has read the one before it
+        issue();
+        slot = out_slot * kSlot;
+        out_slot = out_slot == kDepth ? 0 : out_slot + 1;
+      }
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
         uint4 a[2];
-        const uint4 b = lds128(xmine + 2 * k + v * 64);
-        a[0] = lds128((take + slot) ^ (v * 64));
-        a[1] = lds128(((take + slot) ^ (v * 64)) + 1024);
-        if constexpr (!VEC) {
+        uint4 b;
+        const int left = p.K - k - 32 * v - 8 * t;
+        if constexpr (WAY == kValues) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) a[i] = load8(row[i] + k + 32 * v, left);
+          b = load8(p.x + (int64_t)xrow * p.ldx + 8 * t + k + 32 * v, left);
+        } else {
+          b = lds128(xmine + 2 * k + v * 64);
+          a[0] = lds128((take + slot) ^ (v * 64));
+          a[1] = lds128(((take + slot) ^ (v * 64)) + 1024);
+        }
+        if constexpr (WAY == kShifted) {
           const uint4 c0 = lds128((v ? next1[0] : next0) + slot), c1 = lds128((v ? next1[1] : next0 + 1024) + slot);
           a[0] = shift8(a[0], c0, shift[0]);
           a[1] = shift8(a[1], c1, shift[1]);
           if (k + kPiece > p.K) {  // what lies behind the row's end
-            const int left = p.K - k - 32 * v - 8 * t;
             a[0] = first8(a[0], left);
             a[1] = first8(a[1], left);
           }
@@ -306,6 +337,9 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
   }
 }
 
+// Weights that are shifted rather than loaded value by value, where their rows do not start on 16 bytes.
+constexpr int64_t kShiftFrom = 2 << 20;
+
 bool aligned16(const void* p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld & 7) == 0; }
 
 // CTAs that split K: two where each block's share of the rows would fill less than half a tile and
@@ -315,18 +349,14 @@ int choose_split(const DenseProduct& p, int blocks, int warps) {
   return (int64_t)p.N < (int64_t)blocks * tile / 2 && p.K >= 8 * kPiece * warps ? 2 : 1;
 }
 
-template <int W, bool GATED, bool BF16>
-int launch_rows(const DenseProduct& p, RowsParams& q, bool vec, int dev, cudaStream_t s, const char* who) {
+template <int W, bool GATED, Way WAY, bool BF16>
+int launch_rows(const DenseProduct& p, RowsParams& q, int dev, cudaStream_t s, const char* who) {
   static bool ready[64] = {false};
-  const void* fast = reinterpret_cast<const void*>(&dense_rows_kernel<W, GATED, true, BF16>);
-  const void* slow = reinterpret_cast<const void*>(&dense_rows_kernel<W, GATED, false, BF16>);
-  if (!ready[dev & 63]) {
-    auto allow = [&](const void* kernel, int bytes) {
-      return eas_cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), who,
-                            EAS_ERR_LAUNCH);
-    };
-    int rc = allow(fast, Shape<W, true>::kQueue + kMostX<W>);
-    if (!rc) rc = allow(slow, Shape<W, false>::kQueue + kMostX<W>);
+  const void* kernel = reinterpret_cast<const void*>(&dense_rows_kernel<W, GATED, WAY, BF16>);
+  constexpr int kQueue = Shape<W, WAY>::kQueue;
+  if (WAY != kValues && !ready[dev & 63]) {
+    int rc = eas_cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kQueue + kMostX<W>),
+                            who, EAS_ERR_LAUNCH);
     if (rc) return rc;
     ready[dev & 63] = true;
   }
@@ -335,17 +365,15 @@ int launch_rows(const DenseProduct& p, RowsParams& q, bool vec, int dev, cudaStr
   // no block without rows; four rows a block or more, where there are few
   int groups = resident / q.split;
   if (groups > (p.N + 3) / 4) groups = (p.N + 3) / 4;
-  return dense_launch(vec ? fast : slow, dim3(groups * q.split), q.split > 1 ? q.split : 0, W * 32,
-                      (vec ? Shape<W, true>::kQueue : Shape<W, false>::kQueue) + q.M * (int)x_pitch(q.K), s, &q, who);
+  return dense_launch(kernel, dim3(groups * q.split), q.split > 1 ? q.split : 0, W * 32,
+                      WAY == kValues ? 0 : kQueue + q.M * (int)x_pitch(q.K), s, &q, who);
 }
 
-template <int W>
-int launch_rows(const DenseProduct& p, RowsParams& q, bool vec, int dev, cudaStream_t s, const char* who) {
+template <int W, Way WAY>
+int launch_rows(const DenseProduct& p, RowsParams& q, int dev, cudaStream_t s, const char* who) {
   if (p.bf16)
-    return p.gated ? launch_rows<W, true, true>(p, q, vec, dev, s, who)
-                   : launch_rows<W, false, true>(p, q, vec, dev, s, who);
-  return p.gated ? launch_rows<W, true, false>(p, q, vec, dev, s, who)
-                 : launch_rows<W, false, false>(p, q, vec, dev, s, who);
+    return p.gated ? launch_rows<W, true, WAY, true>(p, q, dev, s, who) : launch_rows<W, false, WAY, true>(p, q, dev, s, who);
+  return p.gated ? launch_rows<W, true, WAY, false>(p, q, dev, s, who) : launch_rows<W, false, WAY, false>(p, q, dev, s, who);
 }
 
 }  // namespace
@@ -371,6 +399,9 @@ int dense_rows(const DenseProduct& p, cudaStream_t stream, const char* who) {
   for (int i = 0; i < (p.gated ? 2 : 1); ++i) q.w_end[i] = q.w[i] + (q.N - 1) * q.ldw[i] + q.K;
   const bool vec = aligned16(p.a[0], p.M > 1 ? p.lda[0] : 0) && aligned16(p.b[0], p.N > 1 ? p.ldb[0] : 0) &&
                    (!p.gated || aligned16(p.b[1], p.N > 1 ? p.ldb[1] : 0));
-  return p.M * x_pitch(p.K) <= kMostX<8> ? launch_rows<8>(p, q, vec, dev, stream, who)
-                                                : launch_rows<16>(p, q, vec, dev, stream, who);
+  const bool narrow = p.M * x_pitch(p.K) <= kMostX<8>;
+  if (vec)
+    return narrow ? launch_rows<8, kWords>(p, q, dev, stream, who) : launch_rows<16, kWords>(p, q, dev, stream, who);
+  if ((int64_t)p.N * p.K * (p.gated ? 2 : 1) < kShiftFrom) return launch_rows<8, kValues>(p, q, dev, stream, who);
+  return narrow ? launch_rows<8, kShifted>(p, q, dev, stream, who) : launch_rows<16, kShifted>(p, q, dev, stream, who);
 }

@@ -17,7 +17,7 @@ VARIANTS = [(141, 9525, 1), (11, 2053, 2908), (5331, 1, 1863), (68, 1, 1601), (9
             (2182, 837, 1), (1755, 785, 1), (1, 1, 9666), (70, 1, 8776), (1, 1722, 4343), (3387, 1292, 72),
             (1, 1355, 2095), (1720, 1511, 66), (2247, 861, 66), (13, 2500, 1355), (1723, 515, 1),
             (2701, 1202, 51), (7, 6215, 795), (177, 7941, 170),
-            (3503, 160, 408), (1, 64, 50000)]
+            (3503, 160, 408), (1, 64, 50000), (6944, 76, 3), (676, 535, 9884), (19, 9943, 2044)]
 
 LINEAR, GATED, LINEAR_BACKWARD, GATED_BACKWARD = range(4)
 DX, DW, DB = 1, 2, 4

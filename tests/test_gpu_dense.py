@@ -287,7 +287,8 @@ def test_special_values_stay_in_their_rows(m):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 5, 7), (1, 300, 64), (2, 17, 65), (3, 70, 1025), (5, 4099, 130), (7, 33, 127),
-                                   (8, 600, 4095), (8, 2, 4999), (4, 21, 9001), (9, 70, 33), (40, 300, 201), (130, 72, 63)])
+                                   (8, 600, 4095), (8, 2, 4999), (4, 21, 9001), (3, 2100, 1025), (1, 33000, 65),
+                                   (2, 520, 4100), (9, 70, 33), (40, 300, 201), (130, 72, 63)])
 def test_rows_at_any_address(m, n, k, dtype):
     """Operands whose rows start anywhere, with NaN all around them, give the bits that aligned copies give."""
     g = gen(m * n + k)
