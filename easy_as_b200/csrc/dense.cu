@@ -55,8 +55,8 @@ __device__ __forceinline__ void repitch(const Repitch& p, int64_t block, int64_t
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t lo = c + 2 * j < m.cols ? __ldg(src + 2 * j) : 0;
-      const uint32_t hi = c + 2 * j + 1 < m.cols ? __ldg(src + 2 * j + 1) : 0;
+      const uint32_t lo = c + 2 * j < m.cols ? src[2 * j] : 0;
+      const uint32_t hi = c + 2 * j + 1 < m.cols ? src[2 * j + 1] : 0;
       w[j] = lo | (hi << 16);
     }
     *reinterpret_cast<uint4*>(m.dst + g * 8) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -180,9 +180,9 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const __grid_constant__ A
                        *pu = GATED ? p.u + m * p.ldu + n0 : nullptr;
         uint4 wd, wg, wu;
         auto fetch = [&]() {
-          wd = __ldg(reinterpret_cast<const uint4*>(pd));
-          if (kG) wg = __ldg(reinterpret_cast<const uint4*>(pg));
-          if (GATED) wu = __ldg(reinterpret_cast<const uint4*>(pu));
+          wd = *reinterpret_cast<const uint4*>(pd);
+          if (kG) wg = *reinterpret_cast<const uint4*>(pg);
+          if (GATED) wu = *reinterpret_cast<const uint4*>(pu);
           pd += sd, pg += sg, pu += su;
         };
         if (m < r1) fetch();

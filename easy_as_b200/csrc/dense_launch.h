@@ -17,7 +17,9 @@ inline bool dense_pdl_on() {
 }
 
 // The grid before this one in the stream may still be running: nothing of global memory is touched
-// before it has finished.  The next grid may be set up meanwhile, and waits in the same place.
+// before it has finished.  The next grid may be set up meanwhile, and waits in the same place.  What comes
+// behind it reads by plain loads: read-only ones (__ldg) promise that nobody writes while the kernel runs,
+// which the grid before may do, and could be moved before the wait.
 __device__ __forceinline__ void grid_order() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");

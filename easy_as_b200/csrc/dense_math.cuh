@@ -189,13 +189,13 @@ struct Gather8 {
     const bool two = s + min(n, 8) > 8;
     inside = word >= lo && word + (two ? 16 : 8) <= hi;
     a = b = make_uint4(0, 0, 0, 0);
-    if (inside && n > 0) a = __ldg(reinterpret_cast<const uint4*>(word));
-    if (inside && two) b = __ldg(reinterpret_cast<const uint4*>(word) + 1);
+    if (inside && n > 0) a = *reinterpret_cast<const uint4*>(word);
+    if (inside && two) b = reinterpret_cast<const uint4*>(word)[1];
   }
   __device__ __forceinline__ uint4 get() const {
     uint4 v = shift8(a, b, s);
     if (!inside) {
-      auto one = [&](int j) { return j < n ? (uint32_t)__ldg(p + j) : 0u; };
+      auto one = [&](int j) { return j < n ? (uint32_t)p[j] : 0u; };
       v = make_uint4(one(0) | one(1) << 16, one(2) | one(3) << 16, one(4) | one(5) << 16, one(6) | one(7) << 16);
     }
     return first8(v, n);

@@ -70,7 +70,7 @@ __device__ __forceinline__ uint4 load8(const uint16_t* p, int n) {
   uint32_t w[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t lo = 2 * j < n ? __ldg(p + 2 * j) : 0, hi = 2 * j + 1 < n ? __ldg(p + 2 * j + 1) : 0;
+    const uint32_t lo = 2 * j < n ? p[2 * j] : 0, hi = 2 * j + 1 < n ? p[2 * j + 1] : 0;
     w[j] = lo | (hi << 16);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);

@@ -265,3 +265,19 @@ def test_scratch_query_checks_its_arguments():
     assert lib.eas_dense_scratch(0, 1, 0, 1, 0, 0, 0, ctypes.byref(need)) == cuda_ext.EAS_ERR_VALUE
     assert lib.eas_dense_scratch(0, 1, 1, 1, 0, 0, 0, None) == cuda_ext.EAS_ERR_VALUE
     assert lib.eas_dense_scratch(2, 0, 1, 1, 0, 7, 15, ctypes.byref(need)) == 0 and need.value == 0
+
+
+def test_kernels_read_by_plain_loads():
+    """The grid before may write what a dense kernel reads while that one is being set up: its loads stay behind
+    the wait, and are no read-only ones."""
+    from pathlib import Path
+
+    import easy_as_b200
+
+    sources = sorted((Path(easy_as_b200.__file__).parent / "csrc").glob("dense*.cu*"))
+    assert len(sources) >= 3
+    for path in sources:
+        text = path.read_text()
+        assert "__ldg(" not in text and "ld.global.nc" not in text and "__restrict__" not in text, path.name
+        for body in text.split("__global__ void")[1:]:
+            assert "grid_order();" in body, path.name
