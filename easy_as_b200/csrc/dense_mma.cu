@@ -196,6 +196,7 @@ __device__ __forceinline__ void settle() {
   const long long t0 = clock64();
   while (clock64() - t0 < 4000000) {
   }
+  __syncwarp();
 }
 
 // ---------------------------------------------------------------------------
@@ -759,6 +760,7 @@ __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == 1) {
+    __syncwarp();  // its first lane was elsewhere
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(BN)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");

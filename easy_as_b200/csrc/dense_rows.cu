@@ -284,6 +284,7 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
         }
         const uint32_t a0[4] = {a[0].x, a[1].x, a[0].y, a[1].y};
         const uint32_t a1[4] = {a[0].z, a[1].z, a[0].w, a[1].w};
+        __syncwarp();  // the copies and loads above may have split the warp, and the instruction is .aligned
         mma_16816<BF16>(acc, a0, b.x, b.y);
         mma_16816<BF16>(acc, a1, b.z, b.w);
       }
