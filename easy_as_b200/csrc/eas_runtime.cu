@@ -208,6 +208,13 @@ extern "C" int eas_set_device(int dev) {
   return EAS_OK;
 }
 
+extern "C" int eas_get_device(int* dev) {
+  if (!dev) return eas_fail(EAS_ERR_VALUE, "eas_get_device: null pointer");
+  int rc = eas_driver_init();
+  if (rc) return rc;
+  return eas_cuda_check(cudaGetDevice(dev), "cudaGetDevice", EAS_ERR_UNAVAILABLE);
+}
+
 extern "C" int eas_device_capability(int dev, int* major, int* minor) {
   int rc = eas_driver_init();
   if (rc) return rc;

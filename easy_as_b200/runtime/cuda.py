@@ -29,7 +29,6 @@ import hashlib
 import math
 import os
 import struct
-import sys
 from collections import deque
 from contextlib import nullcontext
 from pathlib import Path
@@ -295,6 +294,21 @@ class _Bounce:
             self.host_ptr = 0
             self.view = None
         self.dev.free()
+
+
+class _OnDevice:
+    """``device`` is current inside, ``before`` again behind it."""
+
+    __slots__ = ("lib", "device", "before")
+
+    def __init__(self, lib: Any, device: int, before: int):
+        self.lib, self.device, self.before = lib, device, before
+
+    def __enter__(self) -> None:
+        cuda_ext.check(self.lib.eas_set_device(self.device), "set_device")
+
+    def __exit__(self, *_exc: Any) -> None:
+        cuda_ext.check(self.lib.eas_set_device(self.before), "set_device")
 
 
 class CudaRuntime:
@@ -807,13 +821,16 @@ class CudaRuntime:
             return
         self._track(keep, stream, device)
 
-    @staticmethod
-    def on_device(device: int) -> Any:
-        """Context in which ``device`` is current (nothing to do when it is, or without torch)."""
-        t = sys.modules.get("torch")
-        if t is not None and t.cuda.is_initialized() and t.cuda.current_device() != device:
-            return t.cuda.device(device)
-        return _NO_CONTEXT
+    def on_device(self, device: int) -> Any:
+        """Context in which ``device`` is the library's current device, which stream 0 belongs to and an
+        event is created on (nothing to do when it is already)."""
+        lib = self.lib()
+        get = getattr(lib, "eas_get_device", None)
+        if get is None:   # a stand-in for the library that knows one device
+            return _NO_CONTEXT
+        cur = cuda_ext.ctypes.c_int(-1)
+        cuda_ext.check(get(cuda_ext.ctypes.byref(cur)), "get_device")
+        return _NO_CONTEXT if cur.value == device else _OnDevice(lib, device, cur.value)
 
     # -- prepared repeated launches (Kernel.__call__ fast path) ------------------------
     def fast_prepare(self, ck: Any, runtime_args: Mapping[str, Any], opts: Mapping[str, Any],

@@ -40,6 +40,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "eas_is_available": (_int, []),
     "eas_device_count": (_int, [_PINT]),
     "eas_set_device": (_int, [_int]),
+    "eas_get_device": (_int, [_PINT]),
     "eas_device_capability": (_int, [_int, _PINT, _PINT]),
     "eas_versions": (_int, [_PINT, _PINT]),
     "eas_compile": (_int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(ctypes.c_char_p), _int,

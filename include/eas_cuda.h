@@ -55,6 +55,8 @@ int eas_device_count(int* count);
 
 /* Make `dev` current on this thread and initialise its primary context. */
 int eas_set_device(int dev);
+/* The calling thread's current device (what stream NULL belongs to). */
+int eas_get_device(int* dev);
 
 /* Compute capability of `dev` (e.g. 10, 0 for sm_100). */
 int eas_device_capability(int dev, int* major, int* minor);
