@@ -185,7 +185,8 @@ class Tensor:
             rt.synchronize()
         elif int(stream) != -1:
             s = int(stream)
-            rt.stream_wait_pending({1: 0, 2: 2}.get(s, s))
+            with rt.on_device(self._cuda.device):   # the consumer's default stream is that device's
+                rt.stream_wait_pending({1: 0, 2: 2}.get(s, s))
         return export_capsule(self._cuda.ptr, self._shape, self._dtype.itemsize, KDL_CUDA, self._cuda.device, self)
 
     def __dlpack_device__(self) -> tuple[int, int]:

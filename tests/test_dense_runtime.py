@@ -74,6 +74,10 @@ class Library:
         self.calls.append(("event wait", self.events[ev]))
         return 0
 
+    def eas_stream_wait_event(self, stream, ev):
+        self.calls.append(("stream waits", self.current, stream, self.events[ev]))
+        return 0
+
     def eas_stream_is_capturing(self, stream, out):
         out._obj.value = 0
         return 0
@@ -135,3 +139,11 @@ def test_scratch_grows_behind_a_wait_on_its_device(rt):
     call(1, sync=False)
     assert rt.fake.calls[:3] == [("wait", 1, 0), ("free", 1), ("launch", 1, 0)]
     rt.synchronize()
+
+
+def test_a_dlpack_consumer_waits_on_the_tensors_device(rt, monkeypatch):
+    """Its default stream (1) is the one of the device that it is given a tensor of."""
+    monkeypatch.setattr(sys.modules["easy_as_b200.tensor"], "_runtime", lambda: rt)
+    y = call(1, sync=False)[2]
+    y.__dlpack__(stream=1)
+    assert rt.fake.calls[-1] == ("stream waits", 1, 0, 1) and rt.fake.current == 0
