@@ -29,6 +29,7 @@ import hashlib
 import math
 import os
 import struct
+import threading
 from collections import deque
 from contextlib import nullcontext
 from pathlib import Path
@@ -316,6 +317,8 @@ class CudaRuntime:
         self._available: bool | None = None
         self._reason = ""
         self._pipelines: dict[tuple[str, str, int, int], int] = {}
+        # the launches under way (_track and what follows it); waits for events are outside the lock
+        self._lock = threading.RLock()
         self._pending: deque[tuple[int, int, Any, int]] = deque()
         self._max_in_flight: int | None = None
         self._staging: dict[tuple[int, int], list[DeviceBuffer]] = {}
@@ -783,18 +786,20 @@ class CudaRuntime:
     def _track(self, keep: Any, stream: int, device: int) -> None:
         """Asynchronous launch: keep the arguments alive until a completion event covers it.
         One (pooled) event per group of launches; at most EAS_MAX_IN_FLIGHT stay unfinished."""
-        if self._bucket_n and (stream != self._bucket_stream or device != self._bucket_device):
-            self._close_bucket()
-        self._bucket_keep.append(keep)
-        self._bucket_n += 1
-        self._bucket_stream = stream
-        self._bucket_device = device
         limit = self._max_flight()
-        if self._bucket_n >= (max(1, limit // 16) if limit else 64):
-            self._close_bucket()
-        while limit and self.in_flight() > limit:
-            if not self._pending:
+        with self._lock:
+            if self._bucket_n and (stream != self._bucket_stream or device != self._bucket_device):
                 self._close_bucket()
+            self._bucket_keep.append(keep)
+            self._bucket_n += 1
+            self._bucket_stream = stream
+            self._bucket_device = device
+            if self._bucket_n >= (max(1, limit // 16) if limit else 64):
+                self._close_bucket()
+        while limit and self.in_flight() > limit:
+            with self._lock:
+                if not self._pending:
+                    self._close_bucket()
             self._wait_one()
 
     # -- native operators (easy_as_b200.ops) ---------------------------------------------
@@ -993,34 +998,49 @@ class CudaRuntime:
         return True
 
     def _close_bucket(self) -> None:
-        if not self._bucket_n:
-            return
-        lib = self.lib()
-        device = self._bucket_device
-        with self.on_device(device):
-            pool = self._event_pool.get(device)
-            if pool:
-                ev = pool.pop()
-            else:
-                e = cuda_ext.ctypes.c_void_p()
-                cuda_ext.check(lib.eas_event_create(cuda_ext.ctypes.byref(e)), "event_create")
-                ev = int(e.value)
-            cuda_ext.check(lib.eas_event_record(ev, self._bucket_stream), "event_record")
-        self._pending.append((ev, self._bucket_n, self._bucket_keep, device))
-        self._pending_n += self._bucket_n
-        self._bucket_keep, self._bucket_n = [], 0
+        with self._lock:
+            if not self._bucket_n:
+                return
+            lib = self.lib()
+            device = self._bucket_device
+            with self.on_device(device):
+                pool = self._event_pool.get(device)
+                if pool:
+                    ev = pool.pop()
+                else:
+                    e = cuda_ext.ctypes.c_void_p()
+                    cuda_ext.check(lib.eas_event_create(cuda_ext.ctypes.byref(e)), "event_create")
+                    ev = int(e.value)
+                cuda_ext.check(lib.eas_event_record(ev, self._bucket_stream), "event_record")
+            self._pending.append((ev, self._bucket_n, self._bucket_keep, device))
+            self._pending_n += self._bucket_n
+            self._bucket_keep, self._bucket_n = [], 0
 
     def _wait_one(self) -> None:
-        ev, n, _keep, device = self._pending.popleft()
-        self._pending_n -= n
+        """Wait for the oldest group of launches.  It stays listed meanwhile: until its event has come, the
+        other threads' waits are for it too."""
+        with self._lock:
+            if not self._pending:
+                return
+            group = self._pending[0]
+        ev, n, _keep, device = group
         try:
             cuda_ext.check(self.lib().eas_event_synchronize(ev), "kernel execution")
         finally:
-            self._event_pool.setdefault(device, []).append(ev)
+            with self._lock:
+                if self._pending and self._pending[0] is group:   # no other thread waited for it as well
+                    self._pending.popleft()
+                    self._pending_n -= n
+                    self._event_pool.setdefault(device, []).append(ev)
 
     def synchronize(self) -> None:
-        self._close_bucket()
-        while self._pending:
+        with self._lock:
+            self._close_bucket()
+            last = self._pending[-1] if self._pending else None
+        while last is not None:
+            with self._lock:
+                if not any(group is last for group in self._pending):
+                    break
             self._wait_one()
         if self.native_launches:
             for dev in range(8):
@@ -1028,13 +1048,15 @@ class CudaRuntime:
 
     def stream_wait_pending(self, stream: int) -> None:
         """Make ``stream`` wait (device side, no host block) for every launch queued so far."""
-        self._close_bucket()
-        lib = self.lib()
-        for ev, _n, _keep, _dev in self._pending:
-            cuda_ext.check(lib.eas_stream_wait_event(stream, ev), "stream_wait_event")
+        with self._lock:
+            self._close_bucket()
+            lib = self.lib()
+            for ev, _n, _keep, _dev in self._pending:
+                cuda_ext.check(lib.eas_stream_wait_event(stream, ev), "stream_wait_event")
 
     def in_flight(self) -> int:
-        return self._pending_n + self._bucket_n
+        with self._lock:
+            return self._pending_n + self._bucket_n
 
     # -- pipelined host-buffer path ----------------------------------------------------
     PIPELINE_CHUNK_ELEMS = 1 << 23      # elements per operand per chunk (32 MiB of f32)

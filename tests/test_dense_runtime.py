@@ -2,6 +2,8 @@
 
 import ctypes
 import sys
+import threading
+import time
 
 import numpy as np
 import pytest
@@ -14,11 +16,22 @@ from easy_as_b200.tensor import Tensor
 
 class Library:
     """The entries that an operator's call needs.  A dense entry makes the operands' device current and restores the
-    one before; stream 0 is the current device's."""
+    one before; stream 0 is the current device's.  Each thread has a current device of its own."""
 
     def __init__(self, scratch=0):
-        self.current, self.calls, self.need = 0, [], scratch
+        self.calls, self.need = [], scratch
+        self.order = []   # launches and events by pointer and event
         self.events, self.buffers, self.status = {}, {}, {}
+        self.threads = threading.local()
+        self.nap = 0.0   # how long each entry lets other threads run
+
+    @property
+    def current(self):
+        return getattr(self.threads, "device", 0)
+
+    @current.setter
+    def current(self, device):
+        self.threads.device = device
 
     def eas_get_device(self, out):
         out._obj.value = self.current
@@ -34,7 +47,9 @@ class Library:
 
     def _entry(self, args, stream):
         *_pitches, _nbytes, m, n, k, dev, _dtype, _act = ops._E_LINEAR.rest.unpack(args[ops._E_LINEAR.pointers.size:])
+        time.sleep(self.nap)
         self.calls.append(("launch", dev, stream))
+        self.order.append(("launch", dev, ops._E_LINEAR.pointers.unpack_from(args)[0]))
         return 0
 
     eas_linear = _entry
@@ -60,6 +75,7 @@ class Library:
         return 0
 
     def eas_event_create(self, out):
+        time.sleep(self.nap)
         out._obj.value = len(self.events) + 1
         self.events[out._obj.value] = self.current
         return 0
@@ -68,10 +84,14 @@ class Library:
         if self.events[ev] != self.current and not stream:
             return cuda_ext.EAS_ERR_VALUE   # an event of another device
         self.calls.append(("record", self.current, stream))
+        self.order.append(("record", self.current, ev))
+        time.sleep(self.nap)
         return 0
 
     def eas_event_synchronize(self, ev):
+        time.sleep(self.nap)
         self.calls.append(("event wait", self.events[ev]))
+        self.order.append(("done", self.events[ev], ev))
         return 0
 
     def eas_stream_wait_event(self, stream, ev):
@@ -101,8 +121,8 @@ def rt(monkeypatch):
     runtime._bucket_keep, runtime._bucket_n = [], 0
 
 
-def call(device, at=0x10000000, sync=True):
-    t = [Tensor._from_cuda_ptr(at + (i << 20) + (device << 24), s, np.float16, device, owner=None)
+def call(device, at=0x10000000, sync=True, owner=None):
+    t = [Tensor._from_cuda_ptr(at + (i << 20) + (device << 24), s, np.float16, device, owner=owner)
          for i, s in enumerate([(4, 16), (8, 16), (4, 8)])]
     eas.ops.linear(*t, _sync=sync)
     return t
@@ -147,3 +167,85 @@ def test_a_dlpack_consumer_waits_on_the_tensors_device(rt, monkeypatch):
     y = call(1, sync=False)[2]
     y.__dlpack__(stream=1)
     assert rt.fake.calls[-1] == ("stream waits", 1, 0, 1) and rt.fake.current == 0
+
+
+def in_threads(count, work):
+    errors = []
+
+    def run(i):
+        try:
+            work(i)
+        except BaseException as e:  # noqa: BLE001 (shown below)
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(count)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not errors and not any(t.is_alive() for t in threads), errors
+
+
+class Owner:
+    """Memory of one call's buffers: tells when it is let go."""
+
+    def __init__(self, log, ptr):
+        self.log, self.ptr = log, ptr
+
+    def __del__(self):
+        self.log.append(("released", None, self.ptr))
+
+
+def test_threads_with_launches_under_way(rt, monkeypatch):
+    """Four threads on four devices: buffers are let go only when an event of their device, recorded behind their
+    launch, has come; the counts agree at the end, and no event is in use twice."""
+    monkeypatch.setenv("EAS_MAX_IN_FLIGHT", "8")
+    rt.fake.nap = 1e-4
+    lib, before = rt.fake, sys.getswitchinterval()
+
+    def work(device):
+        for i in range(60):
+            at = (0x100 + i) << 32
+            call(device, at, sync=False, owner=Owner(lib.order, at + (device << 24)))
+
+    sys.setswitchinterval(1e-5)
+    try:
+        in_threads(4, work)
+    finally:
+        sys.setswitchinterval(before)
+    rt.synchronize()
+    assert rt.in_flight() == 0 and rt._pending_n == 0 and not rt._pending
+    pooled = [ev for pool in rt._event_pool.values() for ev in pool]
+    assert sorted(pooled) == sorted(lib.events)
+    assert all(lib.events[ev] == device for device, pool in rt._event_pool.items() for ev in pool)
+    launched, covered, recorded = {}, set(), {}
+    for what, device, v in lib.order:
+        if what == "launch":
+            launched[v] = device
+        elif what == "record":
+            recorded[v] = {p for p, d in launched.items() if d == device}
+        elif what == "done":
+            covered |= recorded[v]
+        else:
+            assert v in covered
+            covered.discard(v)
+            del launched[v]
+    assert sum(c[0] == "released" for c in lib.order) == 240 and not launched
+
+
+def test_a_group_is_listed_until_its_event_has_come(rt):
+    """A consumer's stream that another thread makes wait meanwhile waits for it too."""
+    call(0, sync=False)
+    seen = []
+    wait = rt.fake.eas_event_synchronize
+
+    def event_synchronize(ev):
+        other = threading.Thread(target=rt.stream_wait_pending, args=(77,))
+        other.start()
+        other.join(60)
+        seen.append([c for c in rt.fake.calls if c[0] == "stream waits"])
+        return wait(ev)
+
+    rt.fake.eas_event_synchronize = event_synchronize
+    rt.synchronize()
+    assert seen == [[("stream waits", 0, 77, 0)]] and rt.in_flight() == 0
