@@ -257,16 +257,20 @@ class _Call:
             lib = rt.lib()
             need = ctypes.c_uint64()
             cuda_ext.check(lib.eas_dense_scratch(entry.op, *sizes, act, outputs, off, ctypes.byref(need)), self.what)
-            ptr, nbytes, owner = 0, need.value, None
-            if nbytes:
-                if torch is not None:   # on the launch stream: the current one of this device
-                    owner = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{device}")
-                    ptr = owner.data_ptr()
-                else:
-                    ptr, owner = rt.scratch(device, stream, self.what, nbytes)
+            nbytes, owner = need.value, None
             rest = entry.rest.pack(*(r.ld if r else 0 for r in pitched), nbytes, *sizes, device, self.dtype, act)
-            args = entry.pointers.pack(*(r.ptr if r else 0 for r in bufs), ptr) + rest
-            cuda_ext.check(getattr(lib, entry.name)(args, stream), self.what)
+            pointers = [r.ptr if r else 0 for r in bufs]
+            call = getattr(lib, entry.name)
+            if not nbytes:
+                rc = call(entry.pointers.pack(*pointers, 0) + rest, stream)
+            elif torch is not None:   # on the launch stream: the current one of this device
+                owner = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{device}")
+                rc = call(entry.pointers.pack(*pointers, owner.data_ptr()) + rest, stream)
+            else:
+                with rt.scratch_turn:
+                    ptr, owner = rt.scratch(device, stream, self.what, nbytes)
+                    rc = call(entry.pointers.pack(*pointers, ptr) + rest, stream)
+            cuda_ext.check(rc, self.what)
             keep = None
             if not (sync or capturing):
                 # buffers must outlive an asynchronous launch: torch's allocator learns which stream uses

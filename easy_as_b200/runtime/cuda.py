@@ -335,6 +335,9 @@ class CudaRuntime:
         self.launch_count = 0  # kernels launched through this runtime (generic + native)
         self.native_launches = 0  # of which pattern-lowered native kernels
         self._scratch_bufs: dict[tuple[int, int, str], DeviceBuffer] = {}
+        # held by an operator from scratch() to its last launch: what is queued on a stream uses the
+        # cached buffer of that stream one call after the other
+        self.scratch_turn = threading.Lock()
 
     def scratch(self, device: int, stream: int, tag: str, nbytes: int) -> tuple[int, Any] | None:
         """Device scratch of at least ``nbytes`` for a native launch on ``stream``: (pointer, owner);

@@ -249,3 +249,32 @@ def test_a_group_is_listed_until_its_event_has_come(rt):
     rt.fake.eas_event_synchronize = event_synchronize
     rt.synchronize()
     assert seen == [[("stream waits", 0, 77, 0)]] and rt.in_flight() == 0
+
+
+def test_threads_take_turns_with_a_streams_scratch(rt):
+    """The launches of one call are queued together: another thread's call on the stream, which has the same scratch,
+    queues its own before or behind them, and its growth does not free what is about to be used."""
+    log, need = [], threading.local()
+    entry = rt.fake._entry
+
+    def launches(args, stream):
+        scratch = ops._E_LINEAR.pointers.unpack_from(args)[-1]
+        log.append((threading.get_ident(), scratch))
+        time.sleep(1e-4)
+        assert scratch in rt.fake.buffers       # not freed meanwhile
+        log.append((threading.get_ident(), scratch))
+        return entry(args, stream)
+
+    def scratch_bytes(op, m, n, k, act, outputs, off, out):
+        out._obj.value = need.bytes
+        time.sleep(1e-5)
+        return 0
+
+    def work(i):
+        for j in range(40):
+            need.bytes = 1000 * (j // 4 + 1 + i)
+            call(0)
+
+    rt.fake.eas_linear, rt.fake.eas_dense_scratch = launches, scratch_bytes
+    in_threads(4, work)
+    assert len(log) == 320 and log[::2] == log[1::2]
