@@ -112,16 +112,17 @@ PyObject* quick(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       block[n] = reinterpret_cast<uint64_t>(scratch.get());
     }
     std::memcpy(block + n + 1, p.rest.data(), p.rest.size());
+    // Last before the launch: behind it nothing may throw, for the full path would launch again.
+    if (!sync && !capturing)  // the buffers outlive the launch wherever they were allocated
+      for (int i = 0; i < n; ++i)
+        if (tensors[i].defined())
+          c10::cuda::CUDACachingAllocator::recordStream(tensors[i].storage().data_ptr(), stream);
     int rc;
     auto* call = p.call;
     const int device = p.device;
     Py_BEGIN_ALLOW_THREADS;
     rc = call(block, stream.stream());
     Py_END_ALLOW_THREADS;
-    if (!rc && !sync && !capturing)  // the buffers outlive the launch wherever they were allocated
-      for (int i = 0; i < n; ++i)
-        if (tensors[i].defined())
-          c10::cuda::CUDACachingAllocator::recordStream(tensors[i].storage().data_ptr(), stream);
     return Py_BuildValue("iiKi", rc, device, (unsigned long long)reinterpret_cast<uintptr_t>(stream.stream()), capturing);
   } catch (const std::exception&) {
     Py_RETURN_NONE;  // a tensor without memory of its own, no memory for the scratch, ...: the full path tells

@@ -261,16 +261,6 @@ class _Call:
             rest = entry.rest.pack(*(r.ld if r else 0 for r in pitched), nbytes, *sizes, device, self.dtype, act)
             pointers = [r.ptr if r else 0 for r in bufs]
             call = getattr(lib, entry.name)
-            if not nbytes:
-                rc = call(entry.pointers.pack(*pointers, 0) + rest, stream)
-            elif torch is not None:   # on the launch stream: the current one of this device
-                owner = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{device}")
-                rc = call(entry.pointers.pack(*pointers, owner.data_ptr()) + rest, stream)
-            else:
-                with rt.scratch_turn:
-                    ptr, owner = rt.scratch(device, stream, self.what, nbytes)
-                    rc = call(entry.pointers.pack(*pointers, ptr) + rest, stream)
-            cuda_ext.check(rc, self.what)
             keep = None
             if not (sync or capturing):
                 # buffers must outlive an asynchronous launch: torch's allocator learns which stream uses
@@ -282,8 +272,18 @@ class _Call:
                     for b in held:
                         if type(b) is not Tensor:
                             b.record_stream(on)
-                elif owner is not None:
-                    keep.append(owner)
+            if not nbytes:
+                rc = call(entry.pointers.pack(*pointers, 0) + rest, stream)
+            elif torch is not None:   # on the launch stream: the current one of this device
+                owner = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{device}")
+                rc = call(entry.pointers.pack(*pointers, owner.data_ptr()) + rest, stream)
+            else:
+                with rt.scratch_turn:
+                    ptr, owner = rt.scratch(device, stream, self.what, nbytes)
+                    rc = call(entry.pointers.pack(*pointers, ptr) + rest, stream)
+            cuda_ext.check(rc, self.what)
+            if keep is not None and torch is None and owner is not None:
+                keep.append(owner)
             rt.finish_native(device, stream, keep, sync, capturing)
         if torch is not None and not self.copied and _ext is not False and (_ext or _load_ext()):
             self._leave_plan(entry, bufs, given, act, rest, nbytes)
