@@ -613,7 +613,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   }
-  if (threadIdx.x == 0 && *abort_flag && p.status) *p.status = EAS_ERR_TIMEOUT;
+  if (threadIdx.x == 0 && *abort_flag) *p.status = EAS_ERR_TIMEOUT;
 }
 
 // ---------------------------------------------------------------------------
@@ -908,7 +908,7 @@ __global__ void __launch_bounds__(kTileThreads, DEEP ? 1 : 2) dense_tile_kernel(
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(BN) : "memory");
   }
-  if (threadIdx.x == 0 && *abort_flag && p.status) *p.status = EAS_ERR_TIMEOUT;
+  if (threadIdx.x == 0 && *abort_flag) *p.status = EAS_ERR_TIMEOUT;
 }
 
 // ---------------------------------------------------------------------------
@@ -1187,6 +1187,7 @@ int dense_mma(const DenseProduct* p, int count, const DenseColSum& sums, cudaStr
   q.bf16 = p[0].bf16;
   q.sums = sums;
   q.status = eas_native_status_dev(dev);
+  if (!q.status) return eas_fail(EAS_ERR_MEMORY, "%s: no status word, in which an expired wait would be reported", who);
   if (p[0].b_mn) return launch_choice<kBackward>(c, q, dev, stream, who);
   rc = fill_epilogue(q, p[0], who);
   if (rc) return rc;

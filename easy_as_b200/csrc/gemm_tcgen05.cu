@@ -981,30 +981,45 @@ int launch_f16_choice(const F16Choice& ch, bool b_mn, bool tma_c, const CUtensor
 #undef EAS_ARGS
 }
 
-int* g_status_host = nullptr;  // host-mapped status words, one per device
-int* g_status_dev = nullptr;
-std::once_flag g_status_once;
+std::atomic<int*> g_status_host{nullptr};  // host-mapped status words, one per device
+std::atomic<int*> g_status_dev{nullptr};
+std::mutex g_status_mutex;
 
 }  // namespace
 
+// The words are allocated by the first kernel that reports to one.  That may be inside a graph capture,
+// which host allocation would invalidate in its usual mode: the capture is of the stream, and this
+// allocation is no part of it.  A failure is not remembered: the next call tries again.
 int* eas_native_status_dev(int dev) {
-  std::call_once(g_status_once, [] {
-    void* h = nullptr;
-    if (cudaHostAlloc(&h, 64 * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) == cudaSuccess) {
-      g_status_host = static_cast<int*>(h);
-      for (int i = 0; i < 64; ++i) g_status_host[i] = 0;
-      void* d = nullptr;
-      if (cudaHostGetDevicePointer(&d, h, 0) == cudaSuccess) g_status_dev = static_cast<int*>(d);
+  if (dev < 0 || dev >= 64) return nullptr;
+  if (!g_status_dev.load(std::memory_order_acquire)) {
+    std::lock_guard<std::mutex> lock(g_status_mutex);
+    if (!g_status_dev.load(std::memory_order_relaxed)) {
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      const bool relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+      void *h = nullptr, *d = nullptr;
+      if (cudaHostAlloc(&h, 64 * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) == cudaSuccess) {
+        if (cudaHostGetDevicePointer(&d, h, 0) == cudaSuccess) {
+          for (int i = 0; i < 64; ++i) static_cast<int*>(h)[i] = 0;
+          g_status_host.store(static_cast<int*>(h));
+          g_status_dev.store(static_cast<int*>(d), std::memory_order_release);
+        } else {
+          cudaFreeHost(h);
+        }
+      }
+      if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
+      cudaGetLastError();
     }
-    cudaGetLastError();
-  });
-  return (g_status_dev && dev >= 0 && dev < 64) ? g_status_dev + dev : nullptr;
+  }
+  int* words = g_status_dev.load(std::memory_order_acquire);
+  return words ? words + dev : nullptr;
 }
 
 extern "C" int eas_gemm_status(int dev, int* code) {
   if (!code) return eas_fail(EAS_ERR_VALUE, "eas_gemm_status: null pointer");
-  *code = (g_status_host && dev >= 0 && dev < 64) ? g_status_host[dev] : 0;
-  if (g_status_host && dev >= 0 && dev < 64) g_status_host[dev] = 0;
+  volatile int* words = g_status_host.load();
+  *code = (words && dev >= 0 && dev < 64) ? words[dev] : 0;
+  if (words && dev >= 0 && dev < 64) words[dev] = 0;
   return EAS_OK;
 }
 
