@@ -8,7 +8,10 @@
 //
 // A backward pass is one pass over dy (act_grad_kernel: dz, and the column sums of db) and the two
 // products.  dz, dg and du are rounded to the operands' type there: they are operands of matrix
-// products, as x and W are, and that rounding is of the size of the one that dy itself had.
+// products, as x and W are, and a matrix instruction takes 16-bit ones at this rate (a second term
+// for the remainder would double the products).  Half a step more of each operand: the error of dx and
+// dW against 64 bits grows from 1.66e-3 to 2.35e-3 in bf16.  In f16 their range would lose more than
+// that; see "the range of f16" below.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -89,6 +92,12 @@ bool vec_ok(const void* p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p)
 // Past the last value of a matrix.
 const uint16_t* past_end(const uint16_t* p, int64_t ld, int64_t rows, int64_t cols) { return p + (rows - 1) * ld + cols; }
 
+// What a block of act_grad_kernel saw of the values that it rounded to f16 (see "the range of f16").
+struct Range {
+  float largest;  // finite |value|
+  float low;      // > 0: many groups of values have no full precision
+};
+
 struct ActGrad {
   const uint16_t* dy;
   const uint16_t* g;
@@ -97,6 +106,8 @@ struct ActGrad {
   uint16_t* dg;     // dz, or dg; null when dz is dy itself (act none) and only db is wanted
   uint16_t* du;
   float* partial;   // [row blocks][N] sums of dz, or null
+  Range* range;     // [blocks], where f16 may need a scale, else null
+  float* unscale;   // what the products have to be multiplied by, then
   int64_t lddy, ldg, ldu, ldo;
   int M, N, rows_per_block;
   int row_blocks;   // the blocks behind those make copies
@@ -125,108 +136,212 @@ __device__ __forceinline__ void store8(uint16_t* p, int n, const float (&v)[8]) 
   }
 }
 
-// VEC: every array takes 16-byte accesses, so that only the last columns need other ones.  (Others are
-// gathered from aligned words.)  Four blocks per SM: the bytes under way are what the pass lives on (a gated
-// backward call of 4096 x 8192 with dWg of 64 columns alone: 73 us with three blocks, 65 with four).
+// ---- the range of f16 ----
+//
+// dz, dg and du can leave f16's range where dx and dW do not (dh = up = 300: dg would be infinite), or its
+// full precision (gradients of 1e-5 are its subnormals).  They are linear in dy, so a power of two taken
+// out of all of them and put back in the products' epilogue costs no rounding.  act_grad_kernel stores them
+// unscaled and each of its blocks notes what it saw; act_again_kernel behind it looks at all notes
+// and, where a scale is needed, makes the pass again with it.  Only sums over all blocks can choose it:
+//   the largest finite |value| is past 65504: it is brought below 2^15;
+//   of the groups of 8 neighbours that are not all zeros, more than one in 64 is below 2^-11
+//   throughout: the largest value is brought up to 2^14 (or stays).
+// Otherwise at most one group in 64 has typical values among f16's subnormals (below 2^-14), where the
+// rounding error no longer falls with the value: it stays at 2^-25, that of 2^-14.
+// act none and relu leave dy or 0, which f16 holds, and bf16 has the range of f32: neither needs this.
+// The look costs a launch: linear 777 x 1000 x 2088 takes 23.2 us with it (20.6 without), gated 613 x 1376
+// x 512 17.0 (14.1), 2048 x 4096 x 1024 70 (68), 4096 x 8192 x 4096 the same within 1 %.  Made again, with one
+// block per SM, the pass takes 5 to 100 us more (those sizes: 27, 22, 97, 890).  More blocks make it
+// faster and the look slower: with two per SM 2048 x 4096 x 1024 takes 72 and 87 us, for 70 and 97.
+
+constexpr float kLow = 0x1p-11f;
+
+// The values of one thread.
+struct RangeNotes {
+  float largest = 0;
+  int low = 0;  // 63 for each low group, -1 for each other one (2^31 rows: 2 x 63 x 2^31 / 1184 / 8 < 2^25)
+
+  __device__ __forceinline__ void add(const float (&v)[8]) {
+    float g = fabsf(v[0]);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) g = fmaxf(g, fabsf(v[j]));  // passes NaN by
+    if (g == INFINITY) {
+      g = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g = fabsf(v[j]) < INFINITY ? fmaxf(g, fabsf(v[j])) : g;
+    }
+    largest = fmaxf(largest, g);
+    low += g > 0 ? (g < kLow ? 63 : -1) : 0;
+  }
+};
+
+// Of a block's 256 threads: the largest `largest` and the sum of all `low`.
+__device__ __forceinline__ Range block_range(Range r) {
+  __shared__ Range warps[8];
+  // (the bits of values that are not negative are in their order)
+  r.largest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(r.largest)));
+#pragma unroll
+  for (int d = 16; d; d >>= 1) r.low += __shfl_xor_sync(0xffffffffu, r.low, d);
+  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = r;
+  __syncthreads();
+  r = warps[0];
+#pragma unroll
+  for (int w = 1; w < 8; ++w) r.largest = fmaxf(r.largest, warps[w].largest), r.low += warps[w].low;
+  return r;
+}
+
+// e of the scale 2^e: -18 (the largest values are below 65504^2 x 1.13 < 2^33) .. 100 (what is
+// smaller yet is 0 in every result).
+__device__ __forceinline__ int range_exponent(const Range& r) {
+  const int e = 14 - ((int)(__float_as_uint(r.largest) >> 23) - 127);
+  if (r.largest > 65504.0f) return e;
+  return r.low > 0 && e > 0 ? min(e, 100) : 0;
+}
+
+// One block's part: 256 columns of rows_per_block rows.  VEC: every array takes 16-byte accesses, so that
+// only the last columns need other ones.  (Others are gathered from aligned words.)  AGAIN: values times
+// `scale`; else notes and column sums of them unscaled.
+template <bool GATED, bool BF16, bool VEC, bool AGAIN>
+__device__ __forceinline__ void act_grad_part(const ActGrad& p, int bx, int by, float scale, float (&sum)[8],
+                                              RangeNotes& notes) {
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int n0 = (bx * 32 + tx) * 8;
+  const int cols = p.N - n0;
+  if (cols <= 0) return;
+  const int64_t r0 = (int64_t)by * p.rows_per_block;
+  const int64_t r1 = min((int64_t)p.M, r0 + p.rows_per_block);
+  with_act(p.act, [&](auto a) {
+    constexpr int ACT = decltype(a)::value;
+    constexpr bool kG = GATED || ACT != kNone;
+    constexpr bool kNotes = !BF16 && !AGAIN && (GATED || (ACT != kNone && ACT != kRelu));
+    auto put = [&](uint16_t* to, float (&v)[8]) {
+      if constexpr (kNotes) notes.add(v);
+      if constexpr (AGAIN) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= scale;
+      }
+      store8<BF16>(to, cols, v);
+    };
+    auto row = [&](int64_t m, const float (&dy)[8], const float (&g)[8], const float (&u)[8]) {
+      float o[8];
+      if constexpr (GATED) {
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float v, d;
+          act_and_slope<ACT>(g[j], v, d);
+          w[j] = dy[j] * u[j] * d;
+          o[j] = dy[j] * v;
+        }
+        put(p.dg + m * p.ldo + n0, w);
+        put(p.du + m * p.ldo + n0, o);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float v, d = 1.0f;
+          if (ACT != kNone) act_and_slope<ACT>(g[j], v, d);
+          o[j] = dy[j] * d;
+          if (!AGAIN) sum[j] += o[j];
+        }
+        if (p.dg) put(p.dg + m * p.ldo + n0, o);
+      }
+    };
+    float dy[8], g[8], u[8];
+    int64_t m = r0 + ty;
+    if (VEC && cols >= 8) {
+      // the next row's words are under way while this one is worked on
+      const int64_t sd = 8 * p.lddy, sg = 8 * p.ldg, su = 8 * p.ldu;
+      const uint16_t *pd = p.dy + m * p.lddy + n0, *pg = kG ? p.g + m * p.ldg + n0 : nullptr,
+                     *pu = GATED ? p.u + m * p.ldu + n0 : nullptr;
+      uint4 wd, wg, wu;
+      auto fetch = [&]() {
+        wd = *reinterpret_cast<const uint4*>(pd);
+        if (kG) wg = *reinterpret_cast<const uint4*>(pg);
+        if (GATED) wu = *reinterpret_cast<const uint4*>(pu);
+        pd += sd, pg += sg, pu += su;
+      };
+      if (m < r1) fetch();
+      for (; m < r1; m += 8) {
+        widen8<BF16>(wd, dy);
+        if (kG) widen8<BF16>(wg, g);
+        if (GATED) widen8<BF16>(wu, u);
+        if (m + 8 < r1) fetch();
+        row(m, dy, g, u);
+      }
+    }
+    for (; m < r1; m += 8) {
+      const uint16_t *pd = p.dy + m * p.lddy + n0, *pg = kG ? p.g + m * p.ldg + n0 : nullptr,
+                     *pu = GATED ? p.u + m * p.ldu + n0 : nullptr;
+      if constexpr (VEC) {  // the last, partial words
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          dy[j] = j < cols ? to_f32<BF16>(pd[j]) : 0.0f;
+          if (kG) g[j] = j < cols ? to_f32<BF16>(pg[j]) : 0.0f;
+          if (GATED) u[j] = j < cols ? to_f32<BF16>(pu[j]) : 0.0f;
+        }
+      } else {
+        Gather8 wd, wg, wu;
+        wd.fetch(pd, cols, p.dy, p.dy_end);
+        if (kG) wg.fetch(pg, cols, p.g, p.g_end);
+        if (GATED) wu.fetch(pu, cols, p.u, p.u_end);
+        widen8<BF16>(wd.get(), dy);
+        if (kG) widen8<BF16>(wg.get(), g);
+        if (GATED) widen8<BF16>(wu.get(), u);
+      }
+      row(m, dy, g, u);
+    }
+  });
+}
+
+// Four blocks per SM: the bytes under way are what the pass lives on (a gated backward call of 4096 x 8192
+// with dWg of 64 columns alone: 73 us with three blocks, 65 with four).
 template <bool GATED, bool BF16, bool VEC>
 __global__ void __launch_bounds__(256, 4) act_grad_kernel(const __grid_constant__ ActGrad p) {
   __shared__ float sums[8][32][9];
+  grid_order();
   if ((int)blockIdx.y >= p.row_blocks) {
-    grid_order();
     repitch(p.copies, (int64_t)(blockIdx.y - p.row_blocks) * gridDim.x + blockIdx.x,
             (int64_t)(gridDim.y - p.row_blocks) * gridDim.x);
     return;
   }
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int n0 = (blockIdx.x * 32 + tx) * 8;
-  const int cols = p.N - n0;
-  const int64_t r0 = (int64_t)blockIdx.y * p.rows_per_block;
-  const int64_t r1 = min((int64_t)p.M, r0 + p.rows_per_block);
   float sum[8] = {};
-  grid_order();
-  if (cols > 0) {
-    with_act(p.act, [&](auto a) {
-      constexpr int ACT = decltype(a)::value;
-      constexpr bool kG = GATED || ACT != kNone;
-      auto row = [&](int64_t m, const float (&dy)[8], const float (&g)[8], const float (&u)[8]) {
-        float o[8];
-        if constexpr (GATED) {
-          float w[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float v, d;
-            act_and_slope<ACT>(g[j], v, d);
-            w[j] = dy[j] * u[j] * d;
-            o[j] = dy[j] * v;
-          }
-          store8<BF16>(p.dg + m * p.ldo + n0, cols, w);
-          store8<BF16>(p.du + m * p.ldo + n0, cols, o);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float v, d = 1.0f;
-            if (ACT != kNone) act_and_slope<ACT>(g[j], v, d);
-            o[j] = dy[j] * d;
-            sum[j] += o[j];
-          }
-          if (p.dg) store8<BF16>(p.dg + m * p.ldo + n0, cols, o);
-        }
-      };
-      float dy[8], g[8], u[8];
-      int64_t m = r0 + ty;
-      if (VEC && cols >= 8) {
-        // the next row's words are under way while this one is worked on
-        const int64_t sd = 8 * p.lddy, sg = 8 * p.ldg, su = 8 * p.ldu;
-        const uint16_t *pd = p.dy + m * p.lddy + n0, *pg = kG ? p.g + m * p.ldg + n0 : nullptr,
-                       *pu = GATED ? p.u + m * p.ldu + n0 : nullptr;
-        uint4 wd, wg, wu;
-        auto fetch = [&]() {
-          wd = *reinterpret_cast<const uint4*>(pd);
-          if (kG) wg = *reinterpret_cast<const uint4*>(pg);
-          if (GATED) wu = *reinterpret_cast<const uint4*>(pu);
-          pd += sd, pg += sg, pu += su;
-        };
-        if (m < r1) fetch();
-        for (; m < r1; m += 8) {
-          widen8<BF16>(wd, dy);
-          if (kG) widen8<BF16>(wg, g);
-          if (GATED) widen8<BF16>(wu, u);
-          if (m + 8 < r1) fetch();
-          row(m, dy, g, u);
-        }
-      }
-      for (; m < r1; m += 8) {
-        const uint16_t *pd = p.dy + m * p.lddy + n0, *pg = kG ? p.g + m * p.ldg + n0 : nullptr,
-                       *pu = GATED ? p.u + m * p.ldu + n0 : nullptr;
-        if constexpr (VEC) {  // the last, partial words
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            dy[j] = j < cols ? to_f32<BF16>(pd[j]) : 0.0f;
-            if (kG) g[j] = j < cols ? to_f32<BF16>(pg[j]) : 0.0f;
-            if (GATED) u[j] = j < cols ? to_f32<BF16>(pu[j]) : 0.0f;
-          }
-        } else {
-          Gather8 wd, wg, wu;
-          wd.fetch(pd, cols, p.dy, p.dy_end);
-          if (kG) wg.fetch(pg, cols, p.g, p.g_end);
-          if (GATED) wu.fetch(pu, cols, p.u, p.u_end);
-          widen8<BF16>(wd.get(), dy);
-          if (kG) widen8<BF16>(wg.get(), g);
-          if (GATED) widen8<BF16>(wu.get(), u);
-        }
-        row(m, dy, g, u);
-      }
-    });
+  RangeNotes notes;
+  act_grad_part<GATED, BF16, VEC, false>(p, blockIdx.x, blockIdx.y, 1.0f, sum, notes);
+  if (!BF16 && p.range) {
+    const Range r = block_range({notes.largest, (float)notes.low});
+    if (threadIdx.x == 0) p.range[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = r;
   }
   if (GATED || !p.partial) return;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) sums[ty][tx][j] = sum[j];
+  for (int j = 0; j < 8; ++j) sums[threadIdx.x >> 5][threadIdx.x & 31][j] = sum[j];
   __syncthreads();
   const int c = threadIdx.x, n = blockIdx.x * 256 + c;  // one column per thread
   float s = 0;
 #pragma unroll
   for (int r = 0; r < 8; ++r) s += sums[r][c >> 3][c & 7];
   if (n < p.N) p.partial[(int64_t)blockIdx.y * p.N + n] = s;
+}
+
+// The pass again (f16), with the scale that the blocks' notes ask for; mostly they ask for none.
+template <bool GATED, bool VEC>
+__global__ void __launch_bounds__(256, 2) act_again_kernel(const __grid_constant__ ActGrad p) {
+  grid_order();
+  const int width = (p.N + 255) / 256;
+  const int64_t blocks = (int64_t)width * p.row_blocks;
+  Range all = {0, 0};
+  for (int64_t i = threadIdx.x; i < blocks; i += 256) {
+    const Range r = p.range[i];
+    all.largest = fmaxf(all.largest, r.largest);
+    all.low += r.low;
+  }
+  const int e = range_exponent(block_range(all));
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.unscale = __uint_as_float((uint32_t)(127 - e) << 23);
+  if (e == 0) return;
+  float sum[8];
+  RangeNotes notes;
+  for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x)
+    act_grad_part<GATED, false, VEC, true>(p, (int)(b % width), (int)(b / width), __uint_as_float((uint32_t)(127 + e) << 23),
+                                           sum, notes);
 }
 
 template <bool GATED>
@@ -242,8 +357,13 @@ int launch_act_grad(ActGrad& g, int blocks, cudaStream_t s, const char* who) {
                                      : reinterpret_cast<const void*>(&act_grad_kernel<GATED, false, false>));
   const int width = (g.N + 255) / 256;
   g.row_blocks = blocks;
+  const int64_t parts = (int64_t)width * blocks;
   blocks += (repitch_blocks(g.copies) + width - 1) / width;
-  return dense_launch(kernel, dim3((unsigned)width, (unsigned)blocks), 0, 256, 0, s, &g, who);
+  int rc = dense_launch(kernel, dim3((unsigned)width, (unsigned)blocks), 0, 256, 0, s, &g, who);
+  if (rc || !g.range) return rc;
+  kernel = vec ? reinterpret_cast<const void*>(&act_again_kernel<GATED, true>)
+               : reinterpret_cast<const void*>(&act_again_kernel<GATED, false>);
+  return dense_launch(kernel, dim3((unsigned)(parts < 148 ? parts : 148)), 0, 256, 0, s, &g, who);
 }
 
 // Rows per block: enough blocks for 8 per SM, at least 8 rows (one per thread row); with sums at most
@@ -319,12 +439,14 @@ enum { kDx = 1, kDw = 2, kDb = 4 };
 enum { kXOff = 1, kWOff = 2, kUpOff = 4, kDyOff = 8 };
 
 // Layout of a call's scratch: operands that TMA cannot read in place, copied into rows padded to 8
-// elements; of a backward pass also dz (or dg, du) in such rows and the partial sums of db.
+// elements; of a backward pass also dz (or dg, du) in such rows, what was seen of their range, and the
+// partial sums of db.
 struct Scratch {
-  uint64_t x = 0, w = 0, up = 0, dz = 0, dz2 = 0, partial = 0, total = 0;
+  uint64_t x = 0, w = 0, up = 0, dz = 0, dz2 = 0, partial = 0, range = 0, unscale = 0, total = 0;
   uint64_t ldk = 0, ldn = 0;  // padded pitches of rows of K and of N elements
   int rows = 0, blocks = 0;
   bool need_dz = false;
+  bool ranged = false;  // in f16: dz, dg and du may need a scale
   bool direct = false;  // db straight from dy
 
   Scratch(uint32_t N, uint32_t K) : ldk(((uint64_t)K + 7) / 8 * 8), ldn(((uint64_t)N + 7) / 8 * 8) {}
@@ -354,6 +476,11 @@ Scratch backward_scratch(bool gated, uint32_t M, uint32_t N, uint32_t K, int act
   s.need_dz = (outputs & (kDx | kDw)) && (gated || act != kNone || (off & kDyOff));
   if (s.need_dz) s.dz = s.take(2 * (uint64_t)M * s.ldn);
   if (s.need_dz && gated) s.dz2 = s.take(2 * (uint64_t)M * s.ldn);
+  s.ranged = s.need_dz && (gated || (act != kNone && act != kRelu));
+  if (s.ranged) {
+    s.range = s.take((((uint64_t)N + 255) / 256) * s.blocks * sizeof(Range));
+    s.unscale = s.take(sizeof(float));
+  }
   s.direct = (outputs & kDb) && act == kNone && !s.need_dz && M <= kDirectRows;
   if ((outputs & kDb) && !s.direct) s.partial = s.take((uint64_t)s.blocks * N * 4);
   return s;
@@ -396,7 +523,7 @@ struct Copies {
 // dx = sum_t dz_t W_t and dW_t = dz_t^T x, and db: independent of one another, so one launch.
 int backward_products(const char* who, int terms, const Operand (&dz)[2], const Operand (&w)[2], const Operand& x,
                       void* dx, uint64_t lddx, void* const (&dw)[2], const uint64_t (&lddw)[2], const DenseColSum& sums,
-                      uint32_t M, uint32_t N, uint32_t K, int dtype, cudaStream_t s) {
+                      const float* unscale, uint32_t M, uint32_t N, uint32_t K, int dtype, cudaStream_t s) {
   DenseProduct p[2];
   int count = 0;
   if (dx) {
@@ -417,7 +544,7 @@ int backward_products(const char* who, int terms, const Operand (&dz)[2], const 
     d.a_mn = true;
     d.M = (int)N, d.N = (int)K, d.K = (int)M;
   }
-  for (int i = 0; i < count; ++i) p[i].b_mn = true, p[i].bf16 = dtype == kBF16;
+  for (int i = 0; i < count; ++i) p[i].b_mn = true, p[i].bf16 = dtype == kBF16, p[i].unscale = unscale;
   return dense_mma(p, count, sums, s, who);
 }
 
@@ -584,12 +711,14 @@ extern "C" int eas_linear_backward(const eas_linear_backward_args* args, void* s
   uint8_t* base = static_cast<uint8_t*>(scratch);
   uint16_t* dz = sc.need_dz ? reinterpret_cast<uint16_t*>(base + sc.dz) : nullptr;
   float* partial = db && !sc.direct ? reinterpret_cast<float*>(base + sc.partial) : nullptr;
+  float* unscale = sc.ranged && dtype == kF16 ? reinterpret_cast<float*>(base + sc.unscale) : nullptr;
   if (dz || partial) {
     ActGrad g = {};
     g.dy = u16(dy), g.g = u16(pre), g.dg = dz, g.partial = partial;
     g.lddy = lddy, g.ldg = ldp, g.ldo = sc.ldn;
     g.M = M, g.N = N, g.rows_per_block = sc.rows, g.act = act, g.bf16 = dtype == kBF16;
     g.copies = copies.r;
+    if (unscale) g.range = reinterpret_cast<Range*>(base + sc.range), g.unscale = unscale;
     rc = launch_act_grad<false>(g, sc.blocks, s, who);
   } else {
     rc = copies.launch(s, who);
@@ -605,7 +734,8 @@ extern "C" int eas_linear_backward(const eas_linear_backward_args* args, void* s
       sums.partial = partial, sums.rows = sc.blocks;
   }
   if (!dx && !dw) return dense_column_sums(sums, s, who);
-  return backward_products(who, 1, {DZ, {}}, {W, {}}, X, dx, lddx, {dw, nullptr}, {lddw, 0}, sums, M, N, K, dtype, s);
+  return backward_products(who, 1, {DZ, {}}, {W, {}}, X, dx, lddx, {dw, nullptr}, {lddw, 0}, sums, unscale, M, N, K, dtype,
+                           s);
 }
 
 extern "C" int eas_gated_backward(const eas_gated_backward_args* args, void* stream) {
@@ -652,8 +782,10 @@ extern "C" int eas_gated_backward(const eas_gated_backward_args* args, void* str
   g.lddy = lddh, g.ldg = ldg, g.ldu = ldu, g.ldo = sc.ldn;
   g.M = M, g.N = N, g.rows_per_block = sc.rows, g.act = act, g.bf16 = dtype == kBF16;
   g.copies = copies.r;
+  float* unscale = dtype == kF16 ? reinterpret_cast<float*>(base + sc.unscale) : nullptr;
+  if (unscale) g.range = reinterpret_cast<Range*>(base + sc.range), g.unscale = unscale;
   rc = launch_act_grad<true>(g, sc.blocks, s, who);
   if (rc) return rc;
   return backward_products(who, 2, {{dg, sc.ldn}, {du, sc.ldn}}, {G, U}, X, dx, lddx, {dw_gate, dw_up},
-                           {lddwg, lddwu}, DenseColSum(), M, N, K, dtype, s);
+                           {lddwg, lddwu}, DenseColSum(), unscale, M, N, K, dtype, s);
 }

@@ -10,7 +10,7 @@
 // A_t[m][k] is at a[t] + m lda[t] + k, or at a[t] + k lda[t] + m when a_mn; B_t likewise by n.
 // Operand bases and pitches are multiples of 16 bytes; those of the other arrays are arbitrary.
 // Forward products have K-major operands (neither a_mn nor b_mn) and one term; backward ones have b_mn
-// and no epilogue.
+// and no epilogue but a factor, a power of two that was taken out of their first operands.
 struct DenseProduct {
   const uint16_t* a[2] = {nullptr, nullptr};
   const uint16_t* b[2] = {nullptr, nullptr};
@@ -24,6 +24,7 @@ struct DenseProduct {
   uint16_t* pre = nullptr;   // z, or g
   uint16_t* pre2 = nullptr;  // u
   uint64_t ldr = 0, ldy[2] = {0, 0}, ldp = 0, ldp2 = 0;
+  const float* unscale = nullptr;  // of a backward launch: all sums are multiplied by it (null: by 1)
   int act = 0;
   bool bf16 = false;
 };

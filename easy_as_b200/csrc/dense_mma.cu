@@ -48,6 +48,7 @@ struct alignas(64) Params {
   CUtensorMap pre, pre2;
   const uint16_t* bias;
   const uint16_t* residual;
+  const float* unscale;
   uint16_t* pre_ptr;
   uint16_t* pre2_ptr;
   int64_t ldr, ldp, ldp2;
@@ -355,6 +356,10 @@ __device__ __forceinline__ void finish_as(const Params& p, const Job& jb, Boxes&
       }
     });
     if (!GATED && p.residual) add_residual<BF16>(p, bx, lane, m0, n0, v);
+  } else if (!BF16 && p.unscale) {
+    const float s = *p.unscale;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] *= s;
   }
   put<BF16>(bx, lane, &jb.y[z], jb.y_tma, jb.y_ptr[z], jb.ldy[z], jb.M, jb.N, m0, n0, v);
 }
@@ -1185,6 +1190,7 @@ int dense_mma(const DenseProduct* p, int count, const DenseColSum& sums, cudaStr
   q.cluster = c.split[0] > c.split[1] ? c.split[0] : c.split[1];
   if (count == 1) q.job[1].split = 1;
   q.bf16 = p[0].bf16;
+  q.unscale = p[0].unscale;
   q.sums = sums;
   q.status = eas_native_status_dev(dev);
   if (!q.status) return eas_fail(EAS_ERR_MEMORY, "%s: no status word, in which an expired wait would be reported", who);

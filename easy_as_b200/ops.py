@@ -17,8 +17,11 @@ together as the rows (tokens); weights are ``[outputs, inputs]``.  A result must
 along its last dimension and rows that do not overlap; an input that does not is copied first.
 
 Sums are kept in f32 and every result is rounded once.  The backward passes also round ``dz``,
-``dg`` and ``du``, which are operands of matrix products, to the operands' dtype; ``dbias`` is
-summed from the unrounded values.  All results are the same bits on every run.
+``dg`` and ``du``, which are operands of matrix products, to the operands' dtype, which adds half a
+step of that dtype to the error of ``dx`` and the weights' gradients; ``dbias`` is summed from the
+unrounded values.  In f16 they are rounded times a power of two, which the results are divided by, where
+the largest of them would be infinite or many of them would have less than f16's full precision.
+All results are the same bits on every run.
 
 The calls are plain launches: torch's autograd does not see them (nor that a buffer was written),
 and gradients come from the backward calls.

@@ -381,7 +381,8 @@ int eas_gated(const eas_gated_args* args, void* stream);
 
 /* dz = dy act'(pre); dx = dz w, dw = dz^T x, db = the sum of dz's rows (each may
  * be NULL; the residual's gradient is dy itself).  pre may be NULL for act 0.
- * dz is rounded to the operands' type; db is summed from the unrounded dz. */
+ * dz is rounded to the operands' type (f16: times a power of two, which dx and dw
+ * are divided by, where its range asks for one); db is summed from the unrounded dz. */
 typedef struct {
   const void *dy, *pre, *x, *w;
   void *dx, *dw, *db, *scratch;
@@ -392,7 +393,8 @@ typedef struct {
 int eas_linear_backward(const eas_linear_backward_args* args, void* stream);
 
 /* dg = dh up act'(gate), du = dh act(gate); dx = dg w_gate + du w_up,
- * dw_gate = dg^T x, dw_up = du^T x (each may be NULL). */
+ * dw_gate = dg^T x, dw_up = du^T x (each may be NULL).  dg and du are rounded as dz
+ * is there, with one power of two for both. */
 typedef struct {
   const void *dh, *gate, *up, *x, *w_gate, *w_up;
   void *dx, *dw_gate, *dw_up, *scratch;
