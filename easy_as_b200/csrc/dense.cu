@@ -579,8 +579,9 @@ extern "C" int eas_dense_plan(int op, uint32_t M, uint32_t N, uint32_t K, int ou
     p[0].gated = gated;
     p[0].M = (int)M, p[0].N = (int)N, p[0].K = (int)K;
     if (dense_rows_fit((int)M, (int)K)) {
-      *kernel = 0, *width = gated ? 8 : 16, *split0 = dense_rows_split(p[0], num_sms), *split1 = 1;
-      *a_rows = kDenseRows, *ctas_per_sm = 2;
+      const DenseRowsShape c = dense_rows_shape(p[0], true, num_sms);
+      *kernel = 0, *width = gated ? 8 : 16, *split0 = c.split, *split1 = 1;
+      *a_rows = kDenseRows, *ctas_per_sm = 0;  // (eas_dense_rows_plan)
       return EAS_OK;
     }
   } else {
@@ -597,6 +598,22 @@ extern "C" int eas_dense_plan(int op, uint32_t M, uint32_t N, uint32_t K, int ou
   const DenseShape s = dense_shape(p, count, outputs & kDb, num_sms);
   *kernel = s.bn ? 1 : 2, *width = s.bn ? s.bn : 256, *split0 = s.split[0], *split1 = s.split[1];
   *a_rows = s.ar, *ctas_per_sm = s.bn && !s.deep ? 2 : 1;
+  return EAS_OK;
+}
+
+extern "C" int eas_dense_rows_plan(int op, uint32_t M, uint32_t N, uint32_t K, int unaligned, int num_sms, int* way,
+                                   int* warps, int* split) {
+  if (!way || !warps || !split) return eas_fail(EAS_ERR_VALUE, "eas_dense_rows_plan: null pointer");
+  if (op != 0 && op != 1) return eas_fail(EAS_ERR_VALUE, "eas_dense_rows_plan: op must be 0 or 1");
+  int rc = check_sizes("eas_dense_rows_plan", M, N, K, kF16, kNone);
+  if (rc) return rc;
+  if (M == 0 || num_sms <= 0 || !dense_rows_fit((int)M, (int)K))
+    return eas_fail(EAS_ERR_VALUE, "eas_dense_rows_plan: no product of few rows");
+  DenseProduct p;
+  p.gated = op;
+  p.M = (int)M, p.N = (int)N, p.K = (int)K;
+  const DenseRowsShape c = dense_rows_shape(p, !(unaligned & (kXOff | kWOff | (op ? kUpOff : 0))), num_sms);
+  *way = c.way, *warps = c.warps, *split = c.split;
   return EAS_OK;
 }
 

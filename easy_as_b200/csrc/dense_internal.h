@@ -58,5 +58,10 @@ DenseShape dense_shape(const DenseProduct* p, int count, bool sums, int sms);
 // rows that fit in shared memory; operands of any alignment.
 constexpr int kDenseRows = 8;
 bool dense_rows_fit(int M, int K);
-int dense_rows_split(const DenseProduct& p, int sms);
+struct DenseRowsShape {
+  int way;    // of reading W: 0 words of its rows, 1 words that are shifted, 2 values
+  int warps;  // per block: 8 (two blocks per SM) or 16
+  int split;  // CTAs of a cluster that share K
+};
+DenseRowsShape dense_rows_shape(const DenseProduct& p, bool aligned, int sms);
 int dense_rows(const DenseProduct& p, cudaStream_t stream, const char* who);

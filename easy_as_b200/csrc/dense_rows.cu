@@ -350,8 +350,17 @@ int choose_split(const DenseProduct& p, int blocks, int warps) {
   return (int64_t)p.N < (int64_t)blocks * tile / 2 && p.K >= 8 * kPiece * warps ? 2 : 1;
 }
 
+// How a product's launch is made up; `aligned`: every row of x and W starts on 16 bytes.
+DenseRowsShape choose_rows(const DenseProduct& p, bool aligned, int sms) {
+  DenseRowsShape c;
+  c.way = aligned ? kWords : (int64_t)p.N * p.K * (p.gated ? 2 : 1) < kShiftFrom ? kValues : kShifted;
+  c.warps = c.way == kValues || p.M * x_pitch(p.K) <= kMostX<8> ? 8 : 16;
+  c.split = choose_split(p, 16 / c.warps * sms, c.warps);
+  return c;
+}
+
 template <int W, bool GATED, Way WAY, bool BF16>
-int launch_rows(const DenseProduct& p, RowsParams& q, int dev, cudaStream_t s, const char* who) {
+int launch_rows(const DenseProduct& p, RowsParams& q, int split, int dev, cudaStream_t s, const char* who) {
   static bool ready[64] = {false};
   const void* kernel = reinterpret_cast<const void*>(&dense_rows_kernel<W, GATED, WAY, BF16>);
   constexpr int kQueue = Shape<W, WAY>::kQueue;
@@ -362,7 +371,7 @@ int launch_rows(const DenseProduct& p, RowsParams& q, int dev, cudaStream_t s, c
     ready[dev & 63] = true;
   }
   const int resident = 16 / W * dense_sms(dev);
-  q.split = choose_split(p, resident, W);
+  q.split = split;
   // no block without rows; four rows a block or more, where there are few
   int groups = resident / q.split;
   if (groups > (p.N + 3) / 4) groups = (p.N + 3) / 4;
@@ -371,18 +380,17 @@ int launch_rows(const DenseProduct& p, RowsParams& q, int dev, cudaStream_t s, c
 }
 
 template <int W, Way WAY>
-int launch_rows(const DenseProduct& p, RowsParams& q, int dev, cudaStream_t s, const char* who) {
+int launch_rows(const DenseProduct& p, RowsParams& q, int split, int dev, cudaStream_t s, const char* who) {
   if (p.bf16)
-    return p.gated ? launch_rows<W, true, WAY, true>(p, q, dev, s, who) : launch_rows<W, false, WAY, true>(p, q, dev, s, who);
-  return p.gated ? launch_rows<W, true, WAY, false>(p, q, dev, s, who) : launch_rows<W, false, WAY, false>(p, q, dev, s, who);
+    return p.gated ? launch_rows<W, true, WAY, true>(p, q, split, dev, s, who)
+                   : launch_rows<W, false, WAY, true>(p, q, split, dev, s, who);
+  return p.gated ? launch_rows<W, true, WAY, false>(p, q, split, dev, s, who)
+                 : launch_rows<W, false, WAY, false>(p, q, split, dev, s, who);
 }
 
 }  // namespace
 
-int dense_rows_split(const DenseProduct& p, int sms) {
-  const int warps = p.M * x_pitch(p.K) <= kMostX<8> ? 8 : 16;
-  return choose_split(p, 16 / warps * sms, warps);
-}
+DenseRowsShape dense_rows_shape(const DenseProduct& p, bool aligned, int sms) { return choose_rows(p, aligned, sms); }
 
 bool dense_rows_fit(int M, int K) { return M <= kDenseRows && M * x_pitch(K) <= kMostX<16>; }
 
@@ -398,11 +406,13 @@ int dense_rows(const DenseProduct& p, cudaStream_t stream, const char* who) {
   q.M = p.M, q.N = p.N, q.K = p.K, q.act = p.act;
   q.x_end = q.x + (q.M - 1) * q.ldx + q.K;
   for (int i = 0; i < (p.gated ? 2 : 1); ++i) q.w_end[i] = q.w[i] + (q.N - 1) * q.ldw[i] + q.K;
-  const bool vec = aligned16(p.a[0], p.M > 1 ? p.lda[0] : 0) && aligned16(p.b[0], p.N > 1 ? p.ldb[0] : 0) &&
-                   (!p.gated || aligned16(p.b[1], p.N > 1 ? p.ldb[1] : 0));
-  const bool narrow = p.M * x_pitch(p.K) <= kMostX<8>;
-  if (vec)
-    return narrow ? launch_rows<8, kWords>(p, q, dev, stream, who) : launch_rows<16, kWords>(p, q, dev, stream, who);
-  if ((int64_t)p.N * p.K * (p.gated ? 2 : 1) < kShiftFrom) return launch_rows<8, kValues>(p, q, dev, stream, who);
-  return narrow ? launch_rows<8, kShifted>(p, q, dev, stream, who) : launch_rows<16, kShifted>(p, q, dev, stream, who);
+  const bool aligned = aligned16(p.a[0], p.M > 1 ? p.lda[0] : 0) && aligned16(p.b[0], p.N > 1 ? p.ldb[0] : 0) &&
+                       (!p.gated || aligned16(p.b[1], p.N > 1 ? p.ldb[1] : 0));
+  const DenseRowsShape c = choose_rows(p, aligned, dense_sms(dev));
+  if (c.way == kValues) return launch_rows<8, kValues>(p, q, c.split, dev, stream, who);
+  if (c.way == kWords)
+    return c.warps == 8 ? launch_rows<8, kWords>(p, q, c.split, dev, stream, who)
+                        : launch_rows<16, kWords>(p, q, c.split, dev, stream, who);
+  return c.warps == 8 ? launch_rows<8, kShifted>(p, q, c.split, dev, stream, who)
+                      : launch_rows<16, kShifted>(p, q, c.split, dev, stream, who);
 }

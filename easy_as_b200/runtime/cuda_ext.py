@@ -108,6 +108,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "eas_linear_backward": (_int, [_vp, _vp]),
     "eas_gated_backward": (_int, [_vp, _vp]),
     "eas_dense_plan": (_int, [_int, *[_u32] * 3, _int, _int, *[_PINT] * 6]),
+    "eas_dense_rows_plan": (_int, [_int, *[_u32] * 3, _int, _int, *[_PINT] * 3]),
     "eas_dense_scratch": (_int, [_int, *[_u32] * 3, _int, _int, _int, ctypes.POINTER(_u64)]),
 }
 

@@ -415,9 +415,17 @@ int eas_dense_scratch(int op, uint32_t M, uint32_t N, uint32_t K, int act, int o
  * tests): *kernel 0 is the one for few rows, 1 the single-CTA tiles of 128 x
  * *width sums, 2 the CTA pairs (*width 256); *split0 and *split1 CTAs share the
  * sum of one tile (of the first and second product), *a_rows rows of the first
- * operand are staged, *ctas_per_sm is 1 or 2.  op and outputs as above. */
+ * operand are staged, *ctas_per_sm is 1 or 2 (0 for few rows, whose kernel has a
+ * plan of its own).  op and outputs as above; operands on 16 bytes. */
 int eas_dense_plan(int op, uint32_t M, uint32_t N, uint32_t K, int outputs, int num_sms, int* kernel, int* width,
                    int* split0, int* split1, int* a_rows, int* ctas_per_sm);
+
+/* How the kernel for few rows runs a forward product of that many (else
+ * EAS_ERR_VALUE): *way of reading the weights 0 words of their rows, 1 words that
+ * are shifted, 2 single values; *warps of a block 8 (two blocks per SM) or 16;
+ * *split CTAs share K.  op is 0 or 1, unaligned as in eas_dense_scratch. */
+int eas_dense_rows_plan(int op, uint32_t M, uint32_t N, uint32_t K, int unaligned, int num_sms, int* way,
+                        int* warps, int* split);
 
 /* ---- host-side fault injection (tests; no device fault is ever made; no
  *      counterpart in the reference) ---------------------------------------- */
