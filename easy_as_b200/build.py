@@ -117,7 +117,7 @@ def build_ops(verbose: bool = False, force: bool = False) -> Path | None:
 def build(verbose: bool = False, force: bool = False, ptxas_verbose: bool = False) -> Path:
     try:
         build_ops(verbose, force)
-    except (RuntimeError, OSError) as e:   # the library does not need it: eas.ops then takes its full path
+    except Exception as e:   # whatever a broken torch raises: the library does not need it, eas.ops then takes its full path
         print(f"eas_ops extension not built: {e}", file=sys.stderr)
     if not force and not needs_build():
         return LIB
