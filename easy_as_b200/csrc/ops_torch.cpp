@@ -62,7 +62,7 @@ bool make_key(long op, long act, PyObject* bufs, Key& key, at::Tensor* tensors) 
     }
     if (Py_TYPE(o) != reinterpret_cast<PyTypeObject*>(THPVariableClass) && Py_TYPE(o) != g_parameter) return false;
     const at::Tensor& t = THPVariable_Unpack(o);
-    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.has_storage()) return false;
+    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.has_storage() || t.is_neg()) return false;
     key.push_back(((int64_t)t.dim() << 32) | ((int64_t)t.scalar_type() << 16) | (int64_t)t.get_device());
     for (int64_t v : t.sizes()) key.push_back(v);
     for (int64_t v : t.strides()) key.push_back(v);

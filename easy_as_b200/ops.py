@@ -179,6 +179,11 @@ class _Call:
             raise TypeError(f"{self.what}: {name!r} must be on a CUDA device, got {v.device}")
         self.torch = torch
         self._common(name, code, v.get_device())
+        if v.is_neg():   # a view whose memory holds the negatives
+            if written:
+                raise ValueError(f"{self.what}: {name!r} is written and must not be a negative view")
+            v = v.detach().resolve_neg()
+            self.copied = True
         shape = tuple(v.shape)
         n = len(shape)
         if n == 2:

@@ -222,6 +222,7 @@ def test_nothing_is_launched_that_the_full_path_launches_again(extension):
     a, b, c = p.bufs
     for bufs in ((a, b, FakeTensor((1 << 20) + 48, (4, 8))),    # the result overlaps the first
                  (a, b, FakeTensor((3 << 20) + 2, (4, 8))),     # no 16-byte boundary
+                 (FakeTensor(1 << 20, (4, 8), neg=True), b, c),  # memory of the negatives
                  (a, b, FakeTensor(3 << 20, (4, 9))), (a, b, None), (a, b)):
         assert p.quick(bufs=bufs) is None and not p.launches
     p.world.recorded = []
