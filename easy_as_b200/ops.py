@@ -314,12 +314,14 @@ class _Call:
 
 def _share(a: _Rows, b: _Rows) -> bool:
     """Whether two row sets whose address ranges meet have an element in common (False only when both
-    lie in one pitch, side by side)."""
+    lie in one pitch, side by side; a single row lies in any)."""
     if not a.rows or not b.rows or not a.cols or not b.cols:
         return False
-    if a.rows > 1 and b.rows > 1 and a.ld == b.ld and (b.ptr - a.ptr) % 2 == 0:
-        d = ((b.ptr - a.ptr) // 2) % a.ld
-        return not (d >= a.cols and d + b.cols <= a.ld)
+    if (a.rows > 1 or b.rows > 1) and (b.ptr - a.ptr) % 2 == 0:
+        ld = a.ld if a.rows > 1 else b.ld
+        if b.rows == 1 or b.ld == ld:
+            d = ((b.ptr - a.ptr) // 2) % ld
+            return not (d >= a.cols and d + b.cols <= ld)
     return True
 
 
