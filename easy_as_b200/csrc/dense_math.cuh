@@ -77,28 +77,32 @@ __device__ __forceinline__ float act(float z) {
   return z;
 }
 
+// An infinite z is what f16 holds of a finite pre-activation past 65504: the value and the slope are the ones
+// of far values (0 and 0 to the left, where the formula's -inf x 0 is none; slope 1 to the right).
 template <int ACT>
 __device__ __forceinline__ void act_and_slope(float z, float& v, float& d) {
   v = z;
   d = 1.0f;
   float p, q;
+  // (both of them pass NaN by; p and cdf keep it)
+  const float left = fmaxf(z, -3.402823466e38f), far = fminf(left, 3.402823466e38f);
   if constexpr (ACT == kRelu) {
     v = z < 0 ? 0.0f : z;
     d = z > 0 ? 1.0f : (z <= 0 ? 0.0f : z);
   } else if constexpr (ACT == kGelu) {
     float e;
     const float cdf = normal_cdf(z, e);
-    v = z * cdf;
-    d = cdf + z * (0.39894228040143268f * e);
+    v = left * cdf;
+    d = cdf + far * (0.39894228040143268f * e);
   } else if constexpr (ACT == kGeluTanh) {
     const float z2 = fminf(z * z, 1e4f);  // past it s(z) s(-z) is 0 and the bracket must not be infinite
     logistic(kGeluC2 * z * (1.0f + kGeluA * z2), p, q);
-    v = z * p;
-    d = p + z * p * q * (kGeluC2 * (1.0f + 3.0f * kGeluA * z2));
+    v = left * p;
+    d = p + far * p * q * (kGeluC2 * (1.0f + 3.0f * kGeluA * z2));
   } else if constexpr (ACT == kSilu) {
     logistic(z, p, q);
-    v = z * p;
-    d = p * (1.0f + z * q);
+    v = left * p;
+    d = p * (1.0f + far * q);
   } else if constexpr (ACT == kSigmoid) {
     logistic(z, p, q);
     v = p;

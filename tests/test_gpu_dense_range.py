@@ -203,3 +203,35 @@ def test_each_replay_takes_its_own_scale(shape):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(o.nan_to_num(1e4), v.nan_to_num(1e4)) for o, v in zip(outs, want))
+
+
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu", "sigmoid"])
+@pytest.mark.parametrize("m", [3, 200])
+def test_pre_activations_past_f16(act, m):
+    """A pre-activation of -70000 is stored as -inf: the layer's value is 0 (sigmoid's too), and so are the gradients
+    through it; to the right the slope is 1 (sigmoid 0)."""
+    n, k = 72, 40
+    g = gen(m)
+    x, w = torch.ones(m, k, device="cuda", dtype=F16), torch.zeros(n, k, device="cuda", dtype=F16)
+    bias = normal(g, 1, n)[0]
+    w[5, 0], w[5, 1], w[9, 0], w[9, 1] = -60000, -10000, 60000, 10000
+    y, pre = torch.empty(m, n, device="cuda", dtype=F16), torch.empty(m, n, device="cuda", dtype=F16)
+    eas.ops.linear(x, w, y, bias=bias, act=act, pre=pre)
+    assert (pre[:, 5] == -float("inf")).all() and (pre[:, 9] == float("inf")).all() and (y[:, 5] == 0).all()
+    dy = normal(g, m, n)
+    db, dx, dw = torch.empty_like(bias), torch.empty_like(x), torch.empty_like(w)
+    small = normal(g, n, k)
+    eas.ops.linear_backward(dy, x, small, dx=dx, dw=dw, dbias=db, act=act, pre=pre)
+    right = torch.zeros_like(db[9]) if act == "sigmoid" else dy[:, 9].double().sum().half()
+    assert db[5] == 0 and abs(float(db[9]) - float(right)) <= 2.0 ** -10 * abs(float(right)) and db.isfinite().all()
+    assert dx.isfinite().all() and dw.isfinite().all() and (dw[5] == 0).all()
+    nan = pre.clone()
+    nan[:, 5] = float("nan")
+    eas.ops.linear_backward(dy, x, small, dbias=db, act=act, pre=nan)
+    assert db[5].isnan() and int(db.isnan().sum()) == 1
+    # gated: the gate's value is 0 there, whatever the up projection
+    dg, du = torch.empty_like(small), torch.empty_like(small)
+    gate, up = pre.clone(), normal(g, m, n)
+    gate[:, 9] = 1
+    eas.ops.gated_backward(dy, x, small, small, gate, up, dx=dx, dw_gate=dg, dw_up=du, act=act)
+    assert dx.isfinite().all() and (dg[5] == 0).all() and (du[5] == 0).all()
