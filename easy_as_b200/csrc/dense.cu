@@ -294,9 +294,10 @@ __device__ __forceinline__ void act_grad_part(const ActGrad& p, int bx, int by, 
 }
 
 // Four blocks per SM: the bytes under way are what the pass lives on (a gated backward call of 4096 x 8192
-// with dWg of 64 columns alone: 73 us with three blocks, 65 with four).
+// with dWg of 64 columns alone: 73 us with three blocks, 65 with four).  Three where the notes of gathered
+// gated values would spill at 64 registers (613 x 1375 x 512: 18.9 us, 19.4 with four).
 template <bool GATED, bool BF16, bool VEC>
-__global__ void __launch_bounds__(256, 4) act_grad_kernel(const __grid_constant__ ActGrad p) {
+__global__ void __launch_bounds__(256, GATED && !BF16 && !VEC ? 3 : 4) act_grad_kernel(const __grid_constant__ ActGrad p) {
   __shared__ float sums[8][32][9];
   grid_order();
   if ((int)blockIdx.y >= p.row_blocks) {
